@@ -84,6 +84,12 @@ SIGNATURES = {
     "hi2_inverse_factor": (_I, [_P, _P, _L, _P, _P, _Z, _P, _P]),
     "hi2_allocate_solve": (_I, [_P, _P, _I, _L, _D, _P, _P, _P]),
     "hi2_allocate_bits": (_I, [_P, _P, _I, _L, _P, _I, _P, _P]),
+    "hi2_lay_out_rows": (_I, [_P, _P, _P, _P, _P, _P, _P, _P]),
+    "hi2_stored_linear_workspace_bytes": (_Z, [_P, _I, _L]),
+    "hi2_stored_linear": (_I, [_P, _P, _I, _L, _L, _P, _I, _P, _L, _P, _L, _P, _Z, _P]),
+    "hi2_stored_experts_workspace_bytes": (_Z, [_P, _I, _L, _I]),
+    "hi2_stored_experts": (_I, [_P, _P, _P, _I, _L, _L, _P, _P, _I, _I, _P, _L, _P, _Z, _P]),
+    "hi2_route": (_I, [_P, _I, _L, _I, _L, _I, _I, _P, _I, _I, _I, _F, _P, _P, _P]),
 }
 
 _lock = threading.Lock()

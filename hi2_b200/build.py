@@ -34,6 +34,8 @@ SOURCES = [
     "hessian.cu",
     "hessian2.cu",
     "allocate.cu",
+    "stored.cu",
+    "route.cu",
 ]
 FLAGS = [
     "-gencode",

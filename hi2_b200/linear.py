@@ -1,0 +1,261 @@
+"""Products of activations with packed weights on the tensor cores (the product of hi2/format.py:242-249
+``reference_linear``, for evaluating and serving what was encoded).
+
+A packed tensor (or a stack of routed experts) is laid out once with :func:`lay_out` /
+:func:`lay_out_stack`; the layout keeps the packed size (codes and ladder parameters are only re-ordered).
+:func:`stored_linear` then multiplies activations with the fp16 reconstruction, decoded on the fly, and
+applies bias, activation and residual in the same kernel; :func:`hi2_b200.moe.stored_experts` is the
+same for a mixture layer.  bf16 activations are taken to 11 bits in the stored basis, fp16 and fp32 ones to
+22; sums are held in fp32.  Inference only: activations that require a gradient are refused.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from .format import GROUP, HI2Tensor
+from .stack import MARK, stack_dims
+
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+CHUNK = 64  # columns that a row's codes are dealt out by
+_TILE_ROWS, _GROUP_ROWS = 128, 32
+_DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+class _Struct(C.Structure):  # hi2_stored_weight
+    _fields_ = [("data", C.c_void_p), ("groups", C.c_void_p), ("rows", C.c_void_p), ("had", C.c_void_p),
+                ("inv_scale", C.c_void_p), ("status", C.c_void_p), ("experts", C.c_int64), ("rows_per_expert", C.c_int64),
+                ("groups_per_expert", C.c_int64), ("k", C.c_int64)]
+
+
+class StoredWeight:
+    """Packed rows laid out for products: ``shape`` is ``(rows, K)``, or ``(experts, rows, K)`` for a stack.
+    Made by :func:`lay_out` or :func:`lay_out_stack`; read-only, and usable on any stream of its device."""
+
+    def __init__(self, shape, stacked: bool, tensors: dict):
+        experts, rows, k = shape
+        self.shape = tuple(shape) if stacked else (rows, k)
+        self.experts, self.rows, self.k = experts, rows, k
+        self.device = tensors["data"].device
+        self._tensors = tensors
+        self._status = tensors["status"]
+        self._struct = _Struct(*(None if tensors[f] is None else tensors[f].data_ptr()
+                                 for f in ("data", "groups", "rows", "had", "inv_scale", "status")),
+                               experts, rows, tensors["groups"].shape[0] // experts, k)
+        self.arg = C.byref(self._struct)
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in self._tensors.values() if t is not None)
+
+    def check(self) -> None:
+        """Raise ``RuntimeError`` if a device-side wait of a product with this weight ever ran out (waits
+        for the device; products themselves never wait)."""
+        if int(self._status.item()):
+            raise RuntimeError("stored product: a bounded device-side wait ran out; results since then are not valid")
+
+
+def _lay_out(f: dict, experts: int, rows: int, k: int, stacked: bool, device) -> StoredWeight:
+    codes = f["codes"]
+    dev = torch.device(device) if device is not None else (
+        codes.device if codes.is_cuda else torch.device("cuda", torch.cuda.current_device()))
+    if dev.type != "cuda":
+        raise RuntimeError("hi2_b200 runs on CUDA devices only; there is no CPU path")
+    if dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
+    if rows < 1 or k < 1 or k % CHUNK:
+        raise ValueError(f"lay_out: K={k} must be a positive multiple of {CHUNK}, with at least one row")
+    with torch.cuda.device(dev):
+        return _lay_out_on(f, experts, rows, k, stacked, dev)
+
+
+def _lay_out_on(f: dict, experts: int, rows: int, k: int, stacked: bool, dev: torch.device) -> StoredWeight:
+    def up(name, dtype):
+        return _lib.upload(f[name], dev, dtype).reshape(-1)
+
+    codes, params = up("codes", torch.int32), up("blk_params", torch.uint8)
+    code_off, param_off = up("code_off", torch.int32), up("param_off", torch.int32)
+    nbits, block = up("row_nbits", torch.int64), up("row_block", torch.int64)
+    consts = _lib.upload(f["row_consts"], dev, torch.float16).reshape(-1, 3)
+    had = up("had", torch.uint8)
+    total = experts * rows
+    for name, t, n in (("row_nbits", nbits, total), ("row_block", block, total), ("row_consts", consts, 3 * total),
+                       ("code_off", code_off, total + 1), ("param_off", param_off, total + 1),
+                       ("had", had, experts * (k // GROUP))):
+        if t.numel() != n:
+            raise ValueError(f"lay_out: {name} has {t.numel()} entries, expected {n}")
+    scale = None
+    if f.get("col_scale") is not None:
+        scale = up("col_scale", torch.float32)
+        if scale.numel() != experts * k:
+            raise ValueError(f"lay_out: col_scale has {scale.numel()} entries, expected {experts * k}")
+    # everything the copies rely on, read back once
+    known = ((nbits == 2) | (nbits == 4) | (nbits == 8)) & ((block == 16) | (block == 32) | (block == 64))
+    co, po = code_off.long(), param_off.long()
+    fits = (co[1:] - co[:-1] == k * nbits // 32) & (po[1:] - po[:-1] == k // block.clamp_min(1))
+    good = torch.stack([known.all(), fits.all(), (co[0] >= 0) & (co[-1] <= codes.numel()),
+                        (po[0] >= 0) & (2 * po[-1] <= params.numel())]).tolist()
+    if not good[0]:
+        raise ValueError("lay_out: a row's code width or block size is not one of the format's")
+    if not all(good[1:]):
+        raise ValueError("lay_out: the row offsets do not fit the buffers")
+
+    # rows by (block, width), a stable order; a tile's missing rows are padding behind them
+    padded = -(-rows // _TILE_ROWS) * _TILE_ROWS
+    shift = torch.log2(block.double()).round().long() - 4       # 0, 1, 2
+    width = torch.log2(nbits.double()).round().long()           # 1, 2, 3
+    key = torch.full((experts, padded), 99, dtype=torch.int64, device=dev)
+    key[:, :rows] = (4 * shift + width).view(experts, rows)
+    key, order = torch.sort(key, dim=1, stable=True)
+    live = key < 99
+    expert = torch.arange(experts, device=dev)[:, None]
+    src = torch.where(live, expert * rows + order, torch.full_like(order, -1))
+    at = src.clamp_min(0)
+    width = torch.where(live, width[at], torch.zeros_like(order))
+    shift = torch.where(live, shift[at], torch.zeros_like(order))
+
+    # per group of 32 rows: runs of one format, code pieces of 16 bytes run by run, then the parameter pairs
+    def grouped(t):
+        return t.view(-1, _GROUP_ROWS)
+
+    lane = torch.arange(_GROUP_ROWS, device=dev).expand(experts * padded // _GROUP_ROWS, -1)
+    gk = grouped(key)
+    begins = torch.cat([torch.ones_like(gk[:, :1], dtype=torch.bool), gk[:, 1:] != gk[:, :-1]], 1)
+    start = torch.where(begins, lane, torch.zeros_like(lane)).cummax(1).values
+    run = (gk[:, :, None] == gk[:, None, :]).sum(2)             # sorted: equal keys of a group are one run
+    pieces = torch.where(grouped(live), (1 << grouped(width)) // 2, torch.zeros_like(run))
+    before = pieces.cumsum(1) - pieces
+    piece = before.gather(1, start) + lane - start
+    pair_bytes = torch.where(grouped(live), 8 >> grouped(shift), torch.zeros_like(run))
+    pair_at = 16 * pieces.sum(1, keepdim=True) + pair_bytes.cumsum(1) - pair_bytes
+    units = (16 * pieces.sum(1) + pair_bytes.sum(1) + 15) // 16  # of 16 bytes, per chunk
+    base = (units * (k // CHUNK)).cumsum(0)
+    total_units = int(base[-1].item())
+    if total_units >= 2**32:
+        raise ValueError("lay_out: more than 64 GiB of packed rows")
+    base = base - units * (k // CHUNK)
+    form = piece | (pair_at // 2) << 8 | grouped(width) << 20 | grouped(shift) << 22 | run << 24
+    form = torch.where(grouped(live), form, torch.zeros_like(form))
+    half = consts.view(torch.int16).long() & 0xFFFF
+    rows_t = torch.stack([form.reshape(-1), torch.where(live, order, torch.full_like(order, 2**32 - 1)).reshape(-1),
+                          (half[:, 0] | half[:, 1] << 16)[at].reshape(-1), half[:, 2][at].reshape(-1)], 1)
+
+    def words(t):  # the low 32 bits
+        return torch.where(t >= 2**31, t - 2**32, t).to(torch.int32).contiguous()
+
+    tensors = dict(data=torch.zeros(max(total_units, 1) * 16, dtype=torch.uint8, device=dev),
+                   groups=words(torch.stack([base, units], 1)), rows=words(rows_t), had=had.contiguous(),
+                   inv_scale=None if scale is None else scale.reciprocal(),
+                   status=torch.zeros(1, dtype=torch.int32, device=dev))
+    w = StoredWeight((experts, rows, k), stacked, tensors)
+    src = src.reshape(-1).to(torch.int32)
+    _lib.call("hi2_lay_out_rows", w.arg, _lib.ptr(src), _lib.ptr(codes), _lib.ptr(code_off), _lib.ptr(params),
+              _lib.ptr(param_off), _lib.ptr(tensors["data"]), _lib.stream(dev))
+    torch.cuda.current_stream(dev).synchronize()  # complete for every stream that uses it later
+    return w
+
+
+def lay_out(t: HI2Tensor, device=None) -> StoredWeight:
+    """The packed tensor laid out for :func:`stored_linear` on ``device`` (default: where its codes are,
+    else the current device).  Waits for the device."""
+    fields = {name: getattr(t, name) for name in ("codes", "code_off", "blk_params", "param_off", "row_consts", "row_nbits",
+                                                  "row_block", "had", "col_scale")}
+    return _lay_out(fields, 1, int(t.shape[0]), int(t.shape[1]), False, device)
+
+
+def lay_out_stack(arrays: dict, parts: int, device=None) -> StoredWeight:
+    """The arrays of :func:`hi2_b200.stack.build_stack` with ``parts`` parts per expert (2: gate and up,
+    1: down) laid out for :func:`hi2_b200.moe.stored_experts`.  The parts of all experts must have the same
+    number of rows.  Waits for the device."""
+    experts, k = stack_dims(arrays, parts)
+    ends = arrays[MARK].to("cpu", torch.int64)
+    rows = ends[1:] - ends[:-1]
+    if experts == 0 or int(ends[0]) != 0 or not bool((rows == rows[0]).all()):
+        raise ValueError("lay_out_stack: the parts of the stack differ in their number of rows")
+    return _lay_out(arrays, experts, parts * int(rows[0]), k, True, device)
+
+
+def _activation(name) -> int:
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation {name!r} is not one of {', '.join(map(str, ACTIVATIONS))}") from None
+
+
+def _rows_of(x: torch.Tensor, k: int, what: str) -> torch.Tensor:
+    """``x`` as ``[tokens, k]`` with unit column stride (a copy only where the strides ask for one)."""
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"{what}: unsupported dtype {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"{what}: the last dimension must be {k}, got shape {tuple(x.shape)}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: there is no gradient; call it under torch.no_grad()")
+    x = x if x.dim() == 2 else x.reshape(-1, k)
+    return x if x.stride(1) == 1 else x.contiguous()
+
+
+def _output(out, shape, like: torch.Tensor, what: str):
+    """``(result, its rows [tokens, n])``: fresh, or the caller's ``out``."""
+    if out is None:
+        out = torch.empty(shape, dtype=like.dtype, device=like.device)
+        return out, out.view(-1, shape[-1])
+    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{what}: out must have shape {tuple(shape)}, the dtype and the device of the activations")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: there is no gradient; call it under torch.no_grad()")
+    if out.numel() and out.stride(-1) != 1 and out.shape[-1] != 1:
+        raise ValueError(f"{what}: out must have unit column stride")
+    try:
+        rows = out.view(-1, shape[-1])
+    except RuntimeError:
+        raise ValueError(f"{what}: the rows of out must lie at one stride") from None
+    if rows.shape[0] > 1 and rows.stride(0) < shape[-1]:
+        raise ValueError(f"{what}: the rows of out overlap")
+    return out, rows
+
+
+def stored_linear(x: torch.Tensor, w: StoredWeight, bias: torch.Tensor | None = None, activation: str | None = None,
+                  residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``activation(x @ W^T + bias) + residual`` with the packed weight ``w`` (``[rows, K]``), as ``[..., rows]`` in
+    the dtype of ``x [..., K]`` (bf16, fp16 or fp32, any strides).  ``activation`` is None, ``"relu"``, ``"silu"``,
+    ``"gelu"`` or ``"gelu_tanh"``; ``bias [rows]`` and ``residual [..., rows]`` have the dtype of ``x``.
+    ``out`` may be given, and may be ``residual``.  Queued on the current stream of the weight's device; a token with a
+    non-finite activation gets non-finite outputs and leaves the others alone."""
+    if w.experts != 1 or len(w.shape) != 2:
+        raise ValueError("stored_linear: a stack of experts goes through moe.stored_experts")
+    act = _activation(activation)
+    rows = _rows_of(x, w.k, "stored_linear")
+    dev = _lib.need_cuda(x, bias, residual, out)
+    if dev != w.device:
+        raise RuntimeError(f"tensors on different devices: {dev} and {w.device}")
+    n, tokens = w.rows, rows.shape[0]
+    shape = (*x.shape[:-1], n)
+    for name, t, want in (("bias", bias, (n,)), ("residual", residual, shape)):
+        if t is None:
+            continue
+        if tuple(t.shape) != want or t.dtype != x.dtype:
+            raise ValueError(f"stored_linear: {name} must have shape {want} and dtype {x.dtype}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("stored_linear: there is no gradient; call it under torch.no_grad()")
+    y, y_rows = _output(out, shape, x, "stored_linear")
+    if tokens == 0:
+        return y
+    if bias is not None:
+        bias = bias.contiguous()
+    res = None
+    if residual is not None:
+        res = residual if residual.dim() == 2 else residual.reshape(-1, n)
+        res = res if res.stride(1) == 1 else res.contiguous()
+    dtype = _DTYPES[x.dtype]
+    need = _lib.load().hi2_stored_linear_workspace_bytes(w.arg, dtype, tokens)
+    space = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.call("hi2_stored_linear", w.arg, rows.data_ptr(), dtype, tokens, rows.stride(0), _lib.ptr(bias), act, _lib.ptr(res),
+              0 if res is None else res.stride(0), y_rows.data_ptr(), y_rows.stride(0), space.data_ptr(), need,
+              _lib.stream(dev))
+    return y
+
+
+__all__ = ["ACTIVATIONS", "StoredWeight", "lay_out", "lay_out_stack", "stored_linear"]

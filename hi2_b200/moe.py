@@ -16,6 +16,7 @@ import re
 import torch
 from torch import nn
 
+from . import _lib
 from .hessian import HessianStats
 from .stats import ColumnStats
 
@@ -214,6 +215,99 @@ def unfuse_experts(model: nn.Module) -> int:
     return len(names)
 
 
+# ---- routing, and the call of routed experts over packed weights -----------------------------------------
+def route(logits: torch.Tensor, top_k: int, scores: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
+          top_groups: int | None = None, renormalise: bool = False, scale: float = 1.0):
+    """``(index, weight)`` as ``[..., top_k]`` int64 and fp32: the experts of every row of ``logits [..., experts]`` (fp32,
+    fp16 or bf16), best first, and their weights; the inputs of a fused-experts call.
+
+    ``scores`` is ``"softmax"`` (over the row) or ``"sigmoid"``.  ``bias [experts]`` (fp32) is added for the choice
+    only.  With ``groups > 1`` the experts form equal groups in order, a group counts with the sum of its two best
+    biased scores, and only the ``top_groups`` best are open.  Equal keys go to the lowest index.  The weight is the
+    score, over the sum of the chosen ones with ``renormalise`` (at least 1e-20), times ``scale``.  A logit or a bias that is ``-inf`` or NaN
+    closes its expert for the row (it takes no part in the softmax either); slots that no open expert is left for (all of them, in a row without any) get index
+    -1 and weight 0, which :func:`stored_experts` passes over.  At most 1024 experts, 32 groups and ``top_k`` 32."""
+    if scores not in ("softmax", "sigmoid"):
+        raise ValueError(f"route: scores must be 'softmax' or 'sigmoid', not {scores!r}")
+    from .linear import _rows_of
+
+    if logits.dim() < 1:
+        raise ValueError("route: logits must have a dimension of experts")
+    experts = logits.shape[-1]
+    rows = _rows_of(logits, experts, "route")
+    dev = _lib.need_cuda(logits, bias)
+    if bias is not None and (tuple(bias.shape) != (experts,) or bias.dtype != torch.float32):
+        raise ValueError(f"route: bias must be a float32 tensor of shape ({experts},)")
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise ValueError("route: there is no gradient; call it under torch.no_grad()")
+    shape = (*logits.shape[:-1], int(top_k))
+    if top_k < 1 or top_k > experts:
+        raise ValueError(f"route: top_k={top_k} of {experts} experts")
+    index = torch.empty(shape, dtype=torch.int64, device=dev)
+    weight = torch.empty(shape, dtype=torch.float32, device=dev)
+    if bias is not None:
+        bias = bias.contiguous()
+    _lib.call("hi2_route", rows.data_ptr(), _lib.DTYPES[rows.dtype], rows.shape[0], experts, rows.stride(0), int(top_k),
+              1 if scores == "sigmoid" else 0, _lib.ptr(bias), int(groups), int(groups if top_groups is None else top_groups),
+              1 if renormalise else 0, float(scale), index.data_ptr(), weight.data_ptr(), _lib.stream(dev))
+    return index, weight
+
+
+def stored_experts(x: torch.Tensor, index: torch.Tensor, weight: torch.Tensor, gate_up, down, activation: str | None = "silu",
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """``sum_j weight[t, j] * down_e(activation(gate_e(x_t)) * up_e(x_t))`` with ``e = index[t, j]``, as ``[..., hidden]`` in the
+    dtype of ``x [..., hidden]`` (bf16, fp16 or fp32): the call of :class:`ExpertViews` over stacks of packed
+    weights (``gate_up``, ``down``: :func:`hi2_b200.linear.lay_out_stack` with 2 and 1 parts).  ``index`` and ``weight`` are
+    ``[..., top_k]`` as :func:`route` gives them; a slot whose index is not an expert's (-1) adds nothing.  The
+    slots of a token are added in their order: equal inputs give equal bits.  Queued on the current stream; nothing
+    is read back."""
+    from .linear import _DTYPES, _activation, _output, _rows_of
+
+    if len(gate_up.shape) != 3 or len(down.shape) != 3 or gate_up.experts != down.experts or gate_up.k != down.rows or (
+            gate_up.rows != 2 * down.k):
+        raise ValueError(f"stored_experts: stacks {gate_up.shape} and {down.shape} are not the gate/up and down of one layer")
+    act = _activation(activation)
+    rows = _rows_of(x, gate_up.k, "stored_experts")
+    dev = _lib.need_cuda(x, index, weight, out)
+    if dev != gate_up.device or dev != down.device:
+        raise RuntimeError(f"tensors on different devices: {dev}, {gate_up.device} and {down.device}")
+    if index.shape != weight.shape or index.dim() != x.dim() or index.shape[:-1] != x.shape[:-1] or index.shape[-1] < 1:
+        raise ValueError("stored_experts: index and weight must be [..., top_k] over the rows of x")
+    if index.dtype not in (torch.int64, torch.int32) or weight.dtype not in _DTYPES:
+        raise ValueError("stored_experts: index must hold integers, weight fp32, fp16 or bf16")
+    if weight.requires_grad and torch.is_grad_enabled():
+        raise ValueError("stored_experts: there is no gradient; call it under torch.no_grad()")
+    y, y_rows = _output(out, tuple(x.shape), x, "stored_experts")
+    tokens, top_k = rows.shape[0], index.shape[-1]
+    if tokens == 0:
+        return y
+    index, weight = index.to(torch.int64).contiguous(), weight.to(torch.float32).contiguous()
+    dtype = _DTYPES[x.dtype]
+    need = _lib.load().hi2_stored_experts_workspace_bytes(gate_up.arg, dtype, tokens, top_k)
+    space = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.call("hi2_stored_experts", gate_up.arg, down.arg, rows.data_ptr(), dtype, tokens, rows.stride(0), index.data_ptr(),
+              weight.data_ptr(), top_k, act, y_rows.data_ptr(), y_rows.stride(0), space.data_ptr(), need, _lib.stream(dev))
+    return y
+
+
+class StoredExperts(nn.Module):
+    """Drop-in for a fused-experts module (as :class:`ExpertViews`) over stacks of packed weights: the call
+    ``(hidden_states, top_k_index, top_k_weights)``.  ``gate_up`` and ``down`` are laid-out stacks."""
+
+    def __init__(self, gate_up, down, activation: str | None = "silu"):
+        super().__init__()
+        self.gate_up, self.down, self.activation = gate_up, down, activation
+
+    def __len__(self) -> int:
+        return self.gate_up.experts
+
+    def forward(self, hidden_states, top_k_index, top_k_weights):
+        slots = top_k_index.shape[-1]
+        y = stored_experts(hidden_states.reshape(-1, hidden_states.shape[-1]), top_k_index.reshape(-1, slots),
+                           top_k_weights.reshape(-1, slots), self.gate_up, self.down, self.activation)
+        return y.reshape(hidden_states.shape)
+
+
 def expert_weights(tables: dict, share_floor: float = 0.05) -> dict:
     """Allocation multiplier of every expert tensor (hi2/moe.py:188-207): an expert's share of its
     group's calibration tokens relative to an even split, floored at ``share_floor``, divided by
@@ -233,4 +327,5 @@ def expert_weights(tables: dict, share_floor: float = 0.05) -> dict:
 
 
 __all__ = ["expert_parts", "group_key", "sibling_leader", "blend", "accumulate_routed", "top_up",
-           "expert_weights", "coverage", "is_fused_experts", "ExpertViews", "unfuse_experts", "HessianStats", "ColumnStats"]
+           "expert_weights", "coverage", "is_fused_experts", "ExpertViews", "unfuse_experts", "route", "stored_experts",
+           "StoredExperts", "HessianStats", "ColumnStats"]

@@ -329,6 +329,63 @@ int hi2_allocate_solve(const double* cost, const double* bits, int n_cand, int64
 int hi2_allocate_bits(const double* cost, const double* bits, int n_cand, int64_t n_rows,
                       const double* lams_host, int n_lams, double* totals, void* stream);
 
+/* ---- products with packed weights ------------------------------------------------------------
+ * A packed tensor, or a stack of `experts` of them with rows_per_expert rows each, laid out for products
+ * (hi2_lay_out_rows).  This struct lives in HOST memory; its pointers are device pointers.  `rows` holds
+ * four words per sorted row (form, output row, lo constants, step scale), `groups` two per 32 sorted rows
+ * (first 16-byte unit of the group's data, 16-byte units per 64 columns); groups_per_expert is a multiple
+ * of 4.  had [experts, k/16], inv_scale fp32 [experts, k] (reciprocal smoothing vector; null: none).
+ * status: a device int that a bounded wait which ran out raises and nothing clears. */
+typedef struct {
+  const void* data;
+  const uint32_t* groups;
+  const uint32_t* rows;
+  const uint8_t* had;
+  const float* inv_scale;
+  int32_t* status;
+  int64_t experts, rows_per_expert, groups_per_expert, k;
+} hi2_stored_weight;
+
+enum { HI2_ACT_NONE = 0, HI2_ACT_RELU = 1, HI2_ACT_SILU = 2, HI2_ACT_GELU = 3, HI2_ACT_GELU_TANH = 4 };
+
+/* Fill `data` (zeroed by the caller) from the flat buffers of the format: sorted row i is row
+ * src_row[i] of the flat buffers (negative: padding), its place given by w->rows and w->groups.
+ * No counterpart in the reference: its decode kernels live in the inference engine. */
+int hi2_lay_out_rows(const hi2_stored_weight* w_host, const int32_t* src_row, const int32_t* codes,
+                     const int32_t* code_off, const uint8_t* blk_params, const int32_t* param_off, void* data,
+                     void* stream);
+
+/* hi2/format.py:242-249 reference_linear with an epilogue, on tensor cores:
+ * out[m, n] = act(x' @ W^T + bias) + residual, x' the smoothed and rotated activations, W the fp16
+ * reconstruction in the stored basis (w->experts is 1).  x [tokens, k] with row stride ldx; bias [n] and residual
+ * [tokens, n] (row stride ld_residual) may be null; out [tokens, n] with row stride ld_out.  dtype (F32, F16 or
+ * BF16) is that of x, bias, residual and out.  out may be residual. */
+size_t hi2_stored_linear_workspace_bytes(const hi2_stored_weight* w_host, int dtype, int64_t tokens);
+int hi2_stored_linear(const hi2_stored_weight* w_host, const void* x, int dtype, int64_t tokens, int64_t ldx,
+                      const void* bias, int act, const void* residual, int64_t ld_residual, void* out, int64_t ld_out,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* The routed experts of a mixture layer over stacks of packed weights (the call of a fused-experts module,
+ * hi2/moe.py:53-121): out[t] = sum_j weight[t, j] * down_e(act(gate_e(x[t])) * up_e(x[t])) with
+ * e = index[t, j]; a slot whose index lies outside 0 .. experts - 1 adds nothing.  gate_up has 2 I rows per
+ * expert (gate first) over k = hidden columns, down `hidden` rows over I.  x [tokens, hidden] with row stride ldx,
+ * index int64 and weight fp32 [tokens, top_k] contiguous, out [tokens, hidden] with row stride ld_out. */
+size_t hi2_stored_experts_workspace_bytes(const hi2_stored_weight* gate_up_host, int dtype, int64_t tokens, int top_k);
+int hi2_stored_experts(const hi2_stored_weight* gate_up_host, const hi2_stored_weight* down_host, const void* x,
+                       int dtype, int64_t tokens, int64_t ldx, const int64_t* index, const float* weight, int top_k,
+                       int act, void* out, int64_t ld_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Routing: the top_k experts of every row of logits [tokens, experts] (row stride ld) and their weights.
+ * score = softmax over the row (sigmoid = 0) or sigmoid; the choice goes by score + bias (fp32 [experts], may be
+ * null).  With groups > 1 the experts form that many equal groups, a group counts with the sum of its two
+ * best biased scores, and only the top_groups best groups are open.  Ties go to the lowest index.  weight =
+ * score (over the sum of the chosen ones, with renormalise) * scale.  A logit of -inf or NaN (and a bias of
+ * -inf or NaN) closes an expert; slots that no open expert is left for get index -1 and weight 0.
+ * experts <= 1024, top_k <= min(experts, 32), groups <= 32. */
+int hi2_route(const void* logits, int dtype, int64_t tokens, int experts, int64_t ld, int top_k, int sigmoid,
+              const float* bias, int groups, int top_groups, int renormalise, float scale, int64_t* index,
+              float* weight, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
