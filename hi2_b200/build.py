@@ -35,6 +35,7 @@ SOURCES = [
     "hessian2.cu",
     "allocate.cu",
     "stored.cu",
+    "stored_mma.cu",
     "route.cu",
 ]
 FLAGS = [

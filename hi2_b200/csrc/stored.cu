@@ -267,48 +267,6 @@ combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ row_of, 
   }
 }
 
-// ---- the product, in its simplest form ------------------------------------------------------------------
-constexpr int SIMPLE_TOKENS = 8;
-
-// A lane decodes its row chunk by chunk and multiplies with eight activation rows in fp32.
-__global__ void __launch_bounds__(TILE_ROWS)
-simple_product_kernel(const Product p) {
-  TokenTile tile;
-  if (!p.tiles.get(blockIdx.y, tile)) return;
-  const int64_t group = (int64_t)tile.expert * p.w.groups_per_expert + blockIdx.x * 4 + (threadIdx.x >> 5);
-  const RowForm row = load_row(p.w.rows, group * GROUP_ROWS + (threadIdx.x & 31));
-  const float lo_min = __half2float(__ushort_as_half((uint16_t)row.lo_consts));
-  const float lo_scale = __half2float(__ushort_as_half((uint16_t)(row.lo_consts >> 16)));
-  const float step_scale = __half2float(__ushort_as_half((uint16_t)row.step_scale));
-  const uint8_t* slab = static_cast<const uint8_t*>(p.w.data) + (int64_t)p.w.groups[2 * group] * 16;
-  const int64_t slab_bytes = (int64_t)p.w.groups[2 * group + 1] * 16;
-  for (int first = tile.begin; first < tile.end; first += SIMPLE_TOKENS) {
-    float acc[SIMPLE_TOKENS];
-#pragma unroll
-    for (int t = 0; t < SIMPLE_TOKENS; ++t) acc[t] = 0.0f;
-    for (int64_t c = 0; c < p.w.k / CHUNK; ++c) {
-      uint32_t v[CHUNK / 2];
-      decode_chunk(slab + c * slab_bytes, row, lo_min, lo_scale, step_scale, v);
-      for (int part = 0; part < p.parts; ++part)
-#pragma unroll
-        for (int t = 0; t < SIMPLE_TOKENS; ++t) {
-          if (first + t >= tile.end) continue;
-          const __half2* x = reinterpret_cast<const __half2*>(p.xs + (part * p.x_rows + first + t) * p.w.k + c * CHUNK);
-#pragma unroll
-          for (int i = 0; i < CHUNK / 2; ++i) {
-            const float2 a = __half22float2(half2_of(v[i])), b = __half22float2(x[i]);
-            acc[t] = fmaf(a.x, b.x, acc[t]);
-            acc[t] = fmaf(a.y, b.y, acc[t]);
-          }
-        }
-    }
-    if (row.out_row == NO_ROW) continue;
-#pragma unroll
-    for (int t = 0; t < SIMPLE_TOKENS; ++t)
-      if (first + t < tile.end) p.out.put(first + t, row.out_row, p.out.scale_of(first + t), acc[t]);
-  }
-}
-
 inline size_t pad256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Carves the caller's workspace.
@@ -352,7 +310,7 @@ struct ExpertSpace {
     tile_count = used == nullptr ? nullptr : used + 32;
     pair_of = c.take<int32_t>(pairs);
     row_of = c.take<int32_t>(pairs);
-    tiles = c.take<TokenTile>(pairs / SIMPLE_TOKENS + gate_up.experts + 1);
+    tiles = c.take<TokenTile>(pairs / 16 + gate_up.experts + 1);
     x_scale = c.take<float>(pairs);
     h_scale = c.take<float>(pairs);
     xs = c.take<__half>(pairs * hidden * parts_of(dtype));
@@ -381,12 +339,6 @@ bool complete(const hi2_stored_weight* w) {
 bool known_dtype(int dtype) { return dtype == HI2_F32 || dtype == HI2_F16 || dtype == HI2_BF16; }
 
 }  // namespace
-
-int product_simple(const Product& p, cudaStream_t stream) {
-  const dim3 grid((unsigned)(p.w.groups_per_expert / 4), (unsigned)p.max_tiles);
-  simple_product_kernel<<<grid, TILE_ROWS, 0, stream>>>(p);
-  return check_launch("stored: product");
-}
 
 }  // namespace stored
 }  // namespace hi2
@@ -419,7 +371,7 @@ extern "C" int hi2_stored_linear(const hi2_stored_weight* w, const void* x, int 
   HI2_REQUIRE(w->experts == 1, "stored_linear: a stack of experts has no single product");
   HI2_REQUIRE(known_dtype(dtype), "stored_linear: activations must be fp32, fp16 or bf16");
   HI2_REQUIRE(act >= HI2_ACT_NONE && act <= HI2_ACT_GELU_TANH, "stored_linear: unknown activation");
-  HI2_REQUIRE(tokens >= 0 && tokens < (int64_t)1 << 31, "stored_linear: too many tokens");
+  HI2_REQUIRE(tokens >= 0 && tokens < (int64_t)1 << 30, "stored_linear: too many tokens");
   if (tokens == 0) return HI2_OK;
   HI2_REQUIRE(x && out, "stored_linear: null pointer");
   const LinearSpace space(workspace, *w, dtype, tokens);
@@ -429,12 +381,10 @@ extern "C" int hi2_stored_linear(const hi2_stored_weight* w, const void* x, int 
   Source src{x, ldx, HI2_ACT_NONE, rows_aligned(x, ldx, dtype), nullptr, nullptr, nullptr, 1};
   int rc = prepare<false>(src, *w, dtype, tokens, parts_of(dtype), space.xs, space.scale, s);
   if (rc != HI2_OK) return rc;
-  Product p{*w, space.xs, tokens, parts_of(dtype), Tiles{nullptr, nullptr, tokens, SIMPLE_TOKENS}, 0,
-            Epilogue{space.scale, nullptr, nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}};
-  // a column of the grid holds 65535 blocks: wider tiles where there are more tokens than that takes
-  while (ceil_div(tokens, (int64_t)p.tiles.width) > 65535) p.tiles.width *= 2;
-  p.max_tiles = ceil_div(tokens, (int64_t)p.tiles.width);
-  return product_simple(p, s);
+  const int width = tile_width(tokens);
+  const Product p{*w, space.xs, tokens, parts_of(dtype), Tiles{nullptr, nullptr, tokens, width}, ceil_div(tokens, (int64_t)width),
+                  Epilogue{space.scale, nullptr, nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}};
+  return product(p, s, "stored_linear");
 }
 
 extern "C" size_t hi2_stored_experts_workspace_bytes(const hi2_stored_weight* gate_up, int dtype, int64_t tokens, int top_k) {
@@ -452,7 +402,8 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   HI2_REQUIRE(gate_up->experts <= MAX_EXPERTS, "stored_experts: more than 1024 experts");
   HI2_REQUIRE(known_dtype(dtype), "stored_experts: activations must be fp32, fp16 or bf16");
   HI2_REQUIRE(act >= HI2_ACT_NONE && act <= HI2_ACT_GELU_TANH, "stored_experts: unknown activation");
-  HI2_REQUIRE(tokens >= 0 && top_k >= 1 && tokens * top_k < (int64_t)1 << 31, "stored_experts: too many (token, slot) pairs");
+  HI2_REQUIRE(tokens >= 0 && top_k >= 1 && tokens < (int64_t)1 << 30 &&
+                  tokens * top_k < (int64_t)1 << 30, "stored_experts: too many (token, slot) pairs");
   if (tokens == 0) return HI2_OK;
   HI2_REQUIRE(x && index && weight && out, "stored_experts: null pointer");
   const ExpertSpace space(workspace, *gate_up, dtype, tokens, top_k);
@@ -461,8 +412,9 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t pairs = tokens * top_k, hidden = gate_up->k, inner = down->k;
   const int experts = (int)gate_up->experts, parts = parts_of(dtype);
-  int width = SIMPLE_TOKENS;
-  while (pairs / width + experts + 1 > 65535) width *= 2;
+  // tiles wide enough for an expert with half as many tokens again as the average one
+  const int64_t busy = ceil_div(3 * pairs, (int64_t)(2 * experts));
+  const int width = tile_width(busy < pairs ? busy : pairs);
   const size_t smem = (size_t)SORT_WARPS * experts * sizeof(int32_t);
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(dispatch_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
@@ -478,14 +430,14 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   const Tiles tiles{space.tile_count, space.tiles, pairs, width};
   Product p{*gate_up, space.xs, pairs, parts, tiles, max_tiles,
             Epilogue{space.x_scale, space.pair_of, nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}};
-  rc = product_simple(p, s);
+  rc = product(p, s, "stored_experts");
   if (rc != HI2_OK) return rc;
   src = Source{space.z, 2 * inner, act, true, space.pair_of, index, space.used, top_k};
   rc = prepare<true>(src, *down, dtype, pairs, parts, space.hs, space.h_scale, s);
   if (rc != HI2_OK) return rc;
   p = Product{*down, space.hs, pairs, parts, tiles, max_tiles,
               Epilogue{space.h_scale, space.pair_of, weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}};
-  rc = product_simple(p, s);
+  rc = product(p, s, "stored_experts");
   if (rc != HI2_OK) return rc;
   int64_t blocks = ceil_div(tokens * (hidden / 4), (int64_t)256);
   if (blocks > 148 * 16) blocks = 148 * 16;

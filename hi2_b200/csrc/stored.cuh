@@ -197,7 +197,8 @@ struct Product {
   int64_t max_tiles;
   Epilogue out;
 };
-int product_simple(const Product& p, cudaStream_t stream);
+int tile_width(int64_t rows);  // of a tile, for that many activation rows of one tensor
+int product(const Product& p, cudaStream_t stream, const char* what);
 
 }  // namespace stored
 }  // namespace hi2

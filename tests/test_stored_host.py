@@ -49,7 +49,7 @@ def test_stored_experts_arguments():
         assert call(a, b) == _lib.ERR_ARG
     big = [_struct(experts=1025, rows_per_expert=128, k=128), _struct(experts=1025, rows_per_expert=128, k=64)]
     assert call(*big) == _lib.ERR_ARG
-    for kw in (dict(top_k=0), dict(tokens=-1), dict(tokens=1 << 30, top_k=2), dict(dtype=_lib.F64), dict(act=9), dict(index=None)):
+    for kw in (dict(top_k=0), dict(tokens=-1), dict(tokens=1 << 29, top_k=2), dict(dtype=_lib.F64), dict(act=9), dict(index=None)):
         assert call(up, down, **kw) == _lib.ERR_ARG
     need = lib.hi2_stored_experts_workspace_bytes(C.byref(up), _lib.F32, 3, 2)
     assert need > 0
