@@ -35,7 +35,8 @@ SOURCES = [
     "hessian2.cu",
     "allocate.cu",
     "stored.cu",
-    "stored_mma.cu",
+    "stored_few.cu",
+    "stored_wide.cu",
     "route.cu",
 ]
 FLAGS = [

@@ -7,6 +7,8 @@
 // in the flagged groups.  x' is formed in fp32 and rounded to fp16 once, relative to a power of two that
 // takes the row's largest value to [2^14, 2^15): 11 bits for every value within 2^-29 of that.  bf16 calls
 // (8 bits) take that one part; fp16 and fp32 calls take a second part, fp16(x' - first), and twice the products.
+#include <initializer_list>
+
 #include "stored.cuh"
 
 namespace hi2 {
@@ -14,7 +16,7 @@ namespace stored {
 namespace {
 
 // ---- layout -----------------------------------------------------------------------------------------
-// One thread moves one row's 64 columns: codes into their pieces, parameter pairs behind them.
+// One thread moves one row's 64 columns: codes into their words, parameter pairs behind them.
 __global__ void __launch_bounds__(256)
 lay_out_kernel(const hi2_stored_weight w, const int32_t* __restrict__ src_row, const int32_t* __restrict__ codes,
                const int32_t* __restrict__ code_off, const uint8_t* __restrict__ blk_params,
@@ -24,160 +26,110 @@ lay_out_kernel(const hi2_stored_weight w, const int32_t* __restrict__ src_row, c
   for (int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; id < total; id += (int64_t)gridDim.x * blockDim.x) {
     const int64_t chunk = id / n_rows, i = id % n_rows;  // neighbouring threads: rows of one slab
     const int32_t src = src_row[i];
-    const RowForm row = load_row(w.rows, i);
-    if (src < 0 || row.width() == 0) continue;
-    const int64_t g = i / GROUP_ROWS;
-    uint8_t* slab = data + ((int64_t)w.groups[2 * g] + chunk * w.groups[2 * g + 1]) * 16;
-    const int nbits = 1 << row.width();
+    const GroupForm form = load_group(w.groups, i / GROUP_ROWS);
+    if (src < 0 || form.width() == 0) continue;
+    const int g = (int)(i & 7), r = (int)(i >> 3 & 3);
+    uint8_t* slab = data + (int64_t)form.base * 16 + chunk * form.slab_bytes();
+    const int nbits = 1 << form.width(), per_word = 32 / nbits, per_piece = nbits / 2;
     const uint32_t mask = (1u << nbits) - 1u;
     const int32_t* words = codes + code_off[src] + chunk * 2 * nbits;
-    const int per_word = 32 / nbits;
-    for (int q = 0; q < 2 * nbits; ++q) {  // word q of the chunk stays word q: only its fields move
+    for (int q = 0; q < 2 * nbits; ++q) {
       const uint32_t v = (uint32_t)words[q];
-      uint32_t r = 0;
-      for (int f = 0; f < per_word; ++f) r |= (v >> (f * nbits) & mask) << ((f >> 1) * nbits + (f & 1) * 16);
-      uint32_t* piece = reinterpret_cast<uint32_t*>(slab) + 4 * (row.piece() + (q >> 2) * row.piece_stride());
-      piece[q & 3] = r;
+      uint32_t fields = 0;
+      for (int f = 0; f < per_word; ++f) fields |= (v >> (f * nbits) & mask) << ((f >> 1) * nbits + (f & 1) * 16);
+      reinterpret_cast<uint32_t*>(slab)[128 * (q % per_piece) + 4 * (4 * g + q / per_piece) + r] = fields;
     }
-    const int pairs = 4 >> row.block_shift();
+    const int pairs = 4 >> form.shift();
     const uint8_t* from = blk_params + 2 * (param_off[src] + chunk * pairs);
-    for (int b = 0; b < 2 * pairs; ++b) slab[row.params() + b] = from[b];
-  }
-}
-
-// ---- activations ------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ float as_float(T v);
-template <>
-__device__ __forceinline__ float as_float(float v) { return v; }
-template <>
-__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-template <typename T>
-__device__ __forceinline__ void load16(const T* p, bool vector, float (&v)[16]) {
-  if (vector) {
-    constexpr int PER = 16 / (int)sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 16 / PER; ++i) {
-      const uint4 raw = *(reinterpret_cast<const uint4*>(p) + i);
-      const T* t = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) v[PER * i + j] = as_float(t[j]);
+    uint8_t* to = slab + form.code_bytes();
+    for (int t = 0; t < pairs; ++t) {
+      const int unit = 4 * (pairs * g + t) + r;
+      to[2 * unit] = from[2 * t], to[2 * unit + 1] = from[2 * t + 1];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = as_float(p[i]);
   }
 }
 
-struct Source {
-  const void* x;         // [tokens, ldx], or the fp32 [rows, 2 k] result of the gate and up rows
-  int64_t ldx;
-  int act;               // of the gate rows
-  bool vector;           // rows start on 16-byte boundaries
-  const int32_t* pair_of;  // stack: row -> (token, slot) pair, else null
-  const int64_t* index;  // stack: pair -> expert
-  const int32_t* used;   // stack: number of rows in use
-  int top_k;
-};
-
-// 16 columns of a row in the stored basis.  GATED: the row is act(gate) * up.
-template <typename T, bool GATED>
-__device__ __forceinline__ void stored_basis(const Source& s, const hi2_stored_weight& w, int64_t row, int64_t expert,
-                                             int64_t g, float (&v)[16]) {
-  if (GATED) {
-    const float* z = static_cast<const float*>(s.x) + row * s.ldx + g * 16;
-    float u[16];
-    load16(z, true, v);
-    load16(z + w.k, true, u);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = activate(v[i], s.act) * u[i];
-  } else {
-    load16(static_cast<const T*>(s.x) + row * s.ldx + g * 16, s.vector, v);
-  }
-  if (w.inv_scale != nullptr) {
-    float c[16];
-    load16(w.inv_scale + expert * w.k + g * 16, true, c);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] *= c[i];
-  }
-  if (w.had[expert * (w.k / 16) + g] != 0) {
-#pragma unroll
-    for (int span = 1; span < 16; span *= 2)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if ((i & span) == 0) {
-          const float a = v[i], b = v[i + span];
-          v[i] = a + b, v[i + span] = a - b;
-        }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] *= 0.25f;
-  }
-}
-
+// ---- activations of wide products ---------------------------------------------------------------------
+// A team of warps per activation row: largest value, then the fp16 parts relative to its power of two.  A
+// lane keeps up to HOLD pieces of 16 columns in registers; HOLD = 0 forms them twice.
 constexpr int PREP_THREADS = 128;
 
-// One block per activation row: largest value, then the fp16 parts relative to its power of two.
-template <typename T, bool GATED>
+template <int WARPS, int HOLD>
 __global__ void __launch_bounds__(PREP_THREADS)
-prepare_kernel(const Source s, const hi2_stored_weight w, int64_t rows, int parts, __half* __restrict__ xs,
-               float* __restrict__ row_scale) {
-  const int64_t row = blockIdx.x;
+prepare_kernel(const Product p, const int32_t* __restrict__ used) {
+  constexpr int TEAM = WARPS * 32;
+  const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
+  const int64_t row = (int64_t)blockIdx.x * (PREP_THREADS / TEAM) + team;
+  if (row >= (used == nullptr ? p.tiles.rows : (int64_t)*used)) return;  // a team of several warps is the whole block
   int64_t from = row, expert = 0;
-  if (s.pair_of != nullptr) {
-    if (row >= *s.used) return;
-    const int32_t pair = s.pair_of[row];
-    expert = s.index[pair];
-    if (!GATED) from = pair / s.top_k;
+  if (p.tiles.index != nullptr) {
+    const int64_t pair = p.tiles.pair(row);
+    expert = p.tiles.index[pair];
+    if (p.from.kind != FROM_GATED) from = pair / p.from.top_k;
   }
-  const int64_t groups = w.k / 16;
+  const int groups = (int)(p.w.k / 16);
+  constexpr int KEEP = HOLD == 0 ? 1 : HOLD;
+  float v[KEEP][16];
   float top = 0.0f;
-  for (int64_t g = threadIdx.x; g < groups; g += PREP_THREADS) {
-    float v[16];
-    stored_basis<T, GATED>(s, w, from, expert, g, v);
+  if (HOLD > 0) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(v[i]));
+    for (int h = 0; h < KEEP; ++h)
+      if (lane + h * TEAM < groups) {
+        stored_basis(p.from, p.w, from, expert, lane + h * TEAM, v[h]);
+        top = fmaxf(top, largest(v[h]));
+      }
+  } else {
+    for (int g = lane; g < groups; g += TEAM) {
+      stored_basis(p.from, p.w, from, expert, g, v[0]);
+      top = fmaxf(top, largest(v[0]));
+    }
   }
-  __shared__ float warp_top[PREP_THREADS / 32];
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
-  __syncthreads();
+  if (WARPS > 1) {
+    __shared__ float warp_top[WARPS];
+    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < PREP_THREADS / 32; ++i) top = fmaxf(top, warp_top[i]);
-  const int biased = (int)(__float_as_uint(top) >> 23);
-  int e = biased - 127 - 14;  // a row without values, or with an infinity: left as it is
-  if (top == 0.0f || biased == 255) e = 0;
-  if (e < -110) e = -110;     // 2^-e has to be an fp32 number
-  const float to = __uint_as_float((uint32_t)(127 - e) << 23);
-  if (threadIdx.x == 0) row_scale[row] = __uint_as_float((uint32_t)(127 + e) << 23);
-  for (int64_t g = threadIdx.x; g < groups; g += PREP_THREADS) {
-    float v[16];
-    stored_basis<T, GATED>(s, w, from, expert, g, v);
-    uint32_t hi[8], lo[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = v[2 * i] * to, b = v[2 * i + 1] * to;
-      const __half2 h = __floats2half2_rn(a, b);
-      hi[i] = bits(h);
-      lo[i] = bits(__floats2half2_rn(a - __low2float(h), b - __high2float(h)));
+    for (int i = 0; i < WARPS; ++i) top = fmaxf(top, warp_top[i]);
+  }
+  const PowerOfTwo power = power_for(top);
+  if (lane == 0) p.row_scale[row] = power.back;
+  auto store = [&](int g, const float (&x)[16]) {
+    uint4 hi[2], lo[2];
+    split16(x, power.to, hi, lo);
+    uint4* dst = reinterpret_cast<uint4*>(p.xs + row * p.w.k + (int64_t)g * 16);
+    dst[0] = hi[0], dst[1] = hi[1];
+    if (p.parts == 2) {
+      dst = reinterpret_cast<uint4*>(p.xs + (p.tiles.rows + row) * p.w.k + (int64_t)g * 16);
+      dst[0] = lo[0], dst[1] = lo[1];
     }
-    uint4* dst = reinterpret_cast<uint4*>(xs + row * w.k + g * 16);
-    dst[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]), dst[1] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-    if (parts == 2) {
-      dst = reinterpret_cast<uint4*>(xs + (rows + row) * w.k + g * 16);
-      dst[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]), dst[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+  };
+  if (HOLD > 0) {
+#pragma unroll
+    for (int h = 0; h < KEEP; ++h)
+      if (lane + h * TEAM < groups) store(lane + h * TEAM, v[h]);
+  } else {
+    for (int g = lane; g < groups; g += TEAM) {
+      stored_basis(p.from, p.w, from, expert, g, v[0]);
+      store(g, v[0]);
     }
   }
+}
+
+int prepare(const Product& p, const int32_t* used, cudaStream_t stream) {
+  const int64_t rows = p.tiles.rows;
+  if (p.w.k <= 32 * 4 * 16) prepare_kernel<1, 4><<<(unsigned)ceil_div(rows, (int64_t)4), PREP_THREADS, 0, stream>>>(p, used);
+  else if (p.w.k <= 128 * 4 * 16) prepare_kernel<4, 4><<<(unsigned)rows, PREP_THREADS, 0, stream>>>(p, used);
+  else prepare_kernel<4, 0><<<(unsigned)rows, PREP_THREADS, 0, stream>>>(p, used);
+  return check_launch("stored: activations");
 }
 
 // ---- dispatch -----------------------------------------------------------------------------------------
 // Stable counting sort of the (token, slot) pairs by expert in one block: every warp counts its stretch of
-// the pairs (lanes that name the same expert find each other by a match), the counts are summed over
-// the warps and experts, and every warp places its stretch.  Also the list of token tiles.
-constexpr int SORT_WARPS = 32;
+// the pairs, the counts are summed over the warps and experts, and every warp places its stretch in order
+// (lanes that name the same expert find each other by a match).  Also the list of token tiles.
+constexpr int SORT_WARPS = 32, SORT_BATCH = 8;
 constexpr int MAX_EXPERTS = 1024;
 
 __global__ void __launch_bounds__(SORT_WARPS * 32)
@@ -192,12 +144,20 @@ dispatch_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, i
   int32_t* mine = counts + warp * experts;
   const int64_t per = ceil_div(ceil_div(pairs, (int64_t)SORT_WARPS), (int64_t)32) * 32;
   const int64_t first = warp * per, last = first + per < pairs ? first + per : pairs;
-  for (int64_t i = first; i < last; i += 32) {
-    const int64_t e64 = i + lane < last ? index[i + lane] : -1;
-    const int e = e64 >= 0 && e64 < experts ? (int)e64 : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
+  auto load = [&](int64_t i, int64_t (&e)[SORT_BATCH]) {  // several at a time: a load takes most of a microsecond
+#pragma unroll
+    for (int b = 0; b < SORT_BATCH; ++b) {
+      const int64_t at = i + 32 * b + lane;
+      e[b] = at < last ? index[at] : -1;
+      if (e[b] < 0 || e[b] >= experts) e[b] = -1;
+    }
+  };
+  for (int64_t i = first; i < last; i += 32 * SORT_BATCH) {
+    int64_t e[SORT_BATCH];
+    load(i, e);
+#pragma unroll
+    for (int b = 0; b < SORT_BATCH; ++b)
+      if (e[b] >= 0) atomicAdd(mine + e[b], 1);  // a count: the order of the additions does not matter
   }
   __syncthreads();
   // thread e: the expert's total, its first row and its first tile (exclusive sums over the experts)
@@ -229,34 +189,40 @@ dispatch_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, i
     }
   }
   __syncthreads();
-  for (int64_t i = first; i < last; i += 32) {
-    const bool in = i + lane < last;
-    const int64_t e64 = in ? index[i + lane] : -1;
-    const int x = e64 >= 0 && e64 < experts ? (int)e64 : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, x);
-    if (x >= 0) {
-      const int32_t row = mine[x] + __popc(same & ((1u << lane) - 1u));
-      pair_of[row] = (int32_t)(i + lane);
-      row_of[i + lane] = row;
-    } else if (in) {
-      row_of[i + lane] = -1;
+  for (int64_t i = first; i < last; i += 32 * SORT_BATCH) {
+    int64_t e[SORT_BATCH];
+    load(i, e);
+#pragma unroll
+    for (int b = 0; b < SORT_BATCH; ++b) {
+      const int64_t at = i + 32 * b + lane;
+      const int x = (int)e[b];
+      const uint32_t same = __match_any_sync(0xffffffffu, x);
+      int32_t row = -1;
+      if (x >= 0) {
+        row = mine[x] + __popc(same & ((1u << lane) - 1u));
+        pair_of[row] = (int32_t)at;
+      }
+      if (at < last) row_of[at] = row;
+      __syncwarp();
+      if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
+      __syncwarp();
     }
-    __syncwarp();
-    if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
-    __syncwarp();
   }
 }
 
 // out[t] = sum of the token's weighted rows in slot order (a fixed order: the same bits every time).
 __global__ void __launch_bounds__(256)
-combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ row_of, int64_t tokens, int top_k, int64_t hidden,
+combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ row_of, const int64_t* __restrict__ index, int experts, int64_t tokens, int top_k, int64_t hidden,
                void* __restrict__ out, int dtype, int64_t ld_out) {
   const int64_t quads = hidden / 4, total = tokens * quads;
   for (int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; id < total; id += (int64_t)gridDim.x * blockDim.x) {
     const int64_t t = id / quads, c = id % quads * 4;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int j = 0; j < top_k; ++j) {
-      const int32_t row = row_of[t * top_k + j];
+      const int64_t pair = t * top_k + j;
+      int64_t row = pair;
+      if (row_of != nullptr) row = row_of[pair];
+      else if (index[pair] < 0 || index[pair] >= experts) row = -1;
       if (row < 0) continue;
       const float4 v = *reinterpret_cast<const float4*>(y + (int64_t)row * hidden + c);
       sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
@@ -281,55 +247,59 @@ struct Carver {
   }
 };
 
+// Which kernel takes a product.
+inline bool few(const hi2_stored_weight& w, int64_t tokens) { return tokens <= 32; }
+inline int64_t rows_per_expert(int64_t experts, int64_t pairs) {  // with half as many again as on average
+  const int64_t busy = ceil_div(3 * pairs, 2 * experts);
+  return busy < pairs ? busy : pairs;
+}
+inline bool few_experts(int64_t experts, int64_t pairs) { return rows_per_expert(experts, pairs) <= 32; }
+inline bool apart(int64_t pairs) { return pairs <= 16; }  // every pair a tile of its own
+
 inline int parts_of(int dtype) { return dtype == HI2_BF16 ? 1 : 2; }
 inline int64_t size_of(int dtype) { return dtype == HI2_F32 ? 4 : 2; }
 inline bool rows_aligned(const void* p, int64_t ld, int dtype) { return aligned16(p) && ld * size_of(dtype) % 16 == 0; }
+inline int kind_of(int dtype) { return dtype == HI2_BF16 ? FROM_BF16 : dtype == HI2_F16 ? FROM_F16 : FROM_F32; }
 
 struct LinearSpace {
-  __half* xs;
-  float* scale;
+  __half* xs = nullptr;
+  float* scale = nullptr;
   size_t bytes;
   LinearSpace(void* ws, const hi2_stored_weight& w, int dtype, int64_t tokens) {
     Carver c{static_cast<uint8_t*>(ws)};
-    xs = c.take<__half>((size_t)tokens * w.k * parts_of(dtype));
-    scale = c.take<float>(tokens);
+    if (!few(w, tokens)) {
+      xs = c.take<__half>((size_t)tokens * w.k * parts_of(dtype));
+      scale = c.take<float>(tokens);
+    }
     bytes = c.used;
   }
 };
 
 struct ExpertSpace {
-  __half *xs, *hs;
-  float *x_scale, *h_scale, *z, *y;
-  int32_t *pair_of, *row_of, *used, *tile_count;
-  TokenTile* tiles;
+  __half* xs = nullptr;  // of the gate/up product, then of the down product
+  float *scale = nullptr, *z, *y;
+  int32_t *pair_of = nullptr, *row_of = nullptr, *used = nullptr, *tile_count = nullptr;
+  TokenTile* tiles = nullptr;
   size_t bytes;
   ExpertSpace(void* ws, const hi2_stored_weight& gate_up, int dtype, int64_t tokens, int top_k) {
     const size_t pairs = (size_t)tokens * top_k, hidden = gate_up.k, inner = gate_up.rows_per_expert / 2;
     Carver c{static_cast<uint8_t*>(ws)};
-    used = c.take<int32_t>(64);
-    tile_count = used == nullptr ? nullptr : used + 32;
-    pair_of = c.take<int32_t>(pairs);
-    row_of = c.take<int32_t>(pairs);
-    tiles = c.take<TokenTile>(pairs / 16 + gate_up.experts + 1);
-    x_scale = c.take<float>(pairs);
-    h_scale = c.take<float>(pairs);
-    xs = c.take<__half>(pairs * hidden * parts_of(dtype));
     z = c.take<float>(pairs * inner * 2);
-    hs = c.take<__half>(pairs * inner * parts_of(dtype));
     y = c.take<float>(pairs * hidden);
+    if (!apart(pairs)) {
+      used = c.take<int32_t>(64);
+      tile_count = used == nullptr ? nullptr : used + 32;
+      pair_of = c.take<int32_t>(pairs);
+      row_of = c.take<int32_t>(pairs);
+      tiles = c.take<TokenTile>(pairs / 8 + gate_up.experts + 1);
+    }
+    if (!few_experts(gate_up.experts, pairs)) {
+      xs = c.take<__half>(pairs * (hidden > inner ? hidden : inner) * parts_of(dtype));
+      scale = c.take<float>(pairs);
+    }
     bytes = c.used;
   }
 };
-
-template <bool GATED>
-int prepare(const Source& s, const hi2_stored_weight& w, int dtype, int64_t rows, int parts, __half* xs, float* scale,
-            cudaStream_t stream) {
-  const unsigned grid = (unsigned)rows;
-  if (dtype == HI2_BF16) prepare_kernel<__nv_bfloat16, GATED><<<grid, PREP_THREADS, 0, stream>>>(s, w, rows, parts, xs, scale);
-  else if (dtype == HI2_F16) prepare_kernel<__half, GATED><<<grid, PREP_THREADS, 0, stream>>>(s, w, rows, parts, xs, scale);
-  else prepare_kernel<float, GATED><<<grid, PREP_THREADS, 0, stream>>>(s, w, rows, parts, xs, scale);
-  return check_launch("stored: activations");
-}
 
 bool complete(const hi2_stored_weight* w) {
   return w != nullptr && w->data != nullptr && w->groups != nullptr && w->rows != nullptr && w->had != nullptr &&
@@ -375,16 +345,17 @@ extern "C" int hi2_stored_linear(const hi2_stored_weight* w, const void* x, int 
   if (tokens == 0) return HI2_OK;
   HI2_REQUIRE(x && out, "stored_linear: null pointer");
   const LinearSpace space(workspace, *w, dtype, tokens);
-  if (workspace == nullptr || workspace_bytes < space.bytes || !aligned16(workspace))
+  if (space.bytes > 0 && (workspace == nullptr || workspace_bytes < space.bytes || !aligned16(workspace)))
     return fail(HI2_ERR_WORKSPACE, "stored_linear: workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  Source src{x, ldx, HI2_ACT_NONE, rows_aligned(x, ldx, dtype), nullptr, nullptr, nullptr, 1};
-  int rc = prepare<false>(src, *w, dtype, tokens, parts_of(dtype), space.xs, space.scale, s);
-  if (rc != HI2_OK) return rc;
-  const int width = tile_width(tokens);
-  const Product p{*w, space.xs, tokens, parts_of(dtype), Tiles{nullptr, nullptr, tokens, width}, ceil_div(tokens, (int64_t)width),
-                  Epilogue{space.scale, nullptr, nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}};
-  return product(p, s, "stored_linear");
+  const bool small = few(*w, tokens);
+  const int width = small ? few_width(tokens) : wide_width(tokens);
+  const Product p{*w, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), 1},
+                  Tiles{nullptr, nullptr, nullptr, nullptr, tokens, 1, width}, ceil_div(tokens, (int64_t)width), parts_of(dtype),
+                  Epilogue{nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}, space.xs, space.scale};
+  if (small) return product_few(p, s, "stored_linear");
+  const int rc = prepare(p, nullptr, s);
+  return rc != HI2_OK ? rc : product_wide(p, s, "stored_linear");
 }
 
 extern "C" size_t hi2_stored_experts_workspace_bytes(const hi2_stored_weight* gate_up, int dtype, int64_t tokens, int top_k) {
@@ -412,35 +383,37 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t pairs = tokens * top_k, hidden = gate_up->k, inner = down->k;
   const int experts = (int)gate_up->experts, parts = parts_of(dtype);
-  // tiles wide enough for an expert with half as many tokens again as the average one
-  const int64_t busy = ceil_div(3 * pairs, (int64_t)(2 * experts));
-  const int width = tile_width(busy < pairs ? busy : pairs);
-  const size_t smem = (size_t)SORT_WARPS * experts * sizeof(int32_t);
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(dispatch_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return fail(HI2_ERR_LAUNCH, "stored_experts: cannot reserve shared memory");
-  dispatch_kernel<<<1, SORT_WARPS * 32, smem, s>>>(index, pairs, experts, width, space.pair_of, space.row_of, space.used,
-                                                  space.tile_count, space.tiles);
-  int rc = check_launch("stored_experts: dispatch");
-  if (rc != HI2_OK) return rc;
-  Source src{x, ldx, HI2_ACT_NONE, rows_aligned(x, ldx, dtype), space.pair_of, index, space.used, top_k};
-  rc = prepare<false>(src, *gate_up, dtype, pairs, parts, space.xs, space.x_scale, s);
-  if (rc != HI2_OK) return rc;
-  const int64_t max_tiles = pairs / width + experts + 1;
-  const Tiles tiles{space.tile_count, space.tiles, pairs, width};
-  Product p{*gate_up, space.xs, pairs, parts, tiles, max_tiles,
-            Epilogue{space.x_scale, space.pair_of, nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}};
-  rc = product(p, s, "stored_experts");
-  if (rc != HI2_OK) return rc;
-  src = Source{space.z, 2 * inner, act, true, space.pair_of, index, space.used, top_k};
-  rc = prepare<true>(src, *down, dtype, pairs, parts, space.hs, space.h_scale, s);
-  if (rc != HI2_OK) return rc;
-  p = Product{*down, space.hs, pairs, parts, tiles, max_tiles,
-              Epilogue{space.h_scale, space.pair_of, weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}};
-  rc = product(p, s, "stored_experts");
-  if (rc != HI2_OK) return rc;
+  const bool small = few_experts(experts, pairs);
+  Tiles tiles{index, nullptr, nullptr, nullptr, pairs, experts, 1};
+  int64_t max_tiles = pairs;
+  int rc;
+  if (!apart(pairs)) {
+    const int64_t busy = rows_per_expert(experts, pairs);
+    tiles = Tiles{index, space.pair_of, space.tile_count, space.tiles, pairs, experts, small ? few_width(busy) : wide_width(busy)};
+    max_tiles = pairs / tiles.width + experts + 1;
+    const size_t smem = (size_t)SORT_WARPS * experts * sizeof(int32_t);
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(dispatch_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return fail(HI2_ERR_LAUNCH, "stored_experts: cannot reserve shared memory");
+    dispatch_kernel<<<1, SORT_WARPS * 32, smem, s>>>(index, pairs, experts, tiles.width, space.pair_of, space.row_of, space.used,
+                                                    space.tile_count, space.tiles);
+    if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
+  }
+  const Product up{*gate_up, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), top_k}, tiles, max_tiles, parts,
+                   Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, space.xs, space.scale};
+  const Product dn{*down, Source{space.z, 2 * inner, FROM_GATED, act, true, top_k}, tiles, max_tiles, parts,
+                   Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, space.xs, space.scale};
+  for (const Product* p : {&up, &dn}) {
+    if (small) {
+      rc = product_few(*p, s, "stored_experts");
+    } else {
+      rc = prepare(*p, space.used, s);
+      if (rc == HI2_OK) rc = product_wide(*p, s, "stored_experts");
+    }
+    if (rc != HI2_OK) return rc;
+  }
   int64_t blocks = ceil_div(tokens * (hidden / 4), (int64_t)256);
   if (blocks > 148 * 16) blocks = 148 * 16;
-  combine_kernel<<<(unsigned)blocks, 256, 0, s>>>(space.y, space.row_of, tokens, top_k, hidden, out, dtype, ld_out);
+  combine_kernel<<<(unsigned)blocks, 256, 0, s>>>(space.y, space.row_of, index, experts, tokens, top_k, hidden, out, dtype, ld_out);
   return check_launch("stored_experts: combine");
 }

@@ -1,0 +1,310 @@
+// The product of packed rows with up to 32 activation rows: decode steps and small batches, where the packed
+// bytes are what has to be moved.
+//
+// A block takes 128 sorted rows and a slice of the columns; the slices of a row tile are a cluster and join
+// their sums through distributed shared memory in rank order.  Warps 0..3 and 4..7 take the tile's four groups
+// of 32 rows, each half of the warps one half of the columns.  Every warp streams its own part of the packed
+// data through a ring of bulk copies, so the loads of a whole block are in flight before anything is
+// computed, and no barrier between warps is needed while it lasts.
+//
+// The slice is taken in blocks of 1024 columns.  First the warps form the activations' fp16 parts of the block
+// in shared memory (divided, rotated, relative to a power of two per row and half of the BLOCK, so nothing
+// waits for a whole row's largest value); then every warp decodes chunk after chunk straight into the A fragments of warp-level
+// products m16n8k16: lane 4 g + t holds 16 columns of rows g, g + 8, g + 16 and g + 24, and the column order
+// inside a chunk is the same permutation for both operands, so a lane's 16 columns are contiguous in memory.
+// The tensor pipe is idle most of the time; what bounds the kernel is the decoding, about 150 instructions per
+// warp for 2048 INT2 weights, and behind it the packed bytes.
+#include "stored_async.cuh"
+
+namespace hi2 {
+namespace stored {
+namespace {
+
+constexpr int WARPS = 8, THREADS = 256;
+constexpr int BLOCK_CHUNKS = 16, BLOCK_COLUMNS = BLOCK_CHUNKS * CHUNK;
+constexpr int HALF_CHUNKS = BLOCK_CHUNKS / 2;
+constexpr int RING_STAGES = 3, RING_BYTES = 3072;  // a stage: four chunks of INT2, two of INT4, one of INT8
+constexpr int X_PITCH = BLOCK_COLUMNS + 8;         // halves; the extra 16 bytes keep 128-bit reads of eight rows apart
+constexpr int SUM_PITCH = TILE_ROWS + 4;
+constexpr int MAX_SPLIT = 8;
+
+template <int NT>
+struct Shared {
+  union {
+    uint8_t ring[WARPS][RING_STAGES][RING_BYTES];
+    float sums[2][8 * NT][SUM_PITCH];  // of the two halves, once the rings are done with
+  };
+  float scale[2][2][8 * NT];         // of the block being multiplied and of the one before; of each half
+  uint32_t out_row[TILE_ROWS];
+  unsigned long long full[WARPS][RING_STAGES];
+  volatile uint32_t abort;
+};
+template <int NT>
+size_t smem_bytes(int parts) {
+  return sizeof(Shared<NT>) + (size_t)parts * 8 * NT * X_PITCH * sizeof(__half) + 16;
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The lane's 16 columns of its four rows in the chunk at `slab`.
+struct LaneRows {
+  float lo_min[4], lo_scale[4];
+  __half2 step_scale[2];
+};
+template <int NBITS>
+__device__ __forceinline__ void decode_rows(const uint8_t* slab, int lane, int pair_unit, const LaneRows& rows, uint32_t (&w)[4][8]) {
+  const uint2 pairs = *reinterpret_cast<const uint2*>(slab + 256 * NBITS + 8 * pair_unit);
+  Ladder l[4];
+  {
+    const float min01[2] = {rows.lo_min[0], rows.lo_min[1]}, scale01[2] = {rows.lo_scale[0], rows.lo_scale[1]};
+    const float min23[2] = {rows.lo_min[2], rows.lo_min[3]}, scale23[2] = {rows.lo_scale[2], rows.lo_scale[3]};
+    ladders(pairs.x, min01, scale01, rows.step_scale[0], l[0], l[1]);
+    ladders(pairs.y, min23, scale23, rows.step_scale[1], l[2], l[3]);
+  }
+#pragma unroll
+  for (int h = 0; h < NBITS / 2; ++h) {
+    const uint4 v = *reinterpret_cast<const uint4*>(slab + 512 * h + 16 * lane);
+    const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (NBITS == 2) decode_int2(q[r], l[r], w[r]);
+      else if (NBITS == 4) decode_int4(q[r], l[r], w[r] + 4 * h);
+      else decode_int8(q[r], l[r], w[r] + 2 * h);
+    }
+  }
+}
+
+template <int NT>
+__global__ void __launch_bounds__(THREADS, NT < 4 ? 2 : 1)
+few_kernel(const Product p, const int split) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  Shared<NT>& sm = *reinterpret_cast<Shared<NT>*>(raw);
+  __half* const xs = reinterpret_cast<__half*>((reinterpret_cast<uintptr_t>(raw) + sizeof(Shared<NT>) + 15) & ~(uintptr_t)15);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int rank = (int)(blockIdx.x % split);
+  const int row_tiles = (int)(p.w.groups_per_expert / 4);
+  const int row_tile = (int)(blockIdx.x / split) % row_tiles;
+  int32_t* const status = p.w.status;
+  TokenTile tile;
+  if (p.tiles.index != nullptr) chain_wait();  // which expert comes from an earlier kernel
+  if (!p.tiles.get(blockIdx.x / split / row_tiles, tile)) return;  // the same for all blocks of a cluster
+  const int tokens = tile.end - tile.begin;
+
+  // ---- this warp's stream of packed data
+  const int half = warp >> 2, quarter = warp & 3;
+  const int all = (int)(p.w.k / CHUNK);
+  const int c0 = (int)((int64_t)all * rank / split), n = (int)((int64_t)all * (rank + 1) / split) - c0;
+  const int blocks = (n + BLOCK_CHUNKS - 1) / BLOCK_CHUNKS;
+  const int last_chunks = n - (blocks - 1) * BLOCK_CHUNKS;                      // of the last block
+  const int last_half0 = (last_chunks + 1) / 2;
+  const int last_mine = half == 0 ? last_half0 : last_chunks - last_half0;
+  const int mine = (blocks - 1) * HALF_CHUNKS + last_mine;
+  const int64_t group = (int64_t)tile.expert * p.w.groups_per_expert + row_tile * 4 + quarter;
+  const GroupForm form = load_group(p.w.groups, group);
+  const int slab = form.slab_bytes(), copy_shift = 3 - form.width(), per_copy = 1 << copy_shift;  // 4, 2, 1 chunks
+  const uint8_t* const data = static_cast<const uint8_t*>(p.w.data) + (int64_t)form.base * 16;
+  const int copies = form.width() == 0 ? 0 : (mine + per_copy - 1) >> copy_shift;
+  auto issue = [&](int copy, int stage) {  // by one lane
+    const int j = copy << copy_shift, b = j / HALF_CHUNKS, count = min(per_copy, mine - j);
+    const int chunk = c0 + b * BLOCK_CHUNKS + (half == 0 ? 0 : b == blocks - 1 ? last_half0 : HALF_CHUNKS) + j % HALF_CHUNKS;
+    bar_expect(&sm.full[warp][stage], (uint32_t)(count * slab));
+    bulk_load(sm.ring[warp][stage], data + (int64_t)chunk * slab, (uint32_t)(count * slab), &sm.full[warp][stage]);
+  };
+  if (lane == 0) {
+    for (int s = 0; s < RING_STAGES; ++s) bar_init(&sm.full[warp][s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    for (int c = 0; c < RING_STAGES && c < copies; ++c) issue(c, c);
+  }
+  if (threadIdx.x == 0) sm.abort = 0;
+  LaneRows rows;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const RowConsts c = load_row(p.w.rows, group * GROUP_ROWS + 8 * r + g);
+    rows.lo_min[r] = c.lo_min(), rows.lo_scale[r] = c.lo_scale();
+    const __half s = __ushort_as_half((uint16_t)c.step_scale);
+    if (r & 1) rows.step_scale[r / 2] = __halves2half2(__low2half(rows.step_scale[r / 2]), s);
+    else rows.step_scale[r / 2] = __half2half2(s);
+    if (half == 0 && t == 0) sm.out_row[quarter * 32 + 8 * r + g] = c.out_row;
+  }
+  const int pair_unit = (4 >> form.shift()) * g + (t >> form.shift());
+
+  float total[2][NT][4];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total[m][q][i] = 0.0f;
+
+  chain_wait();  // the activations
+  bool ok = true;
+  int copy = 0, at = 0, stage = 0;  // of the ring: copy, chunk inside it, stage
+  uint32_t phase = 0;
+  for (int b = 0; b < blocks; ++b) {
+    const int chunks = b == blocks - 1 ? last_chunks : BLOCK_CHUNKS;
+    const int half0 = b == blocks - 1 ? last_half0 : HALF_CHUNKS;
+    // ---- the block's activations, a warp per row and half: up to 32 pieces of 16 columns, one per lane
+    __syncthreads();  // nobody reads the block before any more (and the barriers' words are set)
+    for (int u = warp; u < 2 * tokens; u += WARPS) {
+      const int r = u >> 1, second = u & 1;
+      const int piece = (second ? 4 * half0 : 0) + lane;
+      const bool in = piece < 4 * (second ? chunks : half0);
+      int64_t from = tile.begin + r;
+      if (p.tiles.index != nullptr && p.from.kind != FROM_GATED) from = p.tiles.pair(from) / p.from.top_k;
+      float v[16];
+      float top = 0.0f;
+      if (in) {
+        stored_basis(p.from, p.w, from, tile.expert, (int64_t)(c0 + b * BLOCK_CHUNKS) * 4 + piece, v);
+        top = largest(v);
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const PowerOfTwo power = power_for(top);
+      if (lane == 0) sm.scale[b & 1][second][r] = power.back;
+      if (in) {
+        uint4 hi[2], lo[2];
+        split16(v, power.to, hi, lo);
+        uint4* dst = reinterpret_cast<uint4*>(xs + r * X_PITCH + piece * 16);
+        dst[0] = hi[0], dst[1] = hi[1];
+        if (p.parts == 2) {
+          dst = reinterpret_cast<uint4*>(xs + (8 * NT + r) * X_PITCH + piece * 16);
+          dst[0] = lo[0], dst[1] = lo[1];
+        }
+      }
+    }
+    __syncthreads();
+    // ---- this warp's chunks of the block
+    float acc[2][NT][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int q = 0; q < NT; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][q][i] = 0.0f;
+    const int first = half == 0 ? 0 : half0, count = half == 0 ? half0 : chunks - half0;
+    if (copies > 0 && ok)
+      for (int i = 0; i < count; ++i) {
+        if (at == 0) {
+          ok = __all_sync(0xffffffffu, bar_wait(&sm.full[warp][stage], phase, &sm.abort, status));
+          if (!ok) break;
+        }
+        const uint8_t* from = sm.ring[warp][stage] + at * slab;
+        uint32_t w[4][8];
+        if (form.width() == 1) decode_rows<2>(from, lane, pair_unit, rows, w);
+        else if (form.width() == 2) decode_rows<4>(from, lane, pair_unit, rows, w);
+        else decode_rows<8>(from, lane, pair_unit, rows, w);
+        for (int part = 0; part < p.parts; ++part) {
+          const __half* x = xs + (part * 8 * NT + g) * X_PITCH + (first + i) * CHUNK + 16 * t;
+#pragma unroll
+          for (int q = 0; q < NT; ++q) {
+            const uint4 x0 = *reinterpret_cast<const uint4*>(x + q * 8 * X_PITCH), x1 = *reinterpret_cast<const uint4*>(x + q * 8 * X_PITCH + 8);
+            const uint32_t k[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              mma(acc[0][q], w[0][2 * s], w[1][2 * s], w[0][2 * s + 1], w[1][2 * s + 1], k[2 * s], k[2 * s + 1]);
+              mma(acc[1][q], w[2][2 * s], w[3][2 * s], w[2][2 * s + 1], w[3][2 * s + 1], k[2 * s], k[2 * s + 1]);
+            }
+          }
+        }
+        if (++at == per_copy) {
+          __syncwarp();  // every lane has read the stage
+          if (lane == 0 && copy + RING_STAGES < copies) issue(copy + RING_STAGES, stage);
+          __syncwarp();
+          ++copy, at = 0;
+          if (++stage == RING_STAGES) stage = 0, phase ^= 1;
+        }
+      }
+#pragma unroll
+    for (int q = 0; q < NT; ++q) {
+      const float s0 = sm.scale[b & 1][half][8 * q + 2 * t], s1 = sm.scale[b & 1][half][8 * q + 2 * t + 1];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        total[m][q][0] += acc[m][q][0] * s0, total[m][q][1] += acc[m][q][1] * s1;
+        total[m][q][2] += acc[m][q][2] * s0, total[m][q][3] += acc[m][q][3] * s1;
+      }
+    }
+  }
+  if (__syncthreads_or(!ok)) let_copies_land();
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int q = 0; q < NT; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sm.sums[half][8 * q + 2 * t + (i & 1)][quarter * 32 + 16 * m + 8 * (i >> 1) + g] = total[m][q][i];
+  __syncthreads();
+  if (split > 1) cluster_sync();
+  const uint32_t here = s32(&sm.sums[0][0][0]);
+  for (int i = rank * THREADS + threadIdx.x; i < tokens * TILE_ROWS; i += split * THREADS) {
+    const int token = i / TILE_ROWS, row = i % TILE_ROWS;
+    const uint32_t off = (uint32_t)(token * SUM_PITCH + row) * 4, other = 8 * NT * SUM_PITCH * 4;
+    float v[2 * MAX_SPLIT];
+    if (split > 1) {
+#pragma unroll
+      for (int q = 0; q < MAX_SPLIT; ++q)
+        if (q < split) {
+          const uint32_t there = in_rank(here, q) + off;
+          v[2 * q] = load_cluster(there), v[2 * q + 1] = load_cluster(there + other);
+        }
+    } else {
+      v[0] = sm.sums[0][token][row], v[1] = sm.sums[1][token][row];
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int q = 0; q < MAX_SPLIT; ++q)
+      if (q < split) sum += v[2 * q] + v[2 * q + 1];
+    const int64_t at = tile.begin + token;
+    if (p.out.pair_weight != nullptr) sum *= p.out.pair_weight[p.tiles.pair(at)];
+    const uint32_t col = sm.out_row[row];
+    if (col != NO_ROW) p.out.put(at, col, sum);
+  }
+  if (split > 1) cluster_sync();  // nobody reads this block's sums any more
+}
+
+template <int NT>
+int launch(const Product& p, int split, cudaStream_t stream, const char* what) {
+  const size_t smem = smem_bytes<NT>(p.parts);
+  if (cudaFuncSetAttribute(few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return fail(HI2_ERR_LAUNCH, "stored product: cannot reserve shared memory");
+  const int64_t blocks = p.w.groups_per_expert / 4 * p.max_tiles * split;
+  if (blocks >= (int64_t)1 << 31) return fail(HI2_ERR_ARG, "stored product: too many tiles");
+  cudaLaunchConfig_t config = {};
+  config.gridDim = (unsigned)blocks, config.blockDim = THREADS, config.dynamicSmemBytes = smem, config.stream = stream;
+  cudaLaunchAttribute attribute[2];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  attribute[1].id = cudaLaunchAttributeClusterDimension;
+  attribute[1].val.clusterDim.x = split, attribute[1].val.clusterDim.y = 1, attribute[1].val.clusterDim.z = 1;
+  config.attrs = attribute, config.numAttrs = 2;
+  cudaLaunchKernelEx(&config, few_kernel<NT>, p, split);
+  return check_launch(what);
+}
+
+}  // namespace
+
+int few_width(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+
+int product_few(const Product& p, cudaStream_t stream, const char* what) {
+  // Slices of the columns: the number that leaves the fullest SM the least work, with what a block costs
+  // besides its chunks (start, activations, the join) counted as twelve of them; each at least four chunks.
+  const int64_t tiles = p.w.groups_per_expert / 4 * p.max_tiles, chunks = p.w.k / CHUNK;
+  const int64_t room = 148 * (p.tiles.width <= 16 ? 2 : 1);
+  int split = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= MAX_SPLIT && (s == 1 || chunks >= 4 * s); ++s) {
+    const int64_t cost = ceil_div(tiles * s, room) * (ceil_div(chunks, (int64_t)s) + 12);
+    if (cost < least) least = cost, split = s;
+  }
+  if (p.tiles.width <= 8) return launch<1>(p, split, stream, what);
+  if (p.tiles.width <= 16) return launch<2>(p, split, stream, what);
+  return launch<4>(p, split, stream, what);
+}
+
+}  // namespace stored
+}  // namespace hi2

@@ -1,0 +1,508 @@
+// The product of packed rows with many activation rows (prompts, large batches), on CTA pairs.
+//
+//     D[r, t] = sum_k V[r, k] xs[t, k]        256 sorted rows x up to 192 activation rows per pair
+//
+// The packed rows are the A operand, kept in tensor memory: a lane decodes the 64 weights of ITS row in a
+// chunk of 64 columns (stored.cuh) and writes them as 32 fp16 pairs into its tensor-memory lane (tcgen05.st),
+// so decoded weights never pass through shared memory.  The activations are the B operand, K-major boxes of 64
+// columns that TMA brings into 128-byte-swizzled shared memory; each block of a pair loads half of a
+// tile's activation rows and both halves serve both blocks (cta_group::2), which halves what a block
+// asks of the L2: with one block per tile that is 64 bytes per clock at the full rate of the tensor pipe, as much as
+// an SM can take.  One thread of the leading block issues the products, M = 256: its block's 128 rows accumulate in its
+// tensor memory, the other 128 in its peer's.
+//
+// Blocks stay for many tiles.  Warps 0..7 decode (warp w: rows 32 (w mod 4) .. of the block's tile, one half of the
+// columns), every warp with its own ring of bulk copies that runs on into the next tile; warp 8 loads activations, warp 9
+// issues; warps 10..17 take finished tiles out of one of two accumulators (2 x 192 columns, beside two slots of 2 x 32
+// columns for decoded chunks) while the next tile is computed in the other.  A step is one chunk of each
+// half of the columns, in a fixed order: equal inputs give equal bits.
+//
+// Every mbarrier wait is bounded by a clock limit and raises *status.
+#include <cuda.h>
+
+#include "stored_async.cuh"
+
+namespace hi2 {
+namespace stored {
+namespace {
+
+constexpr int DECODE_WARPS = 8, X_WARP = 8, MMA_WARP = 9, FIRST_EPILOGUE = 10, EPILOGUE_WARPS = 8;
+constexpr int THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE_WARPS);
+constexpr int MAX_WIDTH = 192;
+constexpr int A_SLOTS = 2, A_COLUMNS = CHUNK / 2, SLOT_COLUMNS = 2 * A_COLUMNS;
+constexpr int FIRST_A_COLUMN = 2 * MAX_WIDTH;   // behind the two accumulators
+constexpr int RING_STAGES = 2, RING_BYTES = 3072;  // a stage: four chunks of INT2, two of INT4, one of INT8
+constexpr int MAX_X_STAGES = 6;
+static_assert(FIRST_A_COLUMN + A_SLOTS * SLOT_COLUMNS == 512, "tensor memory");
+
+struct Control {
+  unsigned long long x_full[MAX_X_STAGES], x_empty[MAX_X_STAGES];
+  unsigned long long a_full[A_SLOTS], a_empty[A_SLOTS];
+  unsigned long long d_full[2], d_empty[2];
+  unsigned long long ring_full[DECODE_WARPS][RING_STAGES];
+  uint32_t tmem_base;
+  volatile uint32_t abort;
+};
+
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// One box into this block's shared memory; the bytes are counted by the leader's barrier.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(s32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(x), "r"(y)
+      : "memory");
+}
+// K-major 128-byte-swizzled operand: rows of 128 B, 8-row groups 1024 B apart.
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t saddr) {
+  uint64_t d = (uint64_t)((saddr & 0x3ffffu) >> 4);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// kind::f16, A (fp16) from tensor memory, B (fp16) K-major from shared memory, D fp32.
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint32_t a_tmem, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Arrives on the barrier at this offset in BOTH blocks once the products issued so far have finished.
+__device__ __forceinline__ void commit_both(unsigned long long* b) {
+  const unsigned short mask = 3;
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(s32(b)), "h"(mask)
+      : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+      "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// The lane's row (8 r + g of its group) in the chunk at `slab`: 64 weights as 32 pairs of neighbouring columns.
+struct LaneRow {
+  float lo_min[2], lo_scale[2];  // twice the same: two pieces are decoded together
+  __half2 step_scale;
+};
+template <int NBITS>
+__device__ __forceinline__ void decode_row(const uint8_t* slab, int g, int r, int shift, const LaneRow& row, uint32_t (&w)[32]) {
+  const uint16_t* pairs = reinterpret_cast<const uint16_t*>(slab + 256 * NBITS) + 4 * ((4 >> shift) * g) + r;
+  Ladder l[4];
+#pragma unroll
+  for (int t = 0; t < 4; t += 2)
+    ladders((uint32_t)pairs[4 * (t >> shift)] | (uint32_t)pairs[4 * ((t + 1) >> shift)] << 16, row.lo_min, row.lo_scale, row.step_scale,
+            l[t], l[t + 1]);
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(slab) + 16 * g + r;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int h = 0; h < NBITS / 2; ++h) {
+      const uint32_t q = words[128 * h + 4 * t];
+      if (NBITS == 2) decode_int2(q, l[t], w + 8 * t);
+      else if (NBITS == 4) decode_int4(q, l[t], w + 8 * t + 4 * h);
+      else decode_int8(q, l[t], w + 8 * t + 2 * h);
+    }
+}
+
+struct Shape {
+  int width;       // activation rows of a tile, a multiple of 16
+  int x_stages;
+};
+
+// What one item of work is: a tile of activation rows and two tiles of packed rows.
+struct Item {
+  TokenTile tile;
+  int row_tile;    // of this block; may lie behind the last one
+};
+__device__ __forceinline__ bool get_item(const Product& p, int64_t item, int row_pairs, uint32_t rank, Item& out) {
+  if (!p.tiles.get(item / row_pairs, out.tile)) return false;
+  out.row_tile = (int)(item % row_pairs) * 2 + (int)rank;
+  return true;
+}
+
+// One warp's packed data of one item.
+struct Stream {
+  const uint8_t* src;
+  int slab, per_copy, chunks, copies;
+};
+__device__ __forceinline__ GroupForm group_form(const Product& p, const Item& item, int quarter) {
+  if (item.row_tile >= (int)(p.w.groups_per_expert / 4)) return GroupForm{0, 0};
+  return load_group(p.w.groups, (int64_t)item.tile.expert * p.w.groups_per_expert + item.row_tile * 4 + quarter);
+}
+__device__ __forceinline__ Stream stream_of(const Product& p, GroupForm form, int half, int half0, int chunks) {
+  Stream s;
+  s.slab = form.slab_bytes(), s.per_copy = 8 >> form.width();
+  s.chunks = half == 0 ? half0 : chunks - half0;
+  s.copies = s.slab == 0 ? 0 : (s.chunks + s.per_copy - 1) / s.per_copy;
+  s.src = static_cast<const uint8_t*>(p.w.data) + (int64_t)form.base * 16 + (int64_t)(half == 0 ? 0 : half0) * s.slab;
+  return s;
+}
+
+// This lane's column of 16 activation rows of a finished tile; the residuals are read before the stores that they
+// could otherwise not pass.
+template <typename T>
+__device__ __forceinline__ void put_columns(const Epilogue& out, float (&v)[16], int count, int64_t row, uint32_t col, float bias) {
+  T* const to = static_cast<T*>(out.out) + row * out.ld_out + col;
+  T res[16];
+  if (out.residual != nullptr) {
+    const T* const from = static_cast<const T*>(out.residual) + row * out.ld_residual + col;
+#pragma unroll
+    for (int t = 0; t < 16; ++t)
+      if (t < count) res[t] = from[t * out.ld_residual];
+  }
+#pragma unroll
+  for (int t = 0; t < 16; ++t) v[t] += bias;
+  switch (out.act) {  // (outside the loop: one activation's code at a time)
+    case HI2_ACT_RELU:
+#pragma unroll
+      for (int t = 0; t < 16; ++t) v[t] = activate(v[t], HI2_ACT_RELU);
+      break;
+    case HI2_ACT_SILU:
+#pragma unroll
+      for (int t = 0; t < 16; ++t) v[t] = activate(v[t], HI2_ACT_SILU);
+      break;
+    case HI2_ACT_GELU:
+#pragma unroll 2
+      for (int t = 0; t < 16; ++t) v[t] = activate(v[t], HI2_ACT_GELU);
+      break;
+    case HI2_ACT_GELU_TANH:
+#pragma unroll 4
+      for (int t = 0; t < 16; ++t) v[t] = activate(v[t], HI2_ACT_GELU_TANH);
+      break;
+    default: break;
+  }
+  if (out.residual != nullptr) {
+#pragma unroll
+    for (int t = 0; t < 16; ++t)
+      if (t < count) v[t] += to_float(res[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < 16; ++t)
+    if (t < count) to[t * out.ld_out] = from_float<T>(v[t]);
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shape shape) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  const int box_bytes = shape.width / 2 * CHUNK * 2;    // one chunk of one part: this block's half of the rows
+  const int stage_bytes = 2 * p.parts * box_bytes;
+  uint8_t* rings = smem + (size_t)shape.x_stages * stage_bytes;
+  Control* ctl = reinterpret_cast<Control*>(rings + DECODE_WARPS * RING_STAGES * RING_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_rank();
+  int32_t* const status = p.w.status;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < shape.x_stages; ++s) bar_init(&ctl->x_full[s], 1), bar_init(&ctl->x_empty[s], 1);
+    for (int s = 0; s < A_SLOTS; ++s) bar_init(&ctl->a_full[s], 2 * DECODE_WARPS), bar_init(&ctl->a_empty[s], 1);
+    for (int b = 0; b < 2; ++b) bar_init(&ctl->d_full[b], 1), bar_init(&ctl->d_empty[b], 2 * EPILOGUE_WARPS);
+    for (int w = 0; w < DECODE_WARPS; ++w)
+      for (int s = 0; s < RING_STAGES; ++s) bar_init(&ctl->ring_full[w][s], 1);
+    ctl->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&ctl->tmem_base)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  cluster_sync();  // the peer's barriers exist before anything signals them
+  fence_after();
+  const uint32_t tmem = ctl->tmem_base;
+  const uint32_t a_tmem = tmem + FIRST_A_COLUMN;
+  const int chunks = (int)(p.w.k / CHUNK), half0 = (chunks + 1) / 2;  // a step: one chunk of each half of the columns
+  const int row_pairs = (int)((p.w.groups_per_expert / 4 + 1) / 2);
+  const int64_t first_item = blockIdx.x >> 1, stride = gridDim.x >> 1;
+  chain_wait();  // the tile list, the activations, and whatever the outputs overwrite
+  bool ok = true;
+  Item item;
+
+  if (warp < DECODE_WARPS) {
+    // ------------------------------------------------------------ decode
+    const int quarter = warp & 3, half = warp >> 2, g = lane & 7, r = lane >> 3;
+    uint8_t* ring = rings + warp * RING_STAGES * RING_BYTES;
+    // the ring is filled ahead of the item being decoded, by one lane with a cursor of its own
+    int64_t ahead_item = first_item;
+    int ahead_copy = 0, ahead_stage = 0;
+    Stream ahead{nullptr, 0, 1, 0, 0};
+    bool more = get_item(p, ahead_item, row_pairs, rank, item);
+    if (more) ahead = stream_of(p, group_form(p, item, quarter), half, half0, chunks);
+    auto produce = [&]() {
+      while (more && ahead_copy == ahead.copies) {
+        ahead_item += stride, ahead_copy = 0;
+        Item next;
+        more = get_item(p, ahead_item, row_pairs, rank, next);
+        if (more) ahead = stream_of(p, group_form(p, next, quarter), half, half0, chunks);
+      }
+      if (!more) return;
+      const int from = ahead_copy * ahead.per_copy, bytes = min(ahead.per_copy, ahead.chunks - from) * ahead.slab;
+      bar_expect(&ctl->ring_full[warp][ahead_stage], (uint32_t)bytes);
+      bulk_load(ring + ahead_stage * RING_BYTES, ahead.src + (int64_t)from * ahead.slab, (uint32_t)bytes, &ctl->ring_full[warp][ahead_stage]);
+      ahead_stage = ahead_stage + 1 == RING_STAGES ? 0 : ahead_stage + 1;
+      ++ahead_copy;
+    };
+    if (lane == 0)
+      for (int s = 0; s < RING_STAGES; ++s) produce();
+    int stage = 0, slot = 0;
+    uint32_t phase = 0, slot_phase = 1;
+    for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
+      const GroupForm form = group_form(p, item, quarter);
+      const Stream s = stream_of(p, form, half, half0, chunks);
+      LaneRow row{};
+      if (s.slab != 0) {
+        const RowConsts c = load_row(p.w.rows, ((int64_t)item.tile.expert * p.w.groups_per_expert + item.row_tile * 4 + quarter) * GROUP_ROWS + lane);
+        row.lo_min[0] = row.lo_min[1] = c.lo_min(), row.lo_scale[0] = row.lo_scale[1] = c.lo_scale();
+        row.step_scale = __half2half2(__ushort_as_half((uint16_t)c.step_scale));
+      }
+      int in_copy = 0;
+      for (int i = 0; i < half0; ++i) {
+        const bool mine = i < s.chunks;  // the second half of an odd number of chunks lacks the last one
+        uint32_t w[32];
+        if (mine && s.slab != 0) {
+          if (in_copy == 0) {
+            ok = __all_sync(0xffffffffu, bar_wait(&ctl->ring_full[warp][stage], phase, &ctl->abort, status));
+            if (!ok) break;
+          }
+          const uint8_t* slab = ring + stage * RING_BYTES + in_copy * s.slab;
+          if (form.width() == 1) decode_row<2>(slab, g, r, form.shift(), row, w);
+          else if (form.width() == 2) decode_row<4>(slab, g, r, form.shift(), row, w);
+          else decode_row<8>(slab, g, r, form.shift(), row, w);
+          if (++in_copy == s.per_copy || i == s.chunks - 1) {
+            in_copy = 0;
+            __syncwarp();  // every lane has read the stage
+            if (lane == 0) produce();
+            __syncwarp();
+            if (++stage == RING_STAGES) stage = 0, phase ^= 1;
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 32; ++q) w[q] = 0;
+        }
+        ok = __all_sync(0xffffffffu, bar_wait(&ctl->a_empty[slot], slot_phase, &ctl->abort, status));
+        if (!ok) break;
+        fence_after();
+        if (mine) tmem_store32(a_tmem + slot * SLOT_COLUMNS + half * A_COLUMNS + ((uint32_t)(quarter * 32) << 16), w);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive_cluster(in_rank(s32(&ctl->a_full[slot]), 0));
+        if (++slot == A_SLOTS) slot = 0, slot_phase ^= 1;
+      }
+    }
+  } else if (warp == X_WARP) {
+    // ------------------------------------------------------------ activations
+    int stage = 0;
+    uint32_t phase = 1;
+    for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
+      const int cols = (item.tile.end - item.tile.begin + 15) & ~15;  // of the product
+      const int y = item.tile.begin + (int)rank * (cols / 2);
+      for (int i = 0; i < half0; ++i) {
+        ok = __all_sync(0xffffffffu, bar_wait(&ctl->x_empty[stage], phase, &ctl->abort, status));
+        if (!ok) break;
+        if (lane == 0) {
+          const bool two = half0 + i < chunks;
+          if (rank == 0) bar_expect(&ctl->x_full[stage], (uint32_t)((two ? 2 : 1) * p.parts * box_bytes * 2));  // both blocks' bytes
+          const uint32_t full = in_rank(s32(&ctl->x_full[stage]), 0);
+          uint8_t* dst = smem + (size_t)stage * stage_bytes;
+          for (int part = 0; part < p.parts; ++part) {
+            tma_load_pair(dst + part * box_bytes, &map, full, i * CHUNK, (int)(part * p.tiles.rows) + y);
+            if (two) tma_load_pair(dst + (p.parts + part) * box_bytes, &map, full, (half0 + i) * CHUNK, (int)(part * p.tiles.rows) + y);
+          }
+        }
+        __syncwarp();
+        if (++stage == shape.x_stages) stage = 0, phase ^= 1;
+      }
+    }
+  } else if (warp == MMA_WARP && rank == 0) {
+    // ------------------------------------------------------------ products (leading block only)
+    const uint32_t d_first = __shfl_sync(0xffffffffu, tmem, 0), a_first = __shfl_sync(0xffffffffu, a_tmem, 0);
+    const uint64_t b_first = desc_kmajor(s32(smem));
+    const uint32_t box = (uint32_t)box_bytes >> 4;
+    int stage = 0, slot = 0, buf = 0;
+    uint32_t phase = 0, slot_phase = 0, d_phase = 1;
+    for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
+      const int cols = (item.tile.end - item.tile.begin + 15) & ~15;
+      // fp16 operands (format 0 at bits 7 and 10), fp32 accumulator (1 << 4), N >> 3 at bit 17, M >> 4 at bit 24
+      const uint32_t idesc = (1u << 4) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(2 * TILE_ROWS >> 4) << 24);
+      const uint32_t d = d_first + buf * MAX_WIDTH;
+      ok = __all_sync(0xffffffffu, bar_wait(&ctl->d_empty[buf], d_phase, &ctl->abort, status));
+      if (!ok) break;
+      for (int i = 0; i < half0; ++i) {
+        const uint32_t a = a_first + slot * SLOT_COLUMNS;
+        const uint64_t b = b_first + (uint32_t)(stage * stage_bytes >> 4);
+        ok = bar_wait(&ctl->x_full[stage], phase, &ctl->abort, status);
+        ok = ok && bar_wait(&ctl->a_full[slot], slot_phase, &ctl->abort, status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        if (lane == 0) {
+          for (int part = 0; part < p.parts; ++part)
+#pragma unroll
+            for (int kk = 0; kk < CHUNK / 16; ++kk)
+              mma_pair(d, a + kk * 8, b + part * box + kk * 2, idesc, i > 0 || part > 0 || kk > 0 ? 1u : 0u);
+          if (half0 + i < chunks)
+            for (int part = 0; part < p.parts; ++part)
+#pragma unroll
+              for (int kk = 0; kk < CHUNK / 16; ++kk)
+                mma_pair(d, a + A_COLUMNS + kk * 8, b + (p.parts + part) * box + kk * 2, idesc, 1u);
+          commit_both(&ctl->a_empty[slot]);
+          commit_both(&ctl->x_empty[stage]);
+          if (i == half0 - 1) commit_both(&ctl->d_full[buf]);
+        }
+        __syncwarp();
+        if (++stage == shape.x_stages) stage = 0, phase ^= 1;
+        if (++slot == A_SLOTS) slot = 0, slot_phase ^= 1;
+      }
+      if (++buf == 2) buf = 0, d_phase ^= 1;
+    }
+  } else if (warp >= FIRST_EPILOGUE) {
+    // ------------------------------------------------------------ epilogue
+    // a warp may only touch the 32 tensor-memory lanes of its index modulo 4
+    const int quarter = warp & 3, second = (warp - FIRST_EPILOGUE) >> 2;
+    int buf = 0;
+    uint32_t phase = 0;
+    for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
+      uint32_t col = NO_ROW;
+      if (item.row_tile < (int)(p.w.groups_per_expert / 4))
+        col = load_row(p.w.rows, ((int64_t)item.tile.expert * p.w.groups_per_expert + item.row_tile * 4 + quarter) * GROUP_ROWS + lane).out_row;
+      const float bias = p.out.bias != nullptr && col != NO_ROW ? load_as_float(p.out.bias, p.out.dtype, col) : 0.0f;
+      const int tokens = item.tile.end - item.tile.begin;
+      ok = __all_sync(0xffffffffu, bar_wait(&ctl->d_full[buf], phase, &ctl->abort, status));
+      if (!ok) break;
+      fence_after();
+      const uint32_t taddr = tmem + buf * MAX_WIDTH + ((uint32_t)(quarter * 32) << 16);
+      for (int t0 = 16 * second; t0 < tokens; t0 += 32) {
+        const int count = min(16, tokens - t0);
+        const int64_t first = item.tile.begin + t0;
+        float scale = 0.0f;  // lane t: of activation row t0 + t
+        if (lane < count) {
+          scale = p.row_scale[first + lane];
+          if (p.out.pair_weight != nullptr) scale *= p.out.pair_weight[p.tiles.pair(first + lane)];
+        }
+        float v[16];
+        tmem_load16(taddr + t0, v);
+#pragma unroll
+        for (int t = 0; t < 16; ++t) v[t] *= __shfl_sync(0xffffffffu, scale, t);
+        if (col != NO_ROW) {
+          if (p.out.dtype == HI2_BF16) put_columns<__nv_bfloat16>(p.out, v, count, first, col, bias);
+          else if (p.out.dtype == HI2_F16) put_columns<__half>(p.out, v, count, first, col, bias);
+          else put_columns<float>(p.out, v, count, first, col, bias);
+        }
+        __syncwarp();  // the next read of tensor memory is the whole warp's
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive_cluster(in_rank(s32(&ctl->d_empty[buf]), 0));
+      if (++buf == 2) buf = 0, phase ^= 1;
+    }
+  }
+  __syncwarp();
+
+  fence_before();
+  if (__syncthreads_or(ctl->abort != 0)) let_copies_land();
+  cluster_sync();  // neither block leaves while its peer may still signal it or read its operands
+  if (warp == MMA_WARP) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static EncodeFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<EncodeFn>(ptr);
+  }();
+  return fn;
+}
+
+}  // namespace
+
+int wide_width(int64_t rows) {
+  const int64_t tiles = ceil_div(rows, (int64_t)MAX_WIDTH);
+  return (int)(ceil_div(ceil_div(rows, tiles), (int64_t)16) * 16);
+}
+
+int product_wide(const Product& p, cudaStream_t stream, const char* what) {
+  EncodeFn enc = encoder();
+  if (enc == nullptr) return fail(HI2_ERR_DRIVER, "stored product: cuTensorMapEncodeTiled unavailable");
+  Shape s;
+  s.width = p.tiles.width;
+  const int stage_bytes = 2 * p.parts * (s.width / 2) * CHUNK * 2;
+  s.x_stages = 150 * 1024 / stage_bytes;  // at least three
+  if (s.x_stages > MAX_X_STAGES) s.x_stages = MAX_X_STAGES;
+  size_t smem = (size_t)s.x_stages * stage_bytes + DECODE_WARPS * RING_STAGES * RING_BYTES + sizeof(Control) + 1024;
+  // A block takes all of an SM's tensor memory: two must never be resident on one SM.
+  if (smem < 120 * 1024) smem = 120 * 1024;
+
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {(cuuint64_t)p.w.k, (cuuint64_t)(p.tiles.rows * p.parts)};
+  const cuuint64_t strides[1] = {(cuuint64_t)p.w.k * 2};
+  const cuuint32_t box[2] = {CHUNK, (cuuint32_t)(s.width / 2)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, p.xs, dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+    return HI2_ERR_DRIVER;
+  }
+  if (cudaFuncSetAttribute(wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return fail(HI2_ERR_LAUNCH, "stored product: cannot reserve shared memory");
+  int device = 0, sms = 148;
+  cudaGetDevice(&device);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  const int64_t items = (p.w.groups_per_expert / 4 + 1) / 2 * p.max_tiles;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = (unsigned)(2 * (items < sms / 2 ? items : sms / 2));
+  config.blockDim = THREADS, config.dynamicSmemBytes = smem, config.stream = stream;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute, config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, wide_kernel, map, p, s);
+  return check_launch(what);
+}
+
+}  // namespace stored
+}  // namespace hi2

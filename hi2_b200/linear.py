@@ -21,7 +21,7 @@ from .stack import MARK, stack_dims
 
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 CHUNK = 64  # columns that a row's codes are dealt out by
-_TILE_ROWS, _GROUP_ROWS = 128, 32
+_GROUP_ROWS, _TILE_GROUPS = 32, 4
 _DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
@@ -103,55 +103,47 @@ def _lay_out_on(f: dict, experts: int, rows: int, k: int, stacked: bool, dev: to
     if not all(good[1:]):
         raise ValueError("lay_out: the row offsets do not fit the buffers")
 
-    # rows by (block, width), a stable order; a tile's missing rows are padding behind them
-    padded = -(-rows // _TILE_ROWS) * _TILE_ROWS
+    # Rows by (block, width), a stable order.  Every format's rows fill groups of 32; the last one of each is
+    # filled up with padding, and so are the groups of an expert to whole tiles.
     shift = torch.log2(block.double()).round().long() - 4       # 0, 1, 2
     width = torch.log2(nbits.double()).round().long()           # 1, 2, 3
-    key = torch.full((experts, padded), 99, dtype=torch.int64, device=dev)
-    key[:, :rows] = (4 * shift + width).view(experts, rows)
-    key, order = torch.sort(key, dim=1, stable=True)
-    live = key < 99
+    key = (3 * shift + width - 1).view(experts, rows)
+    counts = torch.zeros(experts, 9, dtype=torch.int64, device=dev).scatter_add_(1, key, torch.ones_like(key))
+    groups = (counts + _GROUP_ROWS - 1) // _GROUP_ROWS
+    first = groups.cumsum(1) - groups                           # first group of every format
+    most = int(groups.sum(1).max())
+    per_expert = -(-most // _TILE_GROUPS) * _TILE_GROUPS
+    sorted_key, order = torch.sort(key, dim=1, stable=True)
+    before = counts.cumsum(1) - counts
+    place = _GROUP_ROWS * first.gather(1, sorted_key) + torch.arange(rows, device=dev) - before.gather(1, sorted_key)
     expert = torch.arange(experts, device=dev)[:, None]
-    src = torch.where(live, expert * rows + order, torch.full_like(order, -1))
-    at = src.clamp_min(0)
-    width = torch.where(live, width[at], torch.zeros_like(order))
-    shift = torch.where(live, shift[at], torch.zeros_like(order))
-
-    # per group of 32 rows: runs of one format, code pieces of 16 bytes run by run, then the parameter pairs
-    def grouped(t):
-        return t.view(-1, _GROUP_ROWS)
-
-    lane = torch.arange(_GROUP_ROWS, device=dev).expand(experts * padded // _GROUP_ROWS, -1)
-    gk = grouped(key)
-    begins = torch.cat([torch.ones_like(gk[:, :1], dtype=torch.bool), gk[:, 1:] != gk[:, :-1]], 1)
-    start = torch.where(begins, lane, torch.zeros_like(lane)).cummax(1).values
-    run = (gk[:, :, None] == gk[:, None, :]).sum(2)             # sorted: equal keys of a group are one run
-    pieces = torch.where(grouped(live), (1 << grouped(width)) // 2, torch.zeros_like(run))
-    before = pieces.cumsum(1) - pieces
-    piece = before.gather(1, start) + lane - start
-    pair_bytes = torch.where(grouped(live), 8 >> grouped(shift), torch.zeros_like(run))
-    pair_at = 16 * pieces.sum(1, keepdim=True) + pair_bytes.cumsum(1) - pair_bytes
-    units = (16 * pieces.sum(1) + pair_bytes.sum(1) + 15) // 16  # of 16 bytes, per chunk
+    src = torch.full((experts, per_expert * _GROUP_ROWS), -1, dtype=torch.int64, device=dev)
+    src.scatter_(1, place, expert * rows + order)
+    lead = src[:, ::_GROUP_ROWS].reshape(-1)                    # a group's first row is never padding, unless all are
+    at = lead.clamp_min(0)
+    live = lead >= 0
+    form = torch.where(live, width[at] | shift[at] << 2, torch.zeros_like(lead))
+    units = torch.where(live, (16 << width[at]) + (16 >> shift[at]), torch.zeros_like(lead))  # of 16 bytes, per chunk
     base = (units * (k // CHUNK)).cumsum(0)
     total_units = int(base[-1].item())
     if total_units >= 2**32:
         raise ValueError("lay_out: more than 64 GiB of packed rows")
     base = base - units * (k // CHUNK)
-    form = piece | (pair_at // 2) << 8 | grouped(width) << 20 | grouped(shift) << 22 | run << 24
-    form = torch.where(grouped(live), form, torch.zeros_like(form))
+    src = src.reshape(-1)
+    at = src.clamp_min(0)
     half = consts.view(torch.int16).long() & 0xFFFF
-    rows_t = torch.stack([form.reshape(-1), torch.where(live, order, torch.full_like(order, 2**32 - 1)).reshape(-1),
-                          (half[:, 0] | half[:, 1] << 16)[at].reshape(-1), half[:, 2][at].reshape(-1)], 1)
+    rows_t = torch.stack([torch.where(src >= 0, at % rows, torch.full_like(at, 2**32 - 1)),
+                          (half[:, 0] | half[:, 1] << 16)[at], half[:, 2][at], torch.zeros_like(at)], 1)
 
     def words(t):  # the low 32 bits
         return torch.where(t >= 2**31, t - 2**32, t).to(torch.int32).contiguous()
 
     tensors = dict(data=torch.zeros(max(total_units, 1) * 16, dtype=torch.uint8, device=dev),
-                   groups=words(torch.stack([base, units], 1)), rows=words(rows_t), had=had.contiguous(),
+                   groups=words(torch.stack([base, form], 1)), rows=words(rows_t), had=had.contiguous(),
                    inv_scale=None if scale is None else scale.reciprocal(),
                    status=torch.zeros(1, dtype=torch.int32, device=dev))
     w = StoredWeight((experts, rows, k), stacked, tensors)
-    src = src.reshape(-1).to(torch.int32)
+    src = src.to(torch.int32)
     _lib.call("hi2_lay_out_rows", w.arg, _lib.ptr(src), _lib.ptr(codes), _lib.ptr(code_off), _lib.ptr(params),
               _lib.ptr(param_off), _lib.ptr(tensors["data"]), _lib.stream(dev))
     torch.cuda.current_stream(dev).synchronize()  # complete for every stream that uses it later

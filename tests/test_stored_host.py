@@ -23,9 +23,10 @@ def test_stored_linear_arguments():
         return lib.hi2_stored_linear(C.byref(s), x, dtype, tokens, 128, None, act, None, 0, out, 64, ws, size, None)
 
     ok = _struct()
-    need = lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.BF16, 4)
-    assert need >= 4 * 128 * 2 + 4 * 4
-    assert lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.F32, 4) >= 2 * 4 * 128 * 2
+    assert lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.BF16, 4) == 0  # a few rows need none
+    need = lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.BF16, 400)
+    assert need >= 400 * 128 * 2 + 400 * 4
+    assert lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.F32, 400) >= 2 * 400 * 128 * 2
     assert call(ok, tokens=0) == _lib.OK
     for bad in (_struct(k=100), _struct(experts=2), _struct(data=None), _struct(groups_per_expert=3),
                 _struct(rows_per_expert=129), _struct(experts=0), _struct(k=0)):
@@ -33,7 +34,7 @@ def test_stored_linear_arguments():
     for kw in (dict(dtype=_lib.F64), dict(act=5), dict(act=-1), dict(tokens=-1), dict(tokens=1 << 31), dict(x=None), dict(out=None)):
         assert call(ok, **kw) == _lib.ERR_ARG
     for kw in (dict(ws=None), dict(size=need - 1), dict(ws=264)):
-        assert call(ok, **kw) == _lib.ERR_WORKSPACE
+        assert call(ok, tokens=400, **kw) == _lib.ERR_WORKSPACE
 
 
 def test_stored_experts_arguments():
