@@ -37,7 +37,7 @@ lay_out_kernel(const hi2_stored_weight w, const int32_t* __restrict__ src_row, c
       const uint32_t v = (uint32_t)words[q];
       uint32_t fields = 0;
       for (int f = 0; f < per_word; ++f) fields |= (v >> (f * nbits) & mask) << ((f >> 1) * nbits + (f & 1) * 16);
-      reinterpret_cast<uint32_t*>(slab)[128 * (q % per_piece) + 4 * (4 * g + q / per_piece) + r] = fields;
+      reinterpret_cast<uint32_t*>(slab)[128 * (q % per_piece) + code_word(g, q / per_piece) + r] = fields;
     }
     const int pairs = 4 >> form.shift();
     const uint8_t* from = blk_params + 2 * (param_off[src] + chunk * pairs);

@@ -5,9 +5,10 @@
 // chunks of 64 columns; a chunk (a slab) holds the codes of its 32 rows and behind them their (lo, step) byte
 // pairs, so a warp reads a run of chunks as one contiguous range.  Row 8 r + g of a group (g < 8, r < 4) has in
 // a chunk nbits / 2 words of codes for each of its four 16-column pieces t; word h of piece t lies at word
-// 128 h + 4 (4 g + t) + r, so one 128-bit read gives lane 4 g + t the same word of four rows, which is
-// what the fragments of a warp-level matrix product ask for.  The pairs lie the same way: pair (g, t, r) at
-// 16-bit unit 4 ((4 >> shift) g + (t >> shift)) + r with blocks of 16 << shift columns.
+// 128 h + 32 t + 4 ((g + 2 t) mod 8) + r.  One 128-bit read then gives lane 4 g + t the same word of four rows, which is
+// what the fragments of a warp-level matrix product ask for, and one 32-bit read a word of all 32 rows; both
+// without a bank conflict.  The pairs: pair (g, t, r) at 16-bit unit 4 ((4 >> shift) g + (t >> shift)) + r with
+// blocks of 16 << shift columns.
 // Inside a word the codes of even columns fill the low half from its low bits, those of odd columns the
 // high half, so that one mask extracts the codes of two neighbouring columns as an fp16 pair.
 #pragma once
@@ -24,9 +25,10 @@ constexpr int MAX_SLAB = 2304;   // bytes of a chunk of a group: INT8 in blocks 
 
 struct GroupForm {
   uint32_t base;   // first 16-byte unit of the data
-  uint32_t form;   // log2 of the code width (0: padding only, no data) | log2(block / 16) << 2
+  uint32_t form;   // log2 of the code width (0: padding only, no data) | log2(block / 16) << 2 | SMALL steps << 4
   __host__ __device__ int width() const { return form & 3; }
   __host__ __device__ int shift() const { return form >> 2 & 3; }
+  __host__ __device__ bool small_steps() const { return (form >> 4 & 1) != 0; }
   __host__ __device__ int code_bytes() const { return 256 << width(); }  // of a chunk
   __host__ __device__ int slab_bytes() const { return width() == 0 ? 0 : code_bytes() + (256 >> shift()); }
 };
@@ -49,55 +51,85 @@ __device__ __forceinline__ RowConsts load_row(const uint32_t* rows, int64_t i) {
   return RowConsts{v.x, v.y, v.z};
 }
 
+// First word of (g, t) in a chunk's codes.
+__host__ __device__ __forceinline__ int code_word(int g, int t) { return 32 * t + 4 * ((g + 2 * t) & 7); }
+
 __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ __half2 half2_of(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
-// A ladder as (lo, lo), (step, step).  The format defines lo = fp16(fma_f32(u, lo_scale, lo_min)) and
-// step = fp16(u * step_scale).
+// A ladder as (lo, lo), and (step, step) times the powers of two that the decoder below asks for.  The format
+// defines lo = fp16(fma_f32(u, lo_scale, lo_min)) and step = fp16(u * step_scale).
 struct Ladder {
-  __half2 lo, step;
+  __half2 lo, step[3];
 };
+// Two codes of neighbouring columns at bit `AT` of both halves of w -> fp16(lo + code * step).
+//
+// SMALL steps (of all rows of the group: at most 65504 / 2^20, for 8-bit codes 65504 / 2^22): the field by itself is
+// the fp16 subnormal code * 2^(AT - 24), and one fused multiply-add with step * 2^(24 - AT), an fp16 number for the
+// fields' bits 4, 6 and 8 (2-bit codes), 4 (4-bit), 2 (8-bit), forms the weight with the format's single rounding.
+// Any step: 1024 + code * 2^AT is an fp16 number with the code in its mantissa; a fused multiply-add takes
+// it to the code (exact), a second one forms the weight.  fp16 arithmetic issues every other clock and shares its pipe
+// with the warp-level products: 2048 INT2 weights and their products take a scheduler 172 clocks with small
+// steps (52 fp16 instructions and 8 products), 216 without (70 and 8).
+template <int AT, int NBITS, bool SMALL>
+__device__ __forceinline__ uint32_t weight_pair(uint32_t w, __half2 lo, __half2 step) {
+  constexpr uint32_t mask = ((1u << NBITS) - 1u) << AT;
+  if (SMALL) return bits(__hfma2(half2_of(w & (mask | mask << 16)), step, lo));
+  constexpr uint32_t scale = (uint32_t)(15 - AT) << 10, bias = 0x8000u | (uint32_t)(25 - AT) << 10;  // 2^-AT, -2^(10 - AT)
+  uint32_t field;  // (w & mask) | magic in one instruction
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(field) : "r"(w), "r"(mask | mask << 16), "r"(0x64006400u));
+  const __half2 code = AT == 0 ? __hadd2(half2_of(field), half2_of(bias | bias << 16))
+                               : __hfma2(half2_of(field), half2_of(scale | scale << 16), half2_of(bias | bias << 16));
+  return bits(__hfma2(code, step, lo));
+}
 // Two byte pairs of two rows (row 0 in the low half of `pairs`) -> their ladders.  2^23 + u and 1024 + u have
 // u in their low bits, so the bytes become numbers without a conversion; an fp16 product of a byte and
 // an fp16 number rounds once, as the fp32 product rounded to fp16 does (that one is exact).
+template <int NBITS, bool SMALL>
 __device__ __forceinline__ void ladders(uint32_t pairs, const float (&lo_min)[2], const float (&lo_scale)[2], __half2 step_scale,
                                         Ladder& a, Ladder& b) {
   const float u = __uint_as_float(__byte_perm(pairs, 0x4b000000u, 0x7440)) - 8388608.0f;
   const float v = __uint_as_float(__byte_perm(pairs, 0x4b000000u, 0x7442)) - 8388608.0f;
-  const uint32_t lo = bits(__floats2half2_rn(fmaf(u, lo_scale[0], lo_min[0]), fmaf(v, lo_scale[1], lo_min[1])));
+  const __half2 lo = __floats2half2_rn(fmaf(u, lo_scale[0], lo_min[0]), fmaf(v, lo_scale[1], lo_min[1]));
   const __half2 steps = __hadd2(half2_of(__byte_perm(pairs, 0x64646464u, 0x4341)), half2_of(0xe400e400u));
-  const uint32_t st = bits(__hmul2(steps, step_scale));
-  a = Ladder{half2_of(__byte_perm(lo, 0, 0x1010)), half2_of(__byte_perm(st, 0, 0x1010))};
-  b = Ladder{half2_of(__byte_perm(lo, 0, 0x3232)), half2_of(__byte_perm(st, 0, 0x3232))};
+  __half2 step[3];
+  step[0] = __hmul2(steps, step_scale);
+  if (SMALL) {  // 2^10, then 2^6, 2^8, 2^10 or 2^12 (2^20 and 2^22 are no fp16 numbers)
+    const __half2 up = __hmul2(step[0], half2_of(0x64006400u));
+    if (NBITS == 2) step[0] = __hmul2(up, half2_of(0x54005400u)), step[1] = __hmul2(up, half2_of(0x5c005c00u)), step[2] = __hmul2(up, half2_of(0x64006400u));
+    else step[0] = __hmul2(up, half2_of(NBITS == 4 ? 0x64006400u : 0x6c006c00u));
+  }
+  a.lo = __low2half2(lo), b.lo = __high2half2(lo);
+#pragma unroll
+  for (int i = 0; i < (SMALL && NBITS == 2 ? 3 : 1); ++i) a.step[i] = __low2half2(step[i]), b.step[i] = __high2half2(step[i]);
 }
 
-// Two codes at bit `AT` of both halves of w -> fp16(lo + code * step).  1024 + code * 2^AT is an fp16
-// number with the code in its mantissa; one fused multiply-add takes it to the code (exact), a second
-// forms the weight with the format's single rounding.
-template <int AT, int NBITS>
-__device__ __forceinline__ uint32_t weight_pair(uint32_t w, const Ladder& l) {
-  constexpr uint32_t mask = ((1u << NBITS) - 1u) << AT;
-  constexpr uint32_t scale = (uint32_t)(15 - AT) << 10, bias = 0x8000u | (uint32_t)(25 - AT) << 10;  // 2^-AT, -2^(10 - AT)
-  uint32_t field;  // (w & mask) | magic in one instruction
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(field) : "r"(w), "r"(mask | mask << 16), "r"(0x64006400u));
-  const __half2 raw = half2_of(field);
-  const __half2 code = AT == 0 ? __hadd2(raw, half2_of(bias | bias << 16)) : __hfma2(raw, half2_of(scale | scale << 16), half2_of(bias | bias << 16));
-  return bits(__hfma2(code, l.step, l.lo));
-}
-// The words of a 16-column piece -> 8 pairs of neighbouring columns.
-__device__ __forceinline__ void decode_int2(uint32_t w, const Ladder& l, uint32_t* out) {
-  out[0] = weight_pair<0, 2>(w, l), out[1] = weight_pair<2, 2>(w, l), out[2] = weight_pair<4, 2>(w, l);
-  out[3] = weight_pair<6, 2>(w, l), out[4] = weight_pair<8, 2>(w, l);
-  w >>= 10;
-  out[5] = weight_pair<0, 2>(w, l), out[6] = weight_pair<2, 2>(w, l), out[7] = weight_pair<4, 2>(w, l);
-}
-__device__ __forceinline__ void decode_int4(uint32_t w, const Ladder& l, uint32_t* out) {  // one of two words
-  out[0] = weight_pair<0, 4>(w, l), out[1] = weight_pair<4, 4>(w, l);
-  w >>= 8;
-  out[2] = weight_pair<0, 4>(w, l), out[3] = weight_pair<4, 4>(w, l);
-}
-__device__ __forceinline__ void decode_int8(uint32_t w, const Ladder& l, uint32_t* out) {  // one of four words
-  out[0] = weight_pair<0, 8>(w, l), out[1] = weight_pair<0, 8>(w >> 8, l);
+// Word h of a 16-column piece -> its pairs of neighbouring columns.
+template <int NBITS, bool SMALL>
+__device__ __forceinline__ void decode_word(uint32_t w, const Ladder& l, uint32_t* out) {
+  const __half2 lo = l.lo, st = l.step[0];
+  if (NBITS == 2 && SMALL) {
+    const uint32_t up = w << 6, down = w >> 6;
+    out[0] = weight_pair<6, 2, true>(up, lo, l.step[1]), out[1] = weight_pair<8, 2, true>(up, lo, st);
+    out[2] = weight_pair<4, 2, true>(w, lo, l.step[2]), out[3] = weight_pair<6, 2, true>(w, lo, l.step[1]), out[4] = weight_pair<8, 2, true>(w, lo, st);
+    out[5] = weight_pair<4, 2, true>(down, lo, l.step[2]), out[6] = weight_pair<6, 2, true>(down, lo, l.step[1]), out[7] = weight_pair<8, 2, true>(down, lo, st);
+  } else if (NBITS == 2) {
+    out[0] = weight_pair<0, 2, false>(w, lo, st), out[1] = weight_pair<2, 2, false>(w, lo, st), out[2] = weight_pair<4, 2, false>(w, lo, st);
+    out[3] = weight_pair<6, 2, false>(w, lo, st), out[4] = weight_pair<8, 2, false>(w, lo, st);
+    w >>= 10;
+    out[5] = weight_pair<0, 2, false>(w, lo, st), out[6] = weight_pair<2, 2, false>(w, lo, st), out[7] = weight_pair<4, 2, false>(w, lo, st);
+  } else if (NBITS == 4 && SMALL) {
+    out[0] = weight_pair<4, 4, true>(w << 4, lo, st), out[1] = weight_pair<4, 4, true>(w, lo, st);
+    out[2] = weight_pair<4, 4, true>(w >> 4, lo, st), out[3] = weight_pair<4, 4, true>(w >> 8, lo, st);
+  } else if (NBITS == 4) {
+    out[0] = weight_pair<0, 4, false>(w, lo, st), out[1] = weight_pair<4, 4, false>(w, lo, st);
+    w >>= 8;
+    out[2] = weight_pair<0, 4, false>(w, lo, st), out[3] = weight_pair<4, 4, false>(w, lo, st);
+  } else if (SMALL) {
+    out[0] = weight_pair<2, 8, true>(w << 2, lo, st), out[1] = weight_pair<2, 8, true>(w >> 6, lo, st);
+  } else {
+    out[0] = weight_pair<0, 8, false>(w, lo, st), out[1] = weight_pair<0, 8, false>(w >> 8, lo, st);
+  }
 }
 
 // ---- what follows a product ---------------------------------------------------------------------------

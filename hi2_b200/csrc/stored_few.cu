@@ -14,6 +14,8 @@
 // inside a chunk is the same permutation for both operands, so a lane's 16 columns are contiguous in memory.
 // The tensor pipe is idle most of the time; what bounds the kernel is the decoding, about 150 instructions per
 // warp for 2048 INT2 weights, and behind it the packed bytes.
+#include <type_traits>
+
 #include "stored_async.cuh"
 
 namespace hi2 {
@@ -39,9 +41,9 @@ struct Shared {
   unsigned long long full[WARPS][RING_STAGES];
   volatile uint32_t abort;
 };
-template <int NT>
-size_t smem_bytes(int parts) {
-  return sizeof(Shared<NT>) + (size_t)parts * 8 * NT * X_PITCH * sizeof(__half) + 16;
+template <int NT, int PARTS>
+constexpr size_t smem_bytes() {
+  return sizeof(Shared<NT>) + (size_t)PARTS * 8 * NT * X_PITCH * sizeof(__half) + 16;
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -56,30 +58,69 @@ struct LaneRows {
   float lo_min[4], lo_scale[4];
   __half2 step_scale[2];
 };
-template <int NBITS>
-__device__ __forceinline__ void decode_rows(const uint8_t* slab, int lane, int pair_unit, const LaneRows& rows, uint32_t (&w)[4][8]) {
+template <int NBITS, bool SMALL>
+__device__ __forceinline__ void decode_rows(const uint8_t* slab, int first_word, int pair_unit, const LaneRows& rows, uint32_t (&w)[4][8]) {
   const uint2 pairs = *reinterpret_cast<const uint2*>(slab + 256 * NBITS + 8 * pair_unit);
   Ladder l[4];
   {
     const float min01[2] = {rows.lo_min[0], rows.lo_min[1]}, scale01[2] = {rows.lo_scale[0], rows.lo_scale[1]};
     const float min23[2] = {rows.lo_min[2], rows.lo_min[3]}, scale23[2] = {rows.lo_scale[2], rows.lo_scale[3]};
-    ladders(pairs.x, min01, scale01, rows.step_scale[0], l[0], l[1]);
-    ladders(pairs.y, min23, scale23, rows.step_scale[1], l[2], l[3]);
+    ladders<NBITS, SMALL>(pairs.x, min01, scale01, rows.step_scale[0], l[0], l[1]);
+    ladders<NBITS, SMALL>(pairs.y, min23, scale23, rows.step_scale[1], l[2], l[3]);
   }
 #pragma unroll
   for (int h = 0; h < NBITS / 2; ++h) {
-    const uint4 v = *reinterpret_cast<const uint4*>(slab + 512 * h + 16 * lane);
+    const uint4 v = *reinterpret_cast<const uint4*>(slab + 512 * h + 4 * first_word);
     const uint32_t q[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (NBITS == 2) decode_int2(q[r], l[r], w[r]);
-      else if (NBITS == 4) decode_int4(q[r], l[r], w[r] + 4 * h);
-      else decode_int8(q[r], l[r], w[r] + 2 * h);
-    }
+    for (int r = 0; r < 4; ++r) decode_word<NBITS, SMALL>(q[r], l[r], w[r] + 16 / NBITS * h);
   }
 }
 
-template <int NT>
+// Where a warp is in its ring.
+struct Ring {
+  uint8_t* data;
+  unsigned long long* full;
+  int slab, stage;  // bytes of a chunk; stage
+  uint32_t phase;
+};
+
+// `count` chunks against the activations at x.  False when a wait ran out.
+template <int NT, int PARTS, int NBITS, bool SMALL, typename REFILL>
+__device__ __forceinline__ bool multiply(Ring& ring, const __half* x, int count, int first_word, int pair_unit, const LaneRows& rows,
+                                         float (&acc)[2][NT][4], volatile uint32_t* abort, int32_t* status, const REFILL& refill) {
+  constexpr int PER_COPY = 8 / NBITS;
+  while (count > 0) {
+    if (!__all_sync(0xffffffffu, bar_wait(ring.full + ring.stage, ring.phase, abort, status))) return false;
+    const int here = min(PER_COPY, count);
+    const uint8_t* slab = ring.data + ring.stage * RING_BYTES;
+#pragma unroll 1  // (unrolled, the loops of the code widths push one another out of the instruction cache)
+    for (int i = 0; i < here; ++i, x += CHUNK, slab += ring.slab) {
+      uint32_t w[4][8];
+      decode_rows<NBITS, SMALL>(slab, first_word, pair_unit, rows, w);
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int q = 0; q < NT; ++q) {
+          const __half* from = x + (part * 8 * NT + q * 8) * X_PITCH;
+          const uint4 x0 = *reinterpret_cast<const uint4*>(from), x1 = *reinterpret_cast<const uint4*>(from + 8);
+          const uint32_t k[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            mma(acc[0][q], w[0][2 * s], w[1][2 * s], w[0][2 * s + 1], w[1][2 * s + 1], k[2 * s], k[2 * s + 1]);
+            mma(acc[1][q], w[2][2 * s], w[3][2 * s], w[2][2 * s + 1], w[3][2 * s + 1], k[2 * s], k[2 * s + 1]);
+          }
+        }
+    }
+    count -= here;
+    __syncwarp();  // every lane has read the stage
+    refill(ring.stage);
+    if (++ring.stage == RING_STAGES) ring.stage = 0, ring.phase ^= 1;
+  }
+  return true;
+}
+
+template <int NT, int PARTS>
 __global__ void __launch_bounds__(THREADS, NT < 4 ? 2 : 1)
 few_kernel(const Product p, const int split) {
   extern __shared__ __align__(16) uint8_t raw[];
@@ -106,6 +147,9 @@ few_kernel(const Product p, const int split) {
   const int mine = (blocks - 1) * HALF_CHUNKS + last_mine;
   const int64_t group = (int64_t)tile.expert * p.w.groups_per_expert + row_tile * 4 + quarter;
   const GroupForm form = load_group(p.w.groups, group);
+  RowConsts consts[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) consts[r] = load_row(p.w.rows, group * GROUP_ROWS + 8 * r + g);
   const int slab = form.slab_bytes(), copy_shift = 3 - form.width(), per_copy = 1 << copy_shift;  // 4, 2, 1 chunks
   const uint8_t* const data = static_cast<const uint8_t*>(p.w.data) + (int64_t)form.base * 16;
   const int copies = form.width() == 0 ? 0 : (mine + per_copy - 1) >> copy_shift;
@@ -125,14 +169,14 @@ few_kernel(const Product p, const int split) {
   LaneRows rows;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const RowConsts c = load_row(p.w.rows, group * GROUP_ROWS + 8 * r + g);
+    const RowConsts c = consts[r];
     rows.lo_min[r] = c.lo_min(), rows.lo_scale[r] = c.lo_scale();
     const __half s = __ushort_as_half((uint16_t)c.step_scale);
     if (r & 1) rows.step_scale[r / 2] = __halves2half2(__low2half(rows.step_scale[r / 2]), s);
     else rows.step_scale[r / 2] = __half2half2(s);
     if (half == 0 && t == 0) sm.out_row[quarter * 32 + 8 * r + g] = c.out_row;
   }
-  const int pair_unit = (4 >> form.shift()) * g + (t >> form.shift());
+  const int pair_unit = (4 >> form.shift()) * g + (t >> form.shift()), first_word = code_word(g, t);
 
   float total[2][NT][4];
 #pragma unroll
@@ -144,8 +188,13 @@ few_kernel(const Product p, const int split) {
 
   chain_wait();  // the activations
   bool ok = true;
-  int copy = 0, at = 0, stage = 0;  // of the ring: copy, chunk inside it, stage
-  uint32_t phase = 0;
+  Ring ring{&sm.ring[warp][0][0], &sm.full[warp][0], slab, 0, 0};
+  int next_copy = RING_STAGES;
+  auto refill = [&](int stage) {
+    if (lane == 0 && next_copy < copies) issue(next_copy, stage);
+    ++next_copy;
+    __syncwarp();
+  };
   for (int b = 0; b < blocks; ++b) {
     const int chunks = b == blocks - 1 ? last_chunks : BLOCK_CHUNKS;
     const int half0 = b == blocks - 1 ? last_half0 : HALF_CHUNKS;
@@ -172,7 +221,7 @@ few_kernel(const Product p, const int split) {
         split16(v, power.to, hi, lo);
         uint4* dst = reinterpret_cast<uint4*>(xs + r * X_PITCH + piece * 16);
         dst[0] = hi[0], dst[1] = hi[1];
-        if (p.parts == 2) {
+        if (PARTS == 2) {
           dst = reinterpret_cast<uint4*>(xs + (8 * NT + r) * X_PITCH + piece * 16);
           dst[0] = lo[0], dst[1] = lo[1];
         }
@@ -188,38 +237,19 @@ few_kernel(const Product p, const int split) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[m][q][i] = 0.0f;
     const int first = half == 0 ? 0 : half0, count = half == 0 ? half0 : chunks - half0;
-    if (copies > 0 && ok)
-      for (int i = 0; i < count; ++i) {
-        if (at == 0) {
-          ok = __all_sync(0xffffffffu, bar_wait(&sm.full[warp][stage], phase, &sm.abort, status));
-          if (!ok) break;
-        }
-        const uint8_t* from = sm.ring[warp][stage] + at * slab;
-        uint32_t w[4][8];
-        if (form.width() == 1) decode_rows<2>(from, lane, pair_unit, rows, w);
-        else if (form.width() == 2) decode_rows<4>(from, lane, pair_unit, rows, w);
-        else decode_rows<8>(from, lane, pair_unit, rows, w);
-        for (int part = 0; part < p.parts; ++part) {
-          const __half* x = xs + (part * 8 * NT + g) * X_PITCH + (first + i) * CHUNK + 16 * t;
-#pragma unroll
-          for (int q = 0; q < NT; ++q) {
-            const uint4 x0 = *reinterpret_cast<const uint4*>(x + q * 8 * X_PITCH), x1 = *reinterpret_cast<const uint4*>(x + q * 8 * X_PITCH + 8);
-            const uint32_t k[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              mma(acc[0][q], w[0][2 * s], w[1][2 * s], w[0][2 * s + 1], w[1][2 * s + 1], k[2 * s], k[2 * s + 1]);
-              mma(acc[1][q], w[2][2 * s], w[3][2 * s], w[2][2 * s + 1], w[3][2 * s + 1], k[2 * s], k[2 * s + 1]);
-            }
-          }
-        }
-        if (++at == per_copy) {
-          __syncwarp();  // every lane has read the stage
-          if (lane == 0 && copy + RING_STAGES < copies) issue(copy + RING_STAGES, stage);
-          __syncwarp();
-          ++copy, at = 0;
-          if (++stage == RING_STAGES) stage = 0, phase ^= 1;
-        }
-      }
+    if (ok) {  // one loop per code width
+      const __half* x = xs + g * X_PITCH + first * CHUNK + 16 * t;
+      const auto run = [&](auto nbits, auto small) {
+        return multiply<NT, PARTS, decltype(nbits)::value, decltype(small)::value>(ring, x, count, first_word, pair_unit, rows, acc, &sm.abort,
+                                                                                   status, refill);
+      };
+      typedef std::integral_constant<int, 2> Int2;
+      typedef std::integral_constant<int, 4> Int4;
+      typedef std::integral_constant<int, 8> Int8;
+      if (form.width() == 1) ok = form.small_steps() ? run(Int2(), std::true_type()) : run(Int2(), std::false_type());
+      else if (form.width() == 2) ok = form.small_steps() ? run(Int4(), std::true_type()) : run(Int4(), std::false_type());
+      else if (form.width() == 3) ok = form.small_steps() ? run(Int8(), std::true_type()) : run(Int8(), std::false_type());
+    }
 #pragma unroll
     for (int q = 0; q < NT; ++q) {
       const float s0 = sm.scale[b & 1][half][8 * q + 2 * t], s1 = sm.scale[b & 1][half][8 * q + 2 * t + 1];
@@ -267,10 +297,10 @@ few_kernel(const Product p, const int split) {
   if (split > 1) cluster_sync();  // nobody reads this block's sums any more
 }
 
-template <int NT>
+template <int NT, int PARTS>
 int launch(const Product& p, int split, cudaStream_t stream, const char* what) {
-  const size_t smem = smem_bytes<NT>(p.parts);
-  if (cudaFuncSetAttribute(few_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  const size_t smem = smem_bytes<NT, PARTS>();
+  if (cudaFuncSetAttribute(few_kernel<NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return fail(HI2_ERR_LAUNCH, "stored product: cannot reserve shared memory");
   const int64_t blocks = p.w.groups_per_expert / 4 * p.max_tiles * split;
   if (blocks >= (int64_t)1 << 31) return fail(HI2_ERR_ARG, "stored product: too many tiles");
@@ -282,7 +312,7 @@ int launch(const Product& p, int split, cudaStream_t stream, const char* what) {
   attribute[1].id = cudaLaunchAttributeClusterDimension;
   attribute[1].val.clusterDim.x = split, attribute[1].val.clusterDim.y = 1, attribute[1].val.clusterDim.z = 1;
   config.attrs = attribute, config.numAttrs = 2;
-  cudaLaunchKernelEx(&config, few_kernel<NT>, p, split);
+  cudaLaunchKernelEx(&config, few_kernel<NT, PARTS>, p, split);
   return check_launch(what);
 }
 
@@ -301,9 +331,10 @@ int product_few(const Product& p, cudaStream_t stream, const char* what) {
     const int64_t cost = ceil_div(tiles * s, room) * (ceil_div(chunks, (int64_t)s) + 12);
     if (cost < least) least = cost, split = s;
   }
-  if (p.tiles.width <= 8) return launch<1>(p, split, stream, what);
-  if (p.tiles.width <= 16) return launch<2>(p, split, stream, what);
-  return launch<4>(p, split, stream, what);
+  const bool one = p.parts == 1;
+  if (p.tiles.width <= 8) return one ? launch<1, 1>(p, split, stream, what) : launch<1, 2>(p, split, stream, what);
+  if (p.tiles.width <= 16) return one ? launch<2, 1>(p, split, stream, what) : launch<2, 2>(p, split, stream, what);
+  return one ? launch<4, 1>(p, split, stream, what) : launch<4, 2>(p, split, stream, what);
 }
 
 }  // namespace stored

@@ -13,12 +13,14 @@
 //
 // Blocks stay for many tiles.  Warps 0..7 decode (warp w: rows 32 (w mod 4) .. of the block's tile, one half of the
 // columns), every warp with its own ring of bulk copies that runs on into the next tile; warp 8 loads activations, warp 9
-// issues; warps 10..17 take finished tiles out of one of two accumulators (2 x 192 columns, beside two slots of 2 x 32
+// issues; warps 10..13 take finished tiles out of one of two accumulators (2 x 192 columns, beside two slots of 2 x 32
 // columns for decoded chunks) while the next tile is computed in the other.  A step is one chunk of each
 // half of the columns, in a fixed order: equal inputs give equal bits.
 //
 // Every mbarrier wait is bounded by a clock limit and raises *status.
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "stored_async.cuh"
 
@@ -26,7 +28,7 @@ namespace hi2 {
 namespace stored {
 namespace {
 
-constexpr int DECODE_WARPS = 8, X_WARP = 8, MMA_WARP = 9, FIRST_EPILOGUE = 10, EPILOGUE_WARPS = 8;
+constexpr int DECODE_WARPS = 8, X_WARP = 8, MMA_WARP = 9, FIRST_EPILOGUE = 10, EPILOGUE_WARPS = 4;
 constexpr int THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE_WARPS);
 constexpr int MAX_WIDTH = 192;
 constexpr int A_SLOTS = 2, A_COLUMNS = CHUNK / 2, SLOT_COLUMNS = 2 * A_COLUMNS;
@@ -117,24 +119,70 @@ struct LaneRow {
   float lo_min[2], lo_scale[2];  // twice the same: two pieces are decoded together
   __half2 step_scale;
 };
-template <int NBITS>
+template <int NBITS, bool SMALL>
 __device__ __forceinline__ void decode_row(const uint8_t* slab, int g, int r, int shift, const LaneRow& row, uint32_t (&w)[32]) {
   const uint16_t* pairs = reinterpret_cast<const uint16_t*>(slab + 256 * NBITS) + 4 * ((4 >> shift) * g) + r;
   Ladder l[4];
 #pragma unroll
   for (int t = 0; t < 4; t += 2)
-    ladders((uint32_t)pairs[4 * (t >> shift)] | (uint32_t)pairs[4 * ((t + 1) >> shift)] << 16, row.lo_min, row.lo_scale, row.step_scale,
+    ladders<NBITS, SMALL>((uint32_t)pairs[4 * (t >> shift)] | (uint32_t)pairs[4 * ((t + 1) >> shift)] << 16, row.lo_min, row.lo_scale, row.step_scale,
             l[t], l[t + 1]);
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(slab) + 16 * g + r;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(slab) + r;
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int h = 0; h < NBITS / 2; ++h) {
-      const uint32_t q = words[128 * h + 4 * t];
-      if (NBITS == 2) decode_int2(q, l[t], w + 8 * t);
-      else if (NBITS == 4) decode_int4(q, l[t], w + 8 * t + 4 * h);
-      else decode_int8(q, l[t], w + 8 * t + 2 * h);
+    for (int h = 0; h < NBITS / 2; ++h) decode_word<NBITS, SMALL>(words[128 * h + code_word(g, t)], l[t], w + 8 * t + 16 / NBITS * h);
+}
+
+// One warp's packed data of one item.
+struct Stream {
+  const uint8_t* src;
+  int slab, per_copy, chunks, copies;
+};
+
+// A decoding warp's place in its ring and among the slots of decoded chunks.
+struct Decoder {
+  Control* ctl;
+  int32_t* status;
+  const uint8_t* ring;
+  unsigned long long* ring_full;
+  uint32_t tmem;                // of this warp in the first slot
+  uint32_t a_full[A_SLOTS];     // the leading block's barriers
+  int g, r, lane;
+  int stage, slot;
+  uint32_t phase, slot_phase;
+};
+// The steps of an item.  NBITS = 0: rows of padding, zeros.  False when a wait ran out.
+template <int NBITS, bool SMALL, typename PRODUCE>
+__device__ __forceinline__ bool steps(Decoder& d, const Stream& s, int shift, const LaneRow& row, int count, const PRODUCE& produce) {
+  constexpr int PER_COPY = NBITS == 0 ? 1 : 8 / (NBITS == 0 ? 1 : NBITS);
+  int in_copy = 0;
+  for (int i = 0; i < count; ++i) {
+    const bool mine = i < s.chunks;  // the second half of an odd number of chunks lacks the last one
+    uint32_t w[32];
+    if (NBITS == 0 || !mine) {
+#pragma unroll
+      for (int q = 0; q < 32; ++q) w[q] = 0;
+    } else {
+      if (in_copy == 0 && !__all_sync(0xffffffffu, bar_wait(d.ring_full + d.stage, d.phase, &d.ctl->abort, d.status))) return false;
+      decode_row<NBITS == 0 ? 2 : NBITS, SMALL>(d.ring + d.stage * RING_BYTES + in_copy * s.slab, d.g, d.r, shift, row, w);
+      if (++in_copy == PER_COPY || i == s.chunks - 1) {
+        in_copy = 0;
+        __syncwarp();  // every lane has read the stage
+        if (d.lane == 0) produce();
+        __syncwarp();
+        if (++d.stage == RING_STAGES) d.stage = 0, d.phase ^= 1;
+      }
     }
+    if (!__all_sync(0xffffffffu, bar_wait(&d.ctl->a_empty[d.slot], d.slot_phase, &d.ctl->abort, d.status))) return false;
+    fence_after();
+    if (mine) tmem_store32(d.tmem + d.slot * SLOT_COLUMNS, w);
+    fence_before();
+    __syncwarp();
+    if (d.lane == 0) bar_arrive_cluster(d.a_full[d.slot]);
+    if (++d.slot == A_SLOTS) d.slot = 0, d.slot_phase ^= 1;
+  }
+  return true;
 }
 
 struct Shape {
@@ -153,11 +201,6 @@ __device__ __forceinline__ bool get_item(const Product& p, int64_t item, int row
   return true;
 }
 
-// One warp's packed data of one item.
-struct Stream {
-  const uint8_t* src;
-  int slab, per_copy, chunks, copies;
-};
 __device__ __forceinline__ GroupForm group_form(const Product& p, const Item& item, int quarter) {
   if (item.row_tile >= (int)(p.w.groups_per_expert / 4)) return GroupForm{0, 0};
   return load_group(p.w.groups, (int64_t)item.tile.expert * p.w.groups_per_expert + item.row_tile * 4 + quarter);
@@ -173,18 +216,20 @@ __device__ __forceinline__ Stream stream_of(const Product& p, GroupForm form, in
 
 // This lane's column of 16 activation rows of a finished tile; the residuals are read before the stores that they
 // could otherwise not pass.
-template <typename T>
+template <typename T, bool FULL>
 __device__ __forceinline__ void put_columns(const Epilogue& out, float (&v)[16], int count, int64_t row, uint32_t col, float bias) {
-  T* const to = static_cast<T*>(out.out) + row * out.ld_out + col;
+  T* to = static_cast<T*>(out.out) + row * out.ld_out + col;
   T res[16];
   if (out.residual != nullptr) {
-    const T* const from = static_cast<const T*>(out.residual) + row * out.ld_residual + col;
+    const T* from = static_cast<const T*>(out.residual) + row * out.ld_residual + col;
 #pragma unroll
-    for (int t = 0; t < 16; ++t)
-      if (t < count) res[t] = from[t * out.ld_residual];
+    for (int t = 0; t < 16; ++t, from += out.ld_residual)
+      if (FULL || t < count) res[t] = *from;
   }
+  if (out.bias != nullptr) {
 #pragma unroll
-  for (int t = 0; t < 16; ++t) v[t] += bias;
+    for (int t = 0; t < 16; ++t) v[t] += bias;
+  }
   switch (out.act) {  // (outside the loop: one activation's code at a time)
     case HI2_ACT_RELU:
 #pragma unroll
@@ -207,11 +252,16 @@ __device__ __forceinline__ void put_columns(const Epilogue& out, float (&v)[16],
   if (out.residual != nullptr) {
 #pragma unroll
     for (int t = 0; t < 16; ++t)
-      if (t < count) v[t] += to_float(res[t]);
+      if (FULL || t < count) v[t] += to_float(res[t]);
   }
 #pragma unroll
-  for (int t = 0; t < 16; ++t)
-    if (t < count) to[t * out.ld_out] = from_float<T>(v[t]);
+  for (int t = 0; t < 16; ++t, to += out.ld_out)
+    if (FULL || t < count) *to = from_float<T>(v[t]);
+}
+template <typename T>
+__device__ __forceinline__ void put_columns(const Epilogue& out, float (&v)[16], int count, int64_t row, uint32_t col, float bias) {
+  if (count == 16) put_columns<T, true>(out, v, count, row, col, bias);
+  else put_columns<T, false>(out, v, count, row, col, bias);
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -278,8 +328,8 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
     };
     if (lane == 0)
       for (int s = 0; s < RING_STAGES; ++s) produce();
-    int stage = 0, slot = 0;
-    uint32_t phase = 0, slot_phase = 1;
+    Decoder out{ctl, status, ring, ctl->ring_full[warp], a_tmem + half * A_COLUMNS + ((uint32_t)(quarter * 32) << 16),
+                {in_rank(s32(&ctl->a_full[0]), 0), in_rank(s32(&ctl->a_full[1]), 0)}, g, r, lane, 0, 0, 0, 1};
     for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
       const GroupForm form = group_form(p, item, quarter);
       const Stream s = stream_of(p, form, half, half0, chunks);
@@ -289,39 +339,16 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
         row.lo_min[0] = row.lo_min[1] = c.lo_min(), row.lo_scale[0] = row.lo_scale[1] = c.lo_scale();
         row.step_scale = __half2half2(__ushort_as_half((uint16_t)c.step_scale));
       }
-      int in_copy = 0;
-      for (int i = 0; i < half0; ++i) {
-        const bool mine = i < s.chunks;  // the second half of an odd number of chunks lacks the last one
-        uint32_t w[32];
-        if (mine && s.slab != 0) {
-          if (in_copy == 0) {
-            ok = __all_sync(0xffffffffu, bar_wait(&ctl->ring_full[warp][stage], phase, &ctl->abort, status));
-            if (!ok) break;
-          }
-          const uint8_t* slab = ring + stage * RING_BYTES + in_copy * s.slab;
-          if (form.width() == 1) decode_row<2>(slab, g, r, form.shift(), row, w);
-          else if (form.width() == 2) decode_row<4>(slab, g, r, form.shift(), row, w);
-          else decode_row<8>(slab, g, r, form.shift(), row, w);
-          if (++in_copy == s.per_copy || i == s.chunks - 1) {
-            in_copy = 0;
-            __syncwarp();  // every lane has read the stage
-            if (lane == 0) produce();
-            __syncwarp();
-            if (++stage == RING_STAGES) stage = 0, phase ^= 1;
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 32; ++q) w[q] = 0;
-        }
-        ok = __all_sync(0xffffffffu, bar_wait(&ctl->a_empty[slot], slot_phase, &ctl->abort, status));
-        if (!ok) break;
-        fence_after();
-        if (mine) tmem_store32(a_tmem + slot * SLOT_COLUMNS + half * A_COLUMNS + ((uint32_t)(quarter * 32) << 16), w);
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive_cluster(in_rank(s32(&ctl->a_full[slot]), 0));
-        if (++slot == A_SLOTS) slot = 0, slot_phase ^= 1;
-      }
+      const auto run = [&](auto nbits, auto small) {
+        return steps<decltype(nbits)::value, decltype(small)::value>(out, s, form.shift(), row, half0, produce);
+      };
+      typedef std::integral_constant<int, 2> Int2;
+      typedef std::integral_constant<int, 4> Int4;
+      typedef std::integral_constant<int, 8> Int8;
+      if (form.width() == 1) ok = form.small_steps() ? run(Int2(), std::true_type()) : run(Int2(), std::false_type());
+      else if (form.width() == 2) ok = form.small_steps() ? run(Int4(), std::true_type()) : run(Int4(), std::false_type());
+      else if (form.width() == 3) ok = form.small_steps() ? run(Int8(), std::true_type()) : run(Int8(), std::false_type());
+      else ok = run(std::integral_constant<int, 0>(), std::true_type());
     }
   } else if (warp == X_WARP) {
     // ------------------------------------------------------------ activations
@@ -392,7 +419,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
   } else if (warp >= FIRST_EPILOGUE) {
     // ------------------------------------------------------------ epilogue
     // a warp may only touch the 32 tensor-memory lanes of its index modulo 4
-    const int quarter = warp & 3, second = (warp - FIRST_EPILOGUE) >> 2;
+    const int quarter = warp & 3;
     int buf = 0;
     uint32_t phase = 0;
     for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
@@ -405,7 +432,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
       if (!ok) break;
       fence_after();
       const uint32_t taddr = tmem + buf * MAX_WIDTH + ((uint32_t)(quarter * 32) << 16);
-      for (int t0 = 16 * second; t0 < tokens; t0 += 32) {
+      for (int t0 = 0; t0 < tokens; t0 += 16) {
         const int count = min(16, tokens - t0);
         const int64_t first = item.tile.begin + t0;
         float scale = 0.0f;  // lane t: of activation row t0 + t

@@ -122,7 +122,12 @@ def _lay_out_on(f: dict, experts: int, rows: int, k: int, stacked: bool, dev: to
     lead = src[:, ::_GROUP_ROWS].reshape(-1)                    # a group's first row is never padding, unless all are
     at = lead.clamp_min(0)
     live = lead >= 0
-    form = torch.where(live, width[at] | shift[at] << 2, torch.zeros_like(lead))
+    # groups whose largest step, times the power of two that its codes are read with, is still an fp16 number
+    limit = torch.where(nbits == 8, 65504.0 / 2**22, 65504.0 / 2**20)
+    step = 255 * consts[:, 2].float()
+    small = ((step >= 0) & (step <= limit))[src.clamp_min(0)] | (src < 0)
+    small = small.view(-1, _GROUP_ROWS).all(1).long()
+    form = torch.where(live, width[at] | shift[at] << 2 | small << 4, torch.zeros_like(lead))
     units = torch.where(live, (16 << width[at]) + (16 >> shift[at]), torch.zeros_like(lead))  # of 16 bytes, per chunk
     base = (units * (k // CHUNK)).cumsum(0)
     total_units = int(base[-1].item())
