@@ -248,13 +248,13 @@ struct Carver {
 };
 
 // Which kernel takes a product.
-inline bool few(const hi2_stored_weight& w, int64_t tokens) { return tokens <= 32; }
+inline bool few(int64_t tokens) { return tokens <= FEW_WIDTH; }
 inline int64_t rows_per_expert(int64_t experts, int64_t pairs) {  // with half as many again as on average
   const int64_t busy = ceil_div(3 * pairs, 2 * experts);
   return busy < pairs ? busy : pairs;
 }
-inline bool few_experts(int64_t experts, int64_t pairs) { return rows_per_expert(experts, pairs) <= 32; }
-inline bool apart(int64_t pairs) { return pairs <= 16; }  // every pair a tile of its own
+inline bool few_experts(int64_t experts, int64_t pairs) { return rows_per_expert(experts, pairs) <= FEW_WIDTH; }
+inline bool apart(int64_t pairs) { return pairs <= FEW_WIDTH; }  // every pair a tile of its own
 
 inline int parts_of(int dtype) { return dtype == HI2_BF16 ? 1 : 2; }
 inline int64_t size_of(int dtype) { return dtype == HI2_F32 ? 4 : 2; }
@@ -263,13 +263,21 @@ inline int kind_of(int dtype) { return dtype == HI2_BF16 ? FROM_BF16 : dtype == 
 
 struct LinearSpace {
   __half* xs = nullptr;
-  float* scale = nullptr;
+  float *scale = nullptr, *partial = nullptr;
+  int width = FEW_WIDTH;
+  int64_t max_tiles;
   size_t bytes;
   LinearSpace(void* ws, const hi2_stored_weight& w, int dtype, int64_t tokens) {
     Carver c{static_cast<uint8_t*>(ws)};
-    if (!few(w, tokens)) {
+    if (!few(tokens)) {
       xs = c.take<__half>((size_t)tokens * w.k * parts_of(dtype));
       scale = c.take<float>(tokens);
+      width = wide_width(tokens);
+    }
+    max_tiles = ceil_div(tokens, (int64_t)width);
+    if (!few(tokens)) {
+      const int splits = wide_splits(w, Tiles{}, max_tiles);
+      if (splits > 1) partial = c.take<float>((size_t)splits * tokens * w.rows_per_expert);
     }
     bytes = c.used;
   }
@@ -348,11 +356,10 @@ extern "C" int hi2_stored_linear(const hi2_stored_weight* w, const void* x, int 
   if (space.bytes > 0 && (workspace == nullptr || workspace_bytes < space.bytes || !aligned16(workspace)))
     return fail(HI2_ERR_WORKSPACE, "stored_linear: workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool small = few(*w, tokens);
-  const int width = small ? few_width(tokens) : wide_width(tokens);
+  const bool small = few(tokens);
   const Product p{*w, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), 1},
-                  Tiles{nullptr, nullptr, nullptr, nullptr, tokens, 1, width}, ceil_div(tokens, (int64_t)width), parts_of(dtype),
-                  Epilogue{nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}, space.xs, space.scale};
+                  Tiles{nullptr, nullptr, nullptr, nullptr, tokens, 1, space.width}, space.max_tiles, parts_of(dtype),
+                  Epilogue{nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}, space.xs, space.scale, space.partial};
   if (small) return product_few(p, s, "stored_linear");
   const int rc = prepare(p, nullptr, s);
   return rc != HI2_OK ? rc : product_wide(p, s, "stored_linear");
@@ -389,7 +396,7 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   int rc;
   if (!apart(pairs)) {
     const int64_t busy = rows_per_expert(experts, pairs);
-    tiles = Tiles{index, space.pair_of, space.tile_count, space.tiles, pairs, experts, small ? few_width(busy) : wide_width(busy)};
+    tiles = Tiles{index, space.pair_of, space.tile_count, space.tiles, pairs, experts, small ? FEW_WIDTH : wide_width(busy)};
     max_tiles = pairs / tiles.width + experts + 1;
     const size_t smem = (size_t)SORT_WARPS * experts * sizeof(int32_t);
     if (smem > 48 * 1024 &&
@@ -400,9 +407,9 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
     if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
   }
   const Product up{*gate_up, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), top_k}, tiles, max_tiles, parts,
-                   Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, space.xs, space.scale};
+                   Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, space.xs, space.scale, nullptr};
   const Product dn{*down, Source{space.z, 2 * inner, FROM_GATED, act, true, top_k}, tiles, max_tiles, parts,
-                   Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, space.xs, space.scale};
+                   Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, space.xs, space.scale, nullptr};
   for (const Product* p : {&up, &dn}) {
     if (small) {
       rc = product_few(*p, s, "stored_experts");

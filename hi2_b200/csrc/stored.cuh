@@ -320,16 +320,19 @@ struct Product {
   int64_t max_tiles;
   int parts;               // fp16 parts of an activation: 2 where the second holds what the first one's rounding lost
   Epilogue out;
-  // wide products only: the prepared activations fp16 [parts, rows, k], and the powers of two they were divided by
+  // wide products only: the prepared activations fp16 [parts, rows, k], the powers of two they were divided by, and the
+  // sums of the slices fp32 [wide_splits, rows, rows of the tensor] where there are several
   __half* xs;
   float* row_scale;
+  float* partial;
 };
 
-// Products with up to 32 activation rows per tile, which prepare their activations themselves.
-int few_width(int64_t rows);
+// Products with up to 8 activation rows per tile, which prepare their activations themselves.
+constexpr int FEW_WIDTH = 8;
 int product_few(const Product& p, cudaStream_t stream, const char* what);
 // Wide tiles, from prepared activations.
 int wide_width(int64_t rows);
+int wide_splits(const hi2_stored_weight& w, const Tiles& tiles, int64_t max_tiles);
 int product_wide(const Product& p, cudaStream_t stream, const char* what);
 
 }  // namespace stored

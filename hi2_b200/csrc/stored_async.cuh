@@ -21,7 +21,7 @@ __device__ __forceinline__ void bar_arrive(unsigned long long* b) {
 __device__ __forceinline__ bool bar_try(unsigned long long* b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.b32 %0, 1, 0, p;\n\t}"
       : "=r"(ok) : "r"(s32(b)), "r"(parity) : "memory");
   return ok != 0;

@@ -1,4 +1,4 @@
-// The product of packed rows with up to 32 activation rows: decode steps and small batches, where the packed
+// The product of packed rows with up to 8 activation rows: decode steps and small batches, where the packed
 // bytes are what has to be moved.
 //
 // A block takes 128 sorted rows and a slice of the columns; the slices of a row tile are a cluster and join
@@ -30,20 +30,19 @@ constexpr int X_PITCH = BLOCK_COLUMNS + 8;         // halves; the extra 16 bytes
 constexpr int SUM_PITCH = TILE_ROWS + 4;
 constexpr int MAX_SPLIT = 8;
 
-template <int NT>
 struct Shared {
   union {
     uint8_t ring[WARPS][RING_STAGES][RING_BYTES];
-    float sums[2][8 * NT][SUM_PITCH];  // of the two halves, once the rings are done with
+    float sums[2][FEW_WIDTH][SUM_PITCH];  // of the two halves, once the rings are done with
   };
-  float scale[2][2][8 * NT];         // of the block being multiplied and of the one before; of each half
+  float scale[2][2][FEW_WIDTH];         // of the block being multiplied and of the one before; of each half
   uint32_t out_row[TILE_ROWS];
   unsigned long long full[WARPS][RING_STAGES];
   volatile uint32_t abort;
 };
-template <int NT, int PARTS>
+template <int PARTS>
 constexpr size_t smem_bytes() {
-  return sizeof(Shared<NT>) + (size_t)PARTS * 8 * NT * X_PITCH * sizeof(__half) + 16;
+  return sizeof(Shared) + (size_t)PARTS * FEW_WIDTH * X_PITCH * sizeof(__half) + 16;
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -86,9 +85,9 @@ struct Ring {
 };
 
 // `count` chunks against the activations at x.  False when a wait ran out.
-template <int NT, int PARTS, int NBITS, bool SMALL, typename REFILL>
+template <int PARTS, int NBITS, bool SMALL, typename REFILL>
 __device__ __forceinline__ bool multiply(Ring& ring, const __half* x, int count, int first_word, int pair_unit, const LaneRows& rows,
-                                         float (&acc)[2][NT][4], volatile uint32_t* abort, int32_t* status, const REFILL& refill) {
+                                         float (&acc)[2][4], volatile uint32_t* abort, int32_t* status, const REFILL& refill) {
   constexpr int PER_COPY = 8 / NBITS;
   while (count > 0) {
     if (!__all_sync(0xffffffffu, bar_wait(ring.full + ring.stage, ring.phase, abort, status))) return false;
@@ -99,18 +98,16 @@ __device__ __forceinline__ bool multiply(Ring& ring, const __half* x, int count,
       uint32_t w[4][8];
       decode_rows<NBITS, SMALL>(slab, first_word, pair_unit, rows, w);
 #pragma unroll
-      for (int part = 0; part < PARTS; ++part)
+      for (int part = 0; part < PARTS; ++part) {
+        const __half* from = x + part * FEW_WIDTH * X_PITCH;
+        const uint4 x0 = *reinterpret_cast<const uint4*>(from), x1 = *reinterpret_cast<const uint4*>(from + 8);
+        const uint32_t k[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-        for (int q = 0; q < NT; ++q) {
-          const __half* from = x + (part * 8 * NT + q * 8) * X_PITCH;
-          const uint4 x0 = *reinterpret_cast<const uint4*>(from), x1 = *reinterpret_cast<const uint4*>(from + 8);
-          const uint32_t k[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            mma(acc[0][q], w[0][2 * s], w[1][2 * s], w[0][2 * s + 1], w[1][2 * s + 1], k[2 * s], k[2 * s + 1]);
-            mma(acc[1][q], w[2][2 * s], w[3][2 * s], w[2][2 * s + 1], w[3][2 * s + 1], k[2 * s], k[2 * s + 1]);
-          }
+        for (int s = 0; s < 4; ++s) {
+          mma(acc[0], w[0][2 * s], w[1][2 * s], w[0][2 * s + 1], w[1][2 * s + 1], k[2 * s], k[2 * s + 1]);
+          mma(acc[1], w[2][2 * s], w[3][2 * s], w[2][2 * s + 1], w[3][2 * s + 1], k[2 * s], k[2 * s + 1]);
         }
+      }
     }
     count -= here;
     __syncwarp();  // every lane has read the stage
@@ -120,12 +117,12 @@ __device__ __forceinline__ bool multiply(Ring& ring, const __half* x, int count,
   return true;
 }
 
-template <int NT, int PARTS>
-__global__ void __launch_bounds__(THREADS, NT < 4 ? 2 : 1)
+template <int PARTS>
+__global__ void __launch_bounds__(THREADS, 2)
 few_kernel(const Product p, const int split) {
   extern __shared__ __align__(16) uint8_t raw[];
-  Shared<NT>& sm = *reinterpret_cast<Shared<NT>*>(raw);
-  __half* const xs = reinterpret_cast<__half*>((reinterpret_cast<uintptr_t>(raw) + sizeof(Shared<NT>) + 15) & ~(uintptr_t)15);
+  Shared& sm = *reinterpret_cast<Shared*>(raw);
+  __half* const xs = reinterpret_cast<__half*>((reinterpret_cast<uintptr_t>(raw) + sizeof(Shared) + 15) & ~(uintptr_t)15);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = (int)(blockIdx.x % split);
   const int row_tiles = (int)(p.w.groups_per_expert / 4);
@@ -178,13 +175,11 @@ few_kernel(const Product p, const int split) {
   }
   const int pair_unit = (4 >> form.shift()) * g + (t >> form.shift()), first_word = code_word(g, t);
 
-  float total[2][NT][4];
+  float total[2][4];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int q = 0; q < NT; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) total[m][q][i] = 0.0f;
+    for (int i = 0; i < 4; ++i) total[m][i] = 0.0f;
 
   chain_wait();  // the activations
   bool ok = true;
@@ -222,25 +217,23 @@ few_kernel(const Product p, const int split) {
         uint4* dst = reinterpret_cast<uint4*>(xs + r * X_PITCH + piece * 16);
         dst[0] = hi[0], dst[1] = hi[1];
         if (PARTS == 2) {
-          dst = reinterpret_cast<uint4*>(xs + (8 * NT + r) * X_PITCH + piece * 16);
+          dst = reinterpret_cast<uint4*>(xs + (FEW_WIDTH + r) * X_PITCH + piece * 16);
           dst[0] = lo[0], dst[1] = lo[1];
         }
       }
     }
     __syncthreads();
     // ---- this warp's chunks of the block
-    float acc[2][NT][4];
+    float acc[2][4];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int q = 0; q < NT; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][q][i] = 0.0f;
+      for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
     const int first = half == 0 ? 0 : half0, count = half == 0 ? half0 : chunks - half0;
     if (ok) {  // one loop per code width
       const __half* x = xs + g * X_PITCH + first * CHUNK + 16 * t;
       const auto run = [&](auto nbits, auto small) {
-        return multiply<NT, PARTS, decltype(nbits)::value, decltype(small)::value>(ring, x, count, first_word, pair_unit, rows, acc, &sm.abort,
+        return multiply<PARTS, decltype(nbits)::value, decltype(small)::value>(ring, x, count, first_word, pair_unit, rows, acc, &sm.abort,
                                                                                    status, refill);
       };
       typedef std::integral_constant<int, 2> Int2;
@@ -250,30 +243,24 @@ few_kernel(const Product p, const int split) {
       else if (form.width() == 2) ok = form.small_steps() ? run(Int4(), std::true_type()) : run(Int4(), std::false_type());
       else if (form.width() == 3) ok = form.small_steps() ? run(Int8(), std::true_type()) : run(Int8(), std::false_type());
     }
+    const float s0 = sm.scale[b & 1][half][2 * t], s1 = sm.scale[b & 1][half][2 * t + 1];
 #pragma unroll
-    for (int q = 0; q < NT; ++q) {
-      const float s0 = sm.scale[b & 1][half][8 * q + 2 * t], s1 = sm.scale[b & 1][half][8 * q + 2 * t + 1];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        total[m][q][0] += acc[m][q][0] * s0, total[m][q][1] += acc[m][q][1] * s1;
-        total[m][q][2] += acc[m][q][2] * s0, total[m][q][3] += acc[m][q][3] * s1;
-      }
+    for (int m = 0; m < 2; ++m) {
+      total[m][0] += acc[m][0] * s0, total[m][1] += acc[m][1] * s1;
+      total[m][2] += acc[m][2] * s0, total[m][3] += acc[m][3] * s1;
     }
   }
   if (__syncthreads_or(!ok)) let_copies_land();
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int q = 0; q < NT; ++q)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sm.sums[half][8 * q + 2 * t + (i & 1)][quarter * 32 + 16 * m + 8 * (i >> 1) + g] = total[m][q][i];
+    for (int i = 0; i < 4; ++i) sm.sums[half][2 * t + (i & 1)][quarter * 32 + 16 * m + 8 * (i >> 1) + g] = total[m][i];
   __syncthreads();
   if (split > 1) cluster_sync();
   const uint32_t here = s32(&sm.sums[0][0][0]);
   for (int i = rank * THREADS + threadIdx.x; i < tokens * TILE_ROWS; i += split * THREADS) {
     const int token = i / TILE_ROWS, row = i % TILE_ROWS;
-    const uint32_t off = (uint32_t)(token * SUM_PITCH + row) * 4, other = 8 * NT * SUM_PITCH * 4;
+    const uint32_t off = (uint32_t)(token * SUM_PITCH + row) * 4, other = FEW_WIDTH * SUM_PITCH * 4;
     float v[2 * MAX_SPLIT];
     if (split > 1) {
 #pragma unroll
@@ -297,10 +284,10 @@ few_kernel(const Product p, const int split) {
   if (split > 1) cluster_sync();  // nobody reads this block's sums any more
 }
 
-template <int NT, int PARTS>
+template <int PARTS>
 int launch(const Product& p, int split, cudaStream_t stream, const char* what) {
-  const size_t smem = smem_bytes<NT, PARTS>();
-  if (cudaFuncSetAttribute(few_kernel<NT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  const size_t smem = smem_bytes<PARTS>();
+  if (cudaFuncSetAttribute(few_kernel<PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return fail(HI2_ERR_LAUNCH, "stored product: cannot reserve shared memory");
   const int64_t blocks = p.w.groups_per_expert / 4 * p.max_tiles * split;
   if (blocks >= (int64_t)1 << 31) return fail(HI2_ERR_ARG, "stored product: too many tiles");
@@ -312,29 +299,24 @@ int launch(const Product& p, int split, cudaStream_t stream, const char* what) {
   attribute[1].id = cudaLaunchAttributeClusterDimension;
   attribute[1].val.clusterDim.x = split, attribute[1].val.clusterDim.y = 1, attribute[1].val.clusterDim.z = 1;
   config.attrs = attribute, config.numAttrs = 2;
-  cudaLaunchKernelEx(&config, few_kernel<NT, PARTS>, p, split);
+  cudaLaunchKernelEx(&config, few_kernel<PARTS>, p, split);
   return check_launch(what);
 }
 
 }  // namespace
 
-int few_width(int64_t rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
-
 int product_few(const Product& p, cudaStream_t stream, const char* what) {
   // Slices of the columns: the number that leaves the fullest SM the least work, with what a block costs
   // besides its chunks (start, activations, the join) counted as twelve of them; each at least four chunks.
   const int64_t tiles = p.w.groups_per_expert / 4 * p.max_tiles, chunks = p.w.k / CHUNK;
-  const int64_t room = 148 * (p.tiles.width <= 16 ? 2 : 1);
+  const int64_t room = 148 * 2;
   int split = 1;
   int64_t least = INT64_MAX;
   for (int s = 1; s <= MAX_SPLIT && (s == 1 || chunks >= 4 * s); ++s) {
     const int64_t cost = ceil_div(tiles * s, room) * (ceil_div(chunks, (int64_t)s) + 12);
     if (cost < least) least = cost, split = s;
   }
-  const bool one = p.parts == 1;
-  if (p.tiles.width <= 8) return one ? launch<1, 1>(p, split, stream, what) : launch<1, 2>(p, split, stream, what);
-  if (p.tiles.width <= 16) return one ? launch<2, 1>(p, split, stream, what) : launch<2, 2>(p, split, stream, what);
-  return one ? launch<4, 1>(p, split, stream, what) : launch<4, 2>(p, split, stream, what);
+  return p.parts == 1 ? launch<1>(p, split, stream, what) : launch<2>(p, split, stream, what);
 }
 
 }  // namespace stored

@@ -13,8 +13,8 @@
 //
 // Blocks stay for many tiles.  Warps 0..7 decode (warp w: rows 32 (w mod 4) .. of the block's tile, one half of the
 // columns), every warp with its own ring of bulk copies that runs on into the next tile; warp 8 loads activations, warp 9
-// issues; warps 10..13 take finished tiles out of one of two accumulators (2 x 192 columns, beside two slots of 2 x 32
-// columns for decoded chunks) while the next tile is computed in the other.  A step is one chunk of each
+// issues; warps 10..13 take finished tiles out of one of two accumulators (of the tile's width, up to 192 columns) while the
+// next tile is computed in the other; behind them are two to four slots of 2 x 32 columns for decoded chunks.  A step is one chunk of each
 // half of the columns, in a fixed order: equal inputs give equal bits.
 //
 // Every mbarrier wait is bounded by a clock limit and raises *status.
@@ -31,17 +31,16 @@ namespace {
 constexpr int DECODE_WARPS = 8, X_WARP = 8, MMA_WARP = 9, FIRST_EPILOGUE = 10, EPILOGUE_WARPS = 4;
 constexpr int THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE_WARPS);
 constexpr int MAX_WIDTH = 192;
-constexpr int A_SLOTS = 2, A_COLUMNS = CHUNK / 2, SLOT_COLUMNS = 2 * A_COLUMNS;
-constexpr int FIRST_A_COLUMN = 2 * MAX_WIDTH;   // behind the two accumulators
+constexpr int MAX_SLOTS = 4, A_COLUMNS = CHUNK / 2, SLOT_COLUMNS = 2 * A_COLUMNS;
 constexpr int RING_STAGES = 2, RING_BYTES = 3072;  // a stage: four chunks of INT2, two of INT4, one of INT8
 constexpr int MAX_X_STAGES = 6;
-static_assert(FIRST_A_COLUMN + A_SLOTS * SLOT_COLUMNS == 512, "tensor memory");
 
 struct Control {
   unsigned long long x_full[MAX_X_STAGES], x_empty[MAX_X_STAGES];
-  unsigned long long a_full[A_SLOTS], a_empty[A_SLOTS];
+  unsigned long long a_full[MAX_SLOTS], a_empty[MAX_SLOTS];
   unsigned long long d_full[2], d_empty[2];
   unsigned long long ring_full[DECODE_WARPS][RING_STAGES];
+  alignas(16) float scale[EPILOGUE_WARPS][MAX_WIDTH];
   uint32_t tmem_base;
   volatile uint32_t abort;
 };
@@ -51,8 +50,10 @@ __device__ __forceinline__ uint32_t cta_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
+// What these arrivals order is tensor memory, which the fences before and after them do.  A release at cluster
+// scope would wait for everything else the thread has in flight: 1200 clocks where this takes 250.
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // One box into this block's shared memory; the bytes are counted by the leader's barrier.
 __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int x, int y) {
@@ -77,6 +78,13 @@ __device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint32_t a_tmem, uint6
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(d_tmem), "r"(a_tmem), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
+}
+// One lane of a converged warp.  (The compiler keeps a branch on this uniform, with descriptors in uniform registers;
+// behind `lane == 0` every operand of every product is moved there first.)
+__device__ __forceinline__ bool elected() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
 }
 // Arrives on the barrier at this offset in BOTH blocks once the products issued so far have finished.
 __device__ __forceinline__ void commit_both(unsigned long long* b) {
@@ -114,25 +122,39 @@ __device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// The lane's row (8 r + g of its group) in the chunk at `slab`: 64 weights as 32 pairs of neighbouring columns.
+// The lane's row (8 r + g of its group) in a chunk: what it reads, and its 64 weights as 32 pairs of neighbouring
+// columns.  The next chunk's words are asked for before the present one's weights are handed on.
 struct LaneRow {
   float lo_min[2], lo_scale[2];  // twice the same: two pieces are decoded together
   __half2 step_scale;
 };
-template <int NBITS, bool SMALL>
-__device__ __forceinline__ void decode_row(const uint8_t* slab, int g, int r, int shift, const LaneRow& row, uint32_t (&w)[32]) {
-  const uint16_t* pairs = reinterpret_cast<const uint16_t*>(slab + 256 * NBITS) + 4 * ((4 >> shift) * g) + r;
-  Ladder l[4];
+template <int NBITS>
+struct RawRow {
+  uint32_t words[2 * NBITS], pairs[2];
+  __device__ __forceinline__ void load(const uint8_t* slab, int g, int r, int shift) {
+    const uint16_t* from = reinterpret_cast<const uint16_t*>(slab + 256 * NBITS) + 4 * ((4 >> shift) * g) + r;
 #pragma unroll
-  for (int t = 0; t < 4; t += 2)
-    ladders<NBITS, SMALL>((uint32_t)pairs[4 * (t >> shift)] | (uint32_t)pairs[4 * ((t + 1) >> shift)] << 16, row.lo_min, row.lo_scale, row.step_scale,
-            l[t], l[t + 1]);
-  const uint32_t* words = reinterpret_cast<const uint32_t*>(slab) + r;
+    for (int t = 0; t < 4; t += 2)
+      pairs[t / 2] = (uint32_t)from[4 * (t >> shift)] | (uint32_t)from[4 * ((t + 1) >> shift)] << 16;
+    const uint32_t* at = reinterpret_cast<const uint32_t*>(slab) + r;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int h = 0; h < NBITS / 2; ++h) decode_word<NBITS, SMALL>(words[128 * h + code_word(g, t)], l[t], w + 8 * t + 16 / NBITS * h);
-}
+      for (int h = 0; h < NBITS / 2; ++h) words[NBITS / 2 * t + h] = at[128 * h + code_word(g, t)];
+  }
+  template <bool SMALL>
+  __device__ __forceinline__ void expand(const LaneRow& row, uint32_t (&w)[32]) const {
+#pragma unroll
+    for (int t = 0; t < 4; t += 2) {
+      Ladder l[2];
+      ladders<NBITS, SMALL>(pairs[t / 2], row.lo_min, row.lo_scale, row.step_scale, l[0], l[1]);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int h = 0; h < NBITS / 2; ++h) decode_word<NBITS, SMALL>(words[NBITS / 2 * (t + u) + h], l[u], w + 8 * (t + u) + 16 / NBITS * h);
+    }
+  }
+};
 
 // One warp's packed data of one item.
 struct Stream {
@@ -147,90 +169,142 @@ struct Decoder {
   const uint8_t* ring;
   unsigned long long* ring_full;
   uint32_t tmem;                // of this warp in the first slot
-  uint32_t a_full[A_SLOTS];     // the leading block's barriers
-  int g, r, lane;
+  uint32_t a_full;              // the leading block's first barrier
+  int g, r, lane, slots;
   int stage, slot;
   uint32_t phase, slot_phase;
-};
-// The steps of an item.  NBITS = 0: rows of padding, zeros.  False when a wait ran out.
-template <int NBITS, bool SMALL, typename PRODUCE>
-__device__ __forceinline__ bool steps(Decoder& d, const Stream& s, int shift, const LaneRow& row, int count, const PRODUCE& produce) {
-  constexpr int PER_COPY = NBITS == 0 ? 1 : 8 / (NBITS == 0 ? 1 : NBITS);
-  int in_copy = 0;
-  for (int i = 0; i < count; ++i) {
-    const bool mine = i < s.chunks;  // the second half of an odd number of chunks lacks the last one
-    uint32_t w[32];
-    if (NBITS == 0 || !mine) {
-#pragma unroll
-      for (int q = 0; q < 32; ++q) w[q] = 0;
-    } else {
-      if (in_copy == 0 && !__all_sync(0xffffffffu, bar_wait(d.ring_full + d.stage, d.phase, &d.ctl->abort, d.status))) return false;
-      decode_row<NBITS == 0 ? 2 : NBITS, SMALL>(d.ring + d.stage * RING_BYTES + in_copy * s.slab, d.g, d.r, shift, row, w);
-      if (++in_copy == PER_COPY || i == s.chunks - 1) {
-        in_copy = 0;
-        __syncwarp();  // every lane has read the stage
-        if (d.lane == 0) produce();
-        __syncwarp();
-        if (++d.stage == RING_STAGES) d.stage = 0, d.phase ^= 1;
-      }
-    }
-    if (!__all_sync(0xffffffffu, bar_wait(&d.ctl->a_empty[d.slot], d.slot_phase, &d.ctl->abort, d.status))) return false;
+  __device__ __forceinline__ bool wait_ring() { return __all_sync(0xffffffffu, bar_wait(ring_full + stage, phase, &ctl->abort, status)); }
+  // The weights (STORE: there are some) into the next slot, and word of it to the leading block.
+  __device__ __forceinline__ bool hand_on(const uint32_t (&w)[32], bool store) {
+    if (!__all_sync(0xffffffffu, bar_wait(&ctl->a_empty[slot], slot_phase, &ctl->abort, status))) return false;
     fence_after();
-    if (mine) tmem_store32(d.tmem + d.slot * SLOT_COLUMNS, w);
+    if (store) tmem_store32(tmem + slot * SLOT_COLUMNS, w);
     fence_before();
     __syncwarp();
-    if (d.lane == 0) bar_arrive_cluster(d.a_full[d.slot]);
-    if (++d.slot == A_SLOTS) d.slot = 0, d.slot_phase ^= 1;
+    if (lane == 0) bar_arrive_cluster(a_full + 8 * slot);
+    if (++slot == slots) slot = 0, slot_phase ^= 1;
+    return true;
   }
+};
+// The `count` steps of an item; the last of them lacks this warp's chunk where s.chunks is smaller.  False when a wait ran out.
+template <int NBITS, bool SMALL, typename PRODUCE>
+__device__ __forceinline__ bool steps(Decoder& d, const Stream& s, int shift, const LaneRow& row, int count, const PRODUCE& produce) {
+  constexpr int PER_COPY = 8 / NBITS;
+  uint32_t w[32];
+  RawRow<NBITS> raw;
+  int in_copy = 0;
+  if (s.chunks > 0) {
+    if (!d.wait_ring()) return false;
+    raw.load(d.ring + d.stage * RING_BYTES, d.g, d.r, shift);
+  }
+  for (int i = 0; i < s.chunks; ++i) {
+    raw.template expand<SMALL>(row, w);
+    if (++in_copy == PER_COPY || i == s.chunks - 1) {
+      in_copy = 0;
+      __syncwarp();  // every lane has read the stage
+      if (d.lane == 0) produce();
+      __syncwarp();
+      if (++d.stage == RING_STAGES) d.stage = 0, d.phase ^= 1;
+      if (i < s.chunks - 1 && !d.wait_ring()) return false;
+    }
+    if (i < s.chunks - 1) raw.load(d.ring + d.stage * RING_BYTES + in_copy * s.slab, d.g, d.r, shift);
+    if (!d.hand_on(w, true)) return false;
+  }
+  for (int i = s.chunks; i < count; ++i)
+    if (!d.hand_on(w, false)) return false;
+  return true;
+}
+// Rows of padding only: zeros.
+__device__ __forceinline__ bool empty_steps(Decoder& d, int chunks, int count) {
+  uint32_t w[32];
+#pragma unroll
+  for (int q = 0; q < 32; ++q) w[q] = 0;
+  for (int i = 0; i < count; ++i)
+    if (!d.hand_on(w, i < chunks)) return false;
   return true;
 }
 
 struct Shape {
   int width;       // activation rows of a tile, a multiple of 16
   int x_stages;
+  int slots;       // of decoded chunks
+  int splits;      // slices of the columns
+  int row_pairs;   // pairs of tiles of packed rows
+  int chunks, half0;  // of the columns; of their first half (a step takes a chunk of each)
 };
 
-// What one item of work is: a tile of activation rows and two tiles of packed rows.
+// What one item of work is: a tile of activation rows, two tiles of packed rows, a slice of the columns.
 struct Item {
   TokenTile tile;
   int row_tile;    // of this block; may lie behind the last one
+  int slice, first, count;  // its first step, and its steps
 };
-__device__ __forceinline__ bool get_item(const Product& p, int64_t item, int row_pairs, uint32_t rank, Item& out) {
-  if (!p.tiles.get(item / row_pairs, out.tile)) return false;
-  out.row_tile = (int)(item % row_pairs) * 2 + (int)rank;
+__device__ __forceinline__ bool get_item(const Product& p, const Shape& shape, int64_t item, uint32_t rank, Item& out) {
+  const int64_t rest = item / shape.row_pairs;
+  out.slice = (int)(rest % shape.splits);
+  if (!p.tiles.get(rest / shape.splits, out.tile)) return false;
+  out.row_tile = (int)(item % shape.row_pairs) * 2 + (int)rank;
+  out.first = shape.half0 * out.slice / shape.splits;
+  out.count = shape.half0 * (out.slice + 1) / shape.splits - out.first;
   return true;
+}
+// Chunks of the second half in an item: the last step of an odd number of chunks lacks one.
+__device__ __forceinline__ int second_chunks(const Shape& shape, const Item& item) {
+  return min(item.count, shape.chunks - shape.half0 - item.first);
 }
 
 __device__ __forceinline__ GroupForm group_form(const Product& p, const Item& item, int quarter) {
   if (item.row_tile >= (int)(p.w.groups_per_expert / 4)) return GroupForm{0, 0};
   return load_group(p.w.groups, (int64_t)item.tile.expert * p.w.groups_per_expert + item.row_tile * 4 + quarter);
 }
-__device__ __forceinline__ Stream stream_of(const Product& p, GroupForm form, int half, int half0, int chunks) {
+__device__ __forceinline__ Stream stream_of(const Product& p, const Shape& shape, const Item& item, GroupForm form, int half) {
   Stream s;
   s.slab = form.slab_bytes(), s.per_copy = 8 >> form.width();
-  s.chunks = half == 0 ? half0 : chunks - half0;
+  s.chunks = half == 0 ? item.count : second_chunks(shape, item);
   s.copies = s.slab == 0 ? 0 : (s.chunks + s.per_copy - 1) / s.per_copy;
-  s.src = static_cast<const uint8_t*>(p.w.data) + (int64_t)form.base * 16 + (int64_t)(half == 0 ? 0 : half0) * s.slab;
+  s.src = static_cast<const uint8_t*>(p.w.data) + (int64_t)form.base * 16 + (int64_t)(item.first + (half == 0 ? 0 : shape.half0)) * s.slab;
   return s;
 }
 
-// This lane's column of 16 activation rows of a finished tile; the residuals are read before the stores that they
-// could otherwise not pass.
-template <typename T, bool FULL>
-__device__ __forceinline__ void put_columns(const Epilogue& out, float (&v)[16], int count, int64_t row, uint32_t col, float bias) {
-  T* to = static_cast<T*>(out.out) + row * out.ld_out + col;
-  T res[16];
-  if (out.residual != nullptr) {
-    const T* from = static_cast<const T*>(out.residual) + row * out.ld_residual + col;
+// f of 16 values, its code four times over instead of sixteen.
+template <typename F>
+__device__ __forceinline__ void each(float (&v)[16], const F& f) {
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    float a = f(v[0]), b = f(v[1]), c = f(v[2]), d = f(v[3]);
 #pragma unroll
-    for (int t = 0; t < 16; ++t, from += out.ld_residual)
-      if (FULL || t < count) res[t] = *from;
+    for (int t = 0; t < 12; ++t) v[t] = v[t + 4];  // registers move, no index varies
+    v[12] = a, v[13] = b, v[14] = c, v[15] = d;
+  }
+}
+// Column `col` of 16 activation rows from `row` on, of which `count` exist.
+template <typename T>
+__device__ __forceinline__ void read_rows(const void* p, int64_t ld, int64_t row, uint32_t col, int count, float (&v)[16]) {
+  const T* from = static_cast<const T*>(p) + row * ld + col;
+#pragma unroll
+  for (int t = 0; t < 16; ++t, from += ld) v[t] = t < count ? to_float(*from) : 0.0f;
+}
+template <typename T>
+__device__ __forceinline__ void write_rows(void* p, int64_t ld, int64_t row, uint32_t col, int count, const float (&v)[16]) {
+  T* to = static_cast<T*>(p) + row * ld + col;
+#pragma unroll
+  for (int t = 0; t < 16; ++t, to += ld)
+    if (t < count) *to = from_float<T>(v[t]);
+}
+// What follows the product for them.  (One activation's code at a time, none of it repeated for types or rows: the
+// decoding warps' loops share the instruction cache with this.)
+__device__ __forceinline__ void put_rows(const Epilogue& out, float (&v)[16], int64_t row, uint32_t col, int count, float bias) {
+  float res[16];
+  if (out.residual != nullptr) {
+    if (out.dtype == HI2_BF16) read_rows<__nv_bfloat16>(out.residual, out.ld_residual, row, col, count, res);
+    else if (out.dtype == HI2_F16) read_rows<__half>(out.residual, out.ld_residual, row, col, count, res);
+    else read_rows<float>(out.residual, out.ld_residual, row, col, count, res);
   }
   if (out.bias != nullptr) {
 #pragma unroll
     for (int t = 0; t < 16; ++t) v[t] += bias;
   }
-  switch (out.act) {  // (outside the loop: one activation's code at a time)
+  switch (out.act) {
     case HI2_ACT_RELU:
 #pragma unroll
       for (int t = 0; t < 16; ++t) v[t] = activate(v[t], HI2_ACT_RELU);
@@ -239,29 +313,17 @@ __device__ __forceinline__ void put_columns(const Epilogue& out, float (&v)[16],
 #pragma unroll
       for (int t = 0; t < 16; ++t) v[t] = activate(v[t], HI2_ACT_SILU);
       break;
-    case HI2_ACT_GELU:
-#pragma unroll 2
-      for (int t = 0; t < 16; ++t) v[t] = activate(v[t], HI2_ACT_GELU);
-      break;
-    case HI2_ACT_GELU_TANH:
-#pragma unroll 4
-      for (int t = 0; t < 16; ++t) v[t] = activate(v[t], HI2_ACT_GELU_TANH);
-      break;
+    case HI2_ACT_GELU: each(v, [](float x) { return activate(x, HI2_ACT_GELU); }); break;
+    case HI2_ACT_GELU_TANH: each(v, [](float x) { return activate(x, HI2_ACT_GELU_TANH); }); break;
     default: break;
   }
   if (out.residual != nullptr) {
 #pragma unroll
-    for (int t = 0; t < 16; ++t)
-      if (FULL || t < count) v[t] += to_float(res[t]);
+    for (int t = 0; t < 16; ++t) v[t] += res[t];
   }
-#pragma unroll
-  for (int t = 0; t < 16; ++t, to += out.ld_out)
-    if (FULL || t < count) *to = from_float<T>(v[t]);
-}
-template <typename T>
-__device__ __forceinline__ void put_columns(const Epilogue& out, float (&v)[16], int count, int64_t row, uint32_t col, float bias) {
-  if (count == 16) put_columns<T, true>(out, v, count, row, col, bias);
-  else put_columns<T, false>(out, v, count, row, col, bias);
+  if (out.dtype == HI2_BF16) write_rows<__nv_bfloat16>(out.out, out.ld_out, row, col, count, v);
+  else if (out.dtype == HI2_F16) write_rows<__half>(out.out, out.ld_out, row, col, count, v);
+  else write_rows<float>(out.out, out.ld_out, row, col, count, v);
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
@@ -278,7 +340,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < shape.x_stages; ++s) bar_init(&ctl->x_full[s], 1), bar_init(&ctl->x_empty[s], 1);
-    for (int s = 0; s < A_SLOTS; ++s) bar_init(&ctl->a_full[s], 2 * DECODE_WARPS), bar_init(&ctl->a_empty[s], 1);
+    for (int s = 0; s < MAX_SLOTS; ++s) bar_init(&ctl->a_full[s], 2 * DECODE_WARPS), bar_init(&ctl->a_empty[s], 1);
     for (int b = 0; b < 2; ++b) bar_init(&ctl->d_full[b], 1), bar_init(&ctl->d_empty[b], 2 * EPILOGUE_WARPS);
     for (int w = 0; w < DECODE_WARPS; ++w)
       for (int s = 0; s < RING_STAGES; ++s) bar_init(&ctl->ring_full[w][s], 1);
@@ -294,9 +356,8 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
   cluster_sync();  // the peer's barriers exist before anything signals them
   fence_after();
   const uint32_t tmem = ctl->tmem_base;
-  const uint32_t a_tmem = tmem + FIRST_A_COLUMN;
-  const int chunks = (int)(p.w.k / CHUNK), half0 = (chunks + 1) / 2;  // a step: one chunk of each half of the columns
-  const int row_pairs = (int)((p.w.groups_per_expert / 4 + 1) / 2);
+  const uint32_t d_columns = (uint32_t)(shape.width + 31) & ~31u;
+  const uint32_t a_tmem = tmem + 2 * d_columns;  // behind the two accumulators
   const int64_t first_item = blockIdx.x >> 1, stride = gridDim.x >> 1;
   chain_wait();  // the tile list, the activations, and whatever the outputs overwrite
   bool ok = true;
@@ -310,14 +371,14 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
     int64_t ahead_item = first_item;
     int ahead_copy = 0, ahead_stage = 0;
     Stream ahead{nullptr, 0, 1, 0, 0};
-    bool more = get_item(p, ahead_item, row_pairs, rank, item);
-    if (more) ahead = stream_of(p, group_form(p, item, quarter), half, half0, chunks);
+    bool more = get_item(p, shape, ahead_item, rank, item);
+    if (more) ahead = stream_of(p, shape, item, group_form(p, item, quarter), half);
     auto produce = [&]() {
       while (more && ahead_copy == ahead.copies) {
         ahead_item += stride, ahead_copy = 0;
         Item next;
-        more = get_item(p, ahead_item, row_pairs, rank, next);
-        if (more) ahead = stream_of(p, group_form(p, next, quarter), half, half0, chunks);
+        more = get_item(p, shape, ahead_item, rank, next);
+        if (more) ahead = stream_of(p, shape, next, group_form(p, next, quarter), half);
       }
       if (!more) return;
       const int from = ahead_copy * ahead.per_copy, bytes = min(ahead.per_copy, ahead.chunks - from) * ahead.slab;
@@ -329,10 +390,10 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
     if (lane == 0)
       for (int s = 0; s < RING_STAGES; ++s) produce();
     Decoder out{ctl, status, ring, ctl->ring_full[warp], a_tmem + half * A_COLUMNS + ((uint32_t)(quarter * 32) << 16),
-                {in_rank(s32(&ctl->a_full[0]), 0), in_rank(s32(&ctl->a_full[1]), 0)}, g, r, lane, 0, 0, 0, 1};
-    for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
+                in_rank(s32(&ctl->a_full[0]), 0), g, r, lane, shape.slots, 0, 0, 0, 1};
+    for (int64_t at = first_item; ok && get_item(p, shape, at, rank, item); at += stride) {
       const GroupForm form = group_form(p, item, quarter);
-      const Stream s = stream_of(p, form, half, half0, chunks);
+      const Stream s = stream_of(p, shape, item, form, half);
       LaneRow row{};
       if (s.slab != 0) {
         const RowConsts c = load_row(p.w.rows, ((int64_t)item.tile.expert * p.w.groups_per_expert + item.row_tile * 4 + quarter) * GROUP_ROWS + lane);
@@ -340,7 +401,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
         row.step_scale = __half2half2(__ushort_as_half((uint16_t)c.step_scale));
       }
       const auto run = [&](auto nbits, auto small) {
-        return steps<decltype(nbits)::value, decltype(small)::value>(out, s, form.shift(), row, half0, produce);
+        return steps<decltype(nbits)::value, decltype(small)::value>(out, s, form.shift(), row, item.count, produce);
       };
       typedef std::integral_constant<int, 2> Int2;
       typedef std::integral_constant<int, 4> Int4;
@@ -348,26 +409,28 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
       if (form.width() == 1) ok = form.small_steps() ? run(Int2(), std::true_type()) : run(Int2(), std::false_type());
       else if (form.width() == 2) ok = form.small_steps() ? run(Int4(), std::true_type()) : run(Int4(), std::false_type());
       else if (form.width() == 3) ok = form.small_steps() ? run(Int8(), std::true_type()) : run(Int8(), std::false_type());
-      else ok = run(std::integral_constant<int, 0>(), std::true_type());
+      else ok = empty_steps(out, s.chunks, item.count);
     }
   } else if (warp == X_WARP) {
     // ------------------------------------------------------------ activations
     int stage = 0;
     uint32_t phase = 1;
-    for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
+    for (int64_t at = first_item; ok && get_item(p, shape, at, rank, item); at += stride) {
       const int cols = (item.tile.end - item.tile.begin + 15) & ~15;  // of the product
       const int y = item.tile.begin + (int)rank * (cols / 2);
-      for (int i = 0; i < half0; ++i) {
+      const int second = second_chunks(shape, item);
+      for (int i = 0; i < item.count; ++i) {
         ok = __all_sync(0xffffffffu, bar_wait(&ctl->x_empty[stage], phase, &ctl->abort, status));
         if (!ok) break;
         if (lane == 0) {
-          const bool two = half0 + i < chunks;
+          const bool two = i < second;
+          const int chunk = item.first + i;
           if (rank == 0) bar_expect(&ctl->x_full[stage], (uint32_t)((two ? 2 : 1) * p.parts * box_bytes * 2));  // both blocks' bytes
           const uint32_t full = in_rank(s32(&ctl->x_full[stage]), 0);
           uint8_t* dst = smem + (size_t)stage * stage_bytes;
           for (int part = 0; part < p.parts; ++part) {
-            tma_load_pair(dst + part * box_bytes, &map, full, i * CHUNK, (int)(part * p.tiles.rows) + y);
-            if (two) tma_load_pair(dst + (p.parts + part) * box_bytes, &map, full, (half0 + i) * CHUNK, (int)(part * p.tiles.rows) + y);
+            tma_load_pair(dst + part * box_bytes, &map, full, chunk * CHUNK, (int)(part * p.tiles.rows) + y);
+            if (two) tma_load_pair(dst + (p.parts + part) * box_bytes, &map, full, (shape.half0 + chunk) * CHUNK, (int)(part * p.tiles.rows) + y);
           }
         }
         __syncwarp();
@@ -381,14 +444,15 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
     const uint32_t box = (uint32_t)box_bytes >> 4;
     int stage = 0, slot = 0, buf = 0;
     uint32_t phase = 0, slot_phase = 0, d_phase = 1;
-    for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
+    for (int64_t at = first_item; ok && get_item(p, shape, at, rank, item); at += stride) {
       const int cols = (item.tile.end - item.tile.begin + 15) & ~15;
       // fp16 operands (format 0 at bits 7 and 10), fp32 accumulator (1 << 4), N >> 3 at bit 17, M >> 4 at bit 24
       const uint32_t idesc = (1u << 4) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(2 * TILE_ROWS >> 4) << 24);
-      const uint32_t d = d_first + buf * MAX_WIDTH;
+      const uint32_t d = d_first + buf * d_columns;
+      const int second = second_chunks(shape, item);
       ok = __all_sync(0xffffffffu, bar_wait(&ctl->d_empty[buf], d_phase, &ctl->abort, status));
       if (!ok) break;
-      for (int i = 0; i < half0; ++i) {
+      for (int i = 0; i < item.count; ++i) {
         const uint32_t a = a_first + slot * SLOT_COLUMNS;
         const uint64_t b = b_first + (uint32_t)(stage * stage_bytes >> 4);
         ok = bar_wait(&ctl->x_full[stage], phase, &ctl->abort, status);
@@ -396,23 +460,23 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
-        if (lane == 0) {
+        if (elected()) {
           for (int part = 0; part < p.parts; ++part)
 #pragma unroll
             for (int kk = 0; kk < CHUNK / 16; ++kk)
               mma_pair(d, a + kk * 8, b + part * box + kk * 2, idesc, i > 0 || part > 0 || kk > 0 ? 1u : 0u);
-          if (half0 + i < chunks)
+          if (i < second)
             for (int part = 0; part < p.parts; ++part)
 #pragma unroll
               for (int kk = 0; kk < CHUNK / 16; ++kk)
                 mma_pair(d, a + A_COLUMNS + kk * 8, b + (p.parts + part) * box + kk * 2, idesc, 1u);
           commit_both(&ctl->a_empty[slot]);
           commit_both(&ctl->x_empty[stage]);
-          if (i == half0 - 1) commit_both(&ctl->d_full[buf]);
+          if (i == item.count - 1) commit_both(&ctl->d_full[buf]);
         }
         __syncwarp();
         if (++stage == shape.x_stages) stage = 0, phase ^= 1;
-        if (++slot == A_SLOTS) slot = 0, slot_phase ^= 1;
+        if (++slot == shape.slots) slot = 0, slot_phase ^= 1;
       }
       if (++buf == 2) buf = 0, d_phase ^= 1;
     }
@@ -422,33 +486,35 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
     const int quarter = warp & 3;
     int buf = 0;
     uint32_t phase = 0;
-    for (int64_t at = first_item; ok && get_item(p, at, row_pairs, rank, item); at += stride) {
+    for (int64_t at = first_item; ok && get_item(p, shape, at, rank, item); at += stride) {
       uint32_t col = NO_ROW;
       if (item.row_tile < (int)(p.w.groups_per_expert / 4))
         col = load_row(p.w.rows, ((int64_t)item.tile.expert * p.w.groups_per_expert + item.row_tile * 4 + quarter) * GROUP_ROWS + lane).out_row;
       const float bias = p.out.bias != nullptr && col != NO_ROW ? load_as_float(p.out.bias, p.out.dtype, col) : 0.0f;
       const int tokens = item.tile.end - item.tile.begin;
+      float* scale = ctl->scale[warp - FIRST_EPILOGUE];  // of the activation rows; read while the tile is computed
+      __syncwarp();
+      for (int t = lane; t < tokens; t += 32) {
+        scale[t] = p.row_scale[item.tile.begin + t];
+        if (p.out.pair_weight != nullptr) scale[t] *= p.out.pair_weight[p.tiles.pair(item.tile.begin + t)];
+      }
+      __syncwarp();
       ok = __all_sync(0xffffffffu, bar_wait(&ctl->d_full[buf], phase, &ctl->abort, status));
       if (!ok) break;
       fence_after();
-      const uint32_t taddr = tmem + buf * MAX_WIDTH + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t taddr = tmem + buf * d_columns + ((uint32_t)(quarter * 32) << 16);
+      Epilogue out = p.out;
+      if (shape.splits > 1) out.out = static_cast<float*>(out.out) + (int64_t)item.slice * p.tiles.rows * out.ld_out;
+#pragma unroll 1
       for (int t0 = 0; t0 < tokens; t0 += 16) {
-        const int count = min(16, tokens - t0);
-        const int64_t first = item.tile.begin + t0;
-        float scale = 0.0f;  // lane t: of activation row t0 + t
-        if (lane < count) {
-          scale = p.row_scale[first + lane];
-          if (p.out.pair_weight != nullptr) scale *= p.out.pair_weight[p.tiles.pair(first + lane)];
-        }
         float v[16];
         tmem_load16(taddr + t0, v);
 #pragma unroll
-        for (int t = 0; t < 16; ++t) v[t] *= __shfl_sync(0xffffffffu, scale, t);
-        if (col != NO_ROW) {
-          if (p.out.dtype == HI2_BF16) put_columns<__nv_bfloat16>(p.out, v, count, first, col, bias);
-          else if (p.out.dtype == HI2_F16) put_columns<__half>(p.out, v, count, first, col, bias);
-          else put_columns<float>(p.out, v, count, first, col, bias);
+        for (int t = 0; t < 16; t += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(scale + t0 + t);
+          v[t] *= f.x, v[t + 1] *= f.y, v[t + 2] *= f.z, v[t + 3] *= f.w;
         }
+        if (col != NO_ROW) put_rows(out, v, item.tile.begin + t0, col, min(16, tokens - t0), bias);
         __syncwarp();  // the next read of tensor memory is the whole warp's
       }
       fence_before();
@@ -465,6 +531,19 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
   if (warp == MMA_WARP) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// The slices' sums in order, and what follows the product.
+__global__ void __launch_bounds__(256)
+join_kernel(const float* __restrict__ partial, int splits, int64_t rows, int64_t n, const Epilogue out) {
+  chain_wait();
+  const int64_t values = rows * n;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < values; i += (int64_t)gridDim.x * blockDim.x) {
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) sum += partial[s * values + i];
+    out.put(i / n, (uint32_t)(i % n), sum);
   }
 }
 
@@ -485,6 +564,20 @@ EncodeFn encoder() {
 
 }  // namespace
 
+// Slices of the columns of one tensor, for tiles that are fewer than the SM pairs: the number that leaves the busiest
+// pair the fewest steps, with start and end of an item counted as six of them; each at least four steps.
+int wide_splits(const hi2_stored_weight& w, const Tiles& tiles, int64_t max_tiles) {
+  if (tiles.index != nullptr) return 1;
+  const int64_t items = (w.groups_per_expert / 4 + 1) / 2 * max_tiles, count = (w.k / CHUNK + 1) / 2;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int s = 1; s <= 16 && (s == 1 || count >= 4 * s); ++s) {
+    const int64_t cost = ceil_div(items * s, (int64_t)74) * (ceil_div(count, (int64_t)s) + 6);
+    if (cost < least) least = cost, best = s;
+  }
+  return best;
+}
+
 int wide_width(int64_t rows) {
   const int64_t tiles = ceil_div(rows, (int64_t)MAX_WIDTH);
   return (int)(ceil_div(ceil_div(rows, tiles), (int64_t)16) * 16);
@@ -496,11 +589,21 @@ int product_wide(const Product& p, cudaStream_t stream, const char* what) {
   Shape s;
   s.width = p.tiles.width;
   const int stage_bytes = 2 * p.parts * (s.width / 2) * CHUNK * 2;
-  s.x_stages = 150 * 1024 / stage_bytes;  // at least three
+  s.x_stages = 144 * 1024 / stage_bytes;  // at least three
   if (s.x_stages > MAX_X_STAGES) s.x_stages = MAX_X_STAGES;
+  s.slots = (512 - 2 * ((s.width + 31) & ~31)) / SLOT_COLUMNS;  // at least two
+  if (s.slots > MAX_SLOTS) s.slots = MAX_SLOTS;
+  s.chunks = (int)(p.w.k / CHUNK), s.half0 = (s.chunks + 1) / 2;
+  s.row_pairs = (int)((p.w.groups_per_expert / 4 + 1) / 2);
+  s.splits = wide_splits(p.w, p.tiles, p.max_tiles);
   size_t smem = (size_t)s.x_stages * stage_bytes + DECODE_WARPS * RING_STAGES * RING_BYTES + sizeof(Control) + 1024;
   // A block takes all of an SM's tensor memory: two must never be resident on one SM.
   if (smem < 120 * 1024) smem = 120 * 1024;
+  Product q = p;
+  if (s.splits > 1) {  // plain sums of the slices; joined below
+    q.out = Epilogue{};
+    q.out.out = p.partial, q.out.ld_out = p.w.rows_per_expert, q.out.dtype = HI2_F32;
+  }
 
   CUtensorMap map;
   const cuuint64_t dims[2] = {(cuuint64_t)p.w.k, (cuuint64_t)(p.tiles.rows * p.parts)};
@@ -519,7 +622,7 @@ int product_wide(const Product& p, cudaStream_t stream, const char* what) {
   int device = 0, sms = 148;
   cudaGetDevice(&device);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  const int64_t items = (p.w.groups_per_expert / 4 + 1) / 2 * p.max_tiles;
+  const int64_t items = (int64_t)s.row_pairs * s.splits * p.max_tiles;
   cudaLaunchConfig_t config = {};
   config.gridDim = (unsigned)(2 * (items < sms / 2 ? items : sms / 2));
   config.blockDim = THREADS, config.dynamicSmemBytes = smem, config.stream = stream;
@@ -527,7 +630,13 @@ int product_wide(const Product& p, cudaStream_t stream, const char* what) {
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute, config.numAttrs = 1;
-  cudaLaunchKernelEx(&config, wide_kernel, map, p, s);
+  cudaLaunchKernelEx(&config, wide_kernel, map, q, s);
+  const int rc = check_launch(what);
+  if (rc != HI2_OK || s.splits == 1) return rc;
+  const int64_t values = p.tiles.rows * p.w.rows_per_expert;
+  const int64_t blocks = ceil_div(values, (int64_t)256);
+  launch_link(join_kernel, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, stream, p.partial, s.splits, p.tiles.rows,
+              p.w.rows_per_expert, p.out);
   return check_launch(what);
 }
 
