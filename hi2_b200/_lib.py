@@ -174,6 +174,28 @@ def call(name: str, *args) -> None:
     check(fn(*args), name)
 
 
+def launch(name: str, index: int, *args) -> None:
+    """Like :func:`call` for the device ``index``, whose current stream goes behind ``args`` (plain numbers and
+    addresses).  A few microseconds less per launch, which is most of the time of the shortest calls."""
+    fn = _fast.get(name)
+    if fn is None:
+        fn = _fast[name] = getattr(load(), name)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, _current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _current_stream(index))
+    if rc != OK:
+        check(rc, name)
+
+
+_fast: dict = {}
+
+
+def _current_stream(index: int) -> int:
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def ptr(t: torch.Tensor | None):
     """Device address of a tensor (``None`` -> null)."""
     if t is None:

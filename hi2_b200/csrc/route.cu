@@ -63,17 +63,12 @@ __device__ __forceinline__ KEY take_best(KEY (&key)[PER], int lane, uint32_t& at
 
 // The top_k best keys: lane r ends up with the r-th choice's index (-1: none) and score.
 template <int PER, typename KEY, typename SCORE>
-__device__ __forceinline__ void choose(KEY (&key)[PER], const SCORE (&score)[PER], int top_k, int lane, int& index, SCORE& chosen,
-                                       SCORE& sum) {
+__device__ __forceinline__ void choose(KEY (&key)[PER], const SCORE* score, int top_k, int lane, int& index, SCORE& chosen, SCORE& sum) {
   index = -1, chosen = 0, sum = 0;
   for (int r = 0; r < top_k; ++r) {
     uint32_t at;
     if (take_best(key, lane, at) == 0) return;  // no open expert is left
-    SCORE s = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (at >> 5 == (uint32_t)i) s = score[i];
-    s = __shfl_sync(ALL, s, at & 31);
+    const SCORE s = score[at];
     sum += s;
     if (lane == r) index = (int)at, chosen = s;
   }
@@ -83,6 +78,10 @@ template <int PER, bool EXACT_KEYS>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32)
 route_kernel(const RouteParams p) {
   typedef typename std::conditional<EXACT_KEYS, double, float>::type SCORE;
+  __shared__ union {  // a token's scores; before them, where experts form groups, its keys
+    SCORE scores[PER * 32];
+    uint64_t keys[EXACT_KEYS ? PER * 32 : 1];
+  } shared[ROUTE_WARPS];
   const int lane = threadIdx.x & 31;
   const int64_t token = (int64_t)blockIdx.x * ROUTE_WARPS + (threadIdx.x >> 5);
   if (token >= p.tokens) return;
@@ -126,6 +125,7 @@ route_kernel(const RouteParams p) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) score[i] /= sum;
   }
+  SCORE* const of = shared[threadIdx.x >> 5].scores;
   int index;
   SCORE chosen, sum;
   if (EXACT_KEYS) {
@@ -137,19 +137,31 @@ route_kernel(const RouteParams p) {
       key[i] = open >> i & 1 ? key_of((double)score[i] + b) : 0;
     }
     if (p.groups > 1) {
+      // Several lanes read through a group each, and find its two best keys together.
       const int per = p.experts / p.groups;
-      uint64_t total = 0;  // lane q: the key of group q
-      for (int q = 0; q < p.groups; ++q) {
-        uint64_t in[PER];
+      uint64_t* const all = shared[threadIdx.x >> 5].keys;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int e = i * 32 + lane;
-          in[i] = e >= q * per && e < (q + 1) * per ? key[i] : 0;
+      for (int i = 0; i < PER; ++i) all[i * 32 + lane] = key[i];
+      __syncwarp();
+      int team = 32;  // lanes per group
+      while (team * p.groups > 32) team >>= 1;
+      const int mine = lane / team;
+      uint64_t first = 0, second = 0;
+      if (mine < p.groups)
+        for (int e = mine * per + lane % team; e < (mine + 1) * per; e += team) {
+          const uint64_t k = all[e];
+          if (k > first) second = first, first = k;
+          else if (k > second) second = k;
         }
-        uint32_t at;
-        const uint64_t first = take_best(in, lane, at), second = take_best(in, lane, at);
-        if (lane == q && first != 0) total = key_of(value_of(first) + (second != 0 ? value_of(second) : 0.0));
+      for (int d = team >> 1; d > 0; d >>= 1) {
+        const uint64_t f = __shfl_xor_sync(ALL, first, d), s = __shfl_xor_sync(ALL, second, d);
+        const uint64_t low = first < f ? first : f, high = second > s ? second : s;
+        first = first < f ? f : first;
+        second = low > high ? low : high;
       }
+      uint64_t total = first != 0 ? key_of(value_of(first) + (second != 0 ? value_of(second) : 0.0)) : 0;
+      total = __shfl_sync(ALL, total, (lane * team) & 31);  // lane q: the key of group q
+      if (lane >= p.groups) total = 0;
       uint32_t kept = 0;
       uint64_t of_group[1] = {total};
       for (int r = 0; r < p.top_groups; ++r) {
@@ -166,12 +178,19 @@ route_kernel(const RouteParams p) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) key[i] = key[i] != 0 ? key_of(logit[i]) : 0;
     }
-    choose(key, score, p.top_k, lane, index, chosen, sum);
+    __syncwarp();  // the keys have been read
+#pragma unroll
+    for (int i = 0; i < PER; ++i) of[i * 32 + lane] = score[i];
+    __syncwarp();
+    choose(key, of, p.top_k, lane, index, chosen, sum);
   } else {
     uint32_t key[PER];
 #pragma unroll
+    for (int i = 0; i < PER; ++i) of[i * 32 + lane] = score[i];
+    __syncwarp();
+#pragma unroll
     for (int i = 0; i < PER; ++i) key[i] = open >> i & 1 ? key_of(logit[i]) : 0;
-    choose(key, score, p.top_k, lane, index, chosen, sum);
+    choose(key, of, p.top_k, lane, index, chosen, sum);
   }
   if (lane < p.top_k) {
     if (p.renormalise) chosen /= sum > (SCORE)1e-20f ? sum : (SCORE)1e-20f;

@@ -1,10 +1,25 @@
 // Barriers, bulk copies and cluster addressing of the products with packed weights.
 #pragma once
 
+#include <atomic>
+
 #include "stored.cuh"
 
 namespace hi2 {
 namespace stored {
+
+// Lets a kernel have as much shared memory as there is; asked of the driver once per device.
+constexpr int MAX_SMEM = 227 * 1024;
+template <auto KERNEL>
+bool reserve_smem() {
+  static std::atomic<bool> done[64];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  if (device < 64 && done[device].load(std::memory_order_relaxed)) return true;
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM) != cudaSuccess) return false;
+  if (device < 64) done[device].store(true, std::memory_order_relaxed);
+  return true;
+}
 
 constexpr long long WAIT_CYCLES = 2000000000LL;  // about one second
 
@@ -18,12 +33,14 @@ __device__ __forceinline__ void bar_expect(unsigned long long* b, uint32_t bytes
 __device__ __forceinline__ void bar_arrive(unsigned long long* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(b)) : "memory");
 }
+// Sleeps up to 20 us for the phase.  (With the default limit waiting warps came back so often that a third of all
+// instructions of a wide product were their polls.)
 __device__ __forceinline__ bool bar_try(unsigned long long* b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
       "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok) : "r"(s32(b)), "r"(parity) : "memory");
+      : "=r"(ok) : "r"(s32(b)), "r"(parity), "r"(20000u) : "memory");
   return ok != 0;
 }
 // False when the limit ran out or another role of this block gave up.

@@ -287,7 +287,7 @@ few_kernel(const Product p, const int split) {
 template <int PARTS>
 int launch(const Product& p, int split, cudaStream_t stream, const char* what) {
   const size_t smem = smem_bytes<PARTS>();
-  if (cudaFuncSetAttribute(few_kernel<PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  if (!reserve_smem<few_kernel<PARTS>>())
     return fail(HI2_ERR_LAUNCH, "stored product: cannot reserve shared memory");
   const int64_t blocks = p.w.groups_per_expert / 4 * p.max_tiles * split;
   if (blocks >= (int64_t)1 << 31) return fail(HI2_ERR_ARG, "stored product: too many tiles");

@@ -617,11 +617,9 @@ int product_wide(const Product& p, cudaStream_t stream, const char* what) {
     set_error("%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
     return HI2_ERR_DRIVER;
   }
-  if (cudaFuncSetAttribute(wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  if (!reserve_smem<wide_kernel>())
     return fail(HI2_ERR_LAUNCH, "stored product: cannot reserve shared memory");
-  int device = 0, sms = 148;
-  cudaGetDevice(&device);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  constexpr int sms = 148;
   const int64_t items = (int64_t)s.row_pairs * s.splits * p.max_tiles;
   cudaLaunchConfig_t config = {};
   config.gridDim = (unsigned)(2 * (items < sms / 2 ? items : sms / 2));

@@ -16,13 +16,13 @@ import ctypes as C
 import torch
 
 from . import _lib
+from ._args import ACTIVATIONS, activation_number, no_gradient, on_device, output_rows, rows_of, workspace
 from .format import GROUP, HI2Tensor
 from .stack import MARK, stack_dims
 
-ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 CHUNK = 64  # columns that a row's codes are dealt out by
+FEW_TOKENS = 8  # up to here a product needs no workspace
 _GROUP_ROWS, _TILE_GROUPS = 32, 4
-_DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
 class _Struct(C.Structure):  # hi2_stored_weight
@@ -175,84 +175,49 @@ def lay_out_stack(arrays: dict, parts: int, device=None) -> StoredWeight:
     return _lay_out(arrays, experts, parts * int(rows[0]), k, True, device)
 
 
-def _activation(name) -> int:
-    try:
-        return ACTIVATIONS[name]
-    except (KeyError, TypeError):
-        raise ValueError(f"activation {name!r} is not one of {', '.join(map(str, ACTIVATIONS))}") from None
-
-
-def _rows_of(x: torch.Tensor, k: int, what: str) -> torch.Tensor:
-    """``x`` as ``[tokens, k]`` with unit column stride (a copy only where the strides ask for one)."""
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"{what}: unsupported dtype {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"{what}: the last dimension must be {k}, got shape {tuple(x.shape)}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: there is no gradient; call it under torch.no_grad()")
-    x = x if x.dim() == 2 else x.reshape(-1, k)
-    return x if x.stride(1) == 1 else x.contiguous()
-
-
-def _output(out, shape, like: torch.Tensor, what: str):
-    """``(result, its rows [tokens, n])``: fresh, or the caller's ``out``."""
-    if out is None:
-        out = torch.empty(shape, dtype=like.dtype, device=like.device)
-        return out, out.view(-1, shape[-1])
-    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device:
-        raise ValueError(f"{what}: out must have shape {tuple(shape)}, the dtype and the device of the activations")
-    if out.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what}: there is no gradient; call it under torch.no_grad()")
-    if out.numel() and out.stride(-1) != 1 and out.shape[-1] != 1:
-        raise ValueError(f"{what}: out must have unit column stride")
-    try:
-        rows = out.view(-1, shape[-1])
-    except RuntimeError:
-        raise ValueError(f"{what}: the rows of out must lie at one stride") from None
-    if rows.shape[0] > 1 and rows.stride(0) < shape[-1]:
-        raise ValueError(f"{what}: the rows of out overlap")
-    return out, rows
-
-
 def stored_linear(x: torch.Tensor, w: StoredWeight, bias: torch.Tensor | None = None, activation: str | None = None,
                   residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``activation(x @ W^T + bias) + residual`` with the packed weight ``w`` (``[rows, K]``), as ``[..., rows]`` in
     the dtype of ``x [..., K]`` (bf16, fp16 or fp32, any strides).  ``activation`` is None, ``"relu"``, ``"silu"``,
     ``"gelu"`` or ``"gelu_tanh"``; ``bias [rows]`` and ``residual [..., rows]`` have the dtype of ``x``.
-    ``out`` may be given, and may be ``residual``.  Queued on the current stream of the weight's device; a token with a
-    non-finite activation gets non-finite outputs and leaves the others alone."""
-    if w.experts != 1 or len(w.shape) != 2:
+    ``out`` may be given, and may be ``residual`` itself.  Queued on the current stream of the weight's device; a token with a
+    non-finite activation gets non-finite sums and leaves the others alone."""
+    if len(w.shape) != 2:
         raise ValueError("stored_linear: a stack of experts goes through moe.stored_experts")
-    act = _activation(activation)
-    rows = _rows_of(x, w.k, "stored_linear")
-    dev = _lib.need_cuda(x, bias, residual, out)
-    if dev != w.device:
-        raise RuntimeError(f"tensors on different devices: {dev} and {w.device}")
+    act = activation_number(activation)
+    rows, dtype = rows_of(x, w.k, "stored_linear")
+    dev = w.device
+    on_device("stored_linear", dev, x, bias, residual, out)
+    no_gradient("stored_linear", x, bias, residual, out)
     n, tokens = w.rows, rows.shape[0]
-    shape = (*x.shape[:-1], n)
-    for name, t, want in (("bias", bias, (n,)), ("residual", residual, shape)):
-        if t is None:
-            continue
-        if tuple(t.shape) != want or t.dtype != x.dtype:
-            raise ValueError(f"stored_linear: {name} must have shape {want} and dtype {x.dtype}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("stored_linear: there is no gradient; call it under torch.no_grad()")
-    y, y_rows = _output(out, shape, x, "stored_linear")
-    if tokens == 0:
-        return y
+    shape = (tokens, n) if x.dim() == 2 else (*x.shape[:-1], n)
     if bias is not None:
+        if bias.shape != (n,) or bias.dtype != x.dtype:
+            raise ValueError(f"stored_linear: bias must have shape {(n,)} and dtype {x.dtype}")
         bias = bias.contiguous()
-    res = None
+    res_ptr, ld_res = None, 0
     if residual is not None:
-        res = residual if residual.dim() == 2 else residual.reshape(-1, n)
+        if residual.shape != shape or residual.dtype != x.dtype:
+            raise ValueError(f"stored_linear: residual must have shape {shape} and dtype {x.dtype}")
+        res = residual if len(shape) == 2 else residual.reshape(-1, n)
         res = res if res.stride(1) == 1 else res.contiguous()
-    dtype = _DTYPES[x.dtype]
-    need = _lib.load().hi2_stored_linear_workspace_bytes(w.arg, dtype, tokens)
-    space = torch.empty(need, dtype=torch.uint8, device=dev)
-    _lib.call("hi2_stored_linear", w.arg, rows.data_ptr(), dtype, tokens, rows.stride(0), _lib.ptr(bias), act, _lib.ptr(res),
-              0 if res is None else res.stride(0), y_rows.data_ptr(), y_rows.stride(0), space.data_ptr(), need,
-              _lib.stream(dev))
-    return y
+        res_ptr, ld_res = res.data_ptr(), res.stride(0)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        ld_out = n
+    else:
+        y = output_rows(out, shape, x, "stored_linear")
+        ld_out = y.stride(0)
+    if tokens == 0:
+        return out
+    need = 0
+    space = at = None
+    if tokens > FEW_TOKENS:
+        need = _lib.load().hi2_stored_linear_workspace_bytes(w.arg, dtype, tokens)
+        space, at = workspace(need, dev)
+    _lib.launch("hi2_stored_linear", dev.index, w.arg, rows.data_ptr(), dtype, tokens, rows.stride(0),
+                None if bias is None else bias.data_ptr(), act, res_ptr, ld_res, out.data_ptr(), ld_out, at, need)
+    return out
 
 
 __all__ = ["ACTIVATIONS", "StoredWeight", "lay_out", "lay_out_stack", "stored_linear"]

@@ -17,9 +17,11 @@ import torch
 from torch import nn
 
 from . import _lib
+from ._args import DTYPES, activation_number, no_gradient, on_device, output_rows, rows_of, workspace
 from .hessian import HessianStats
 from .stats import ColumnStats
 
+_SCORES = {"softmax": 0, "sigmoid": 1}
 _EXPERT = re.compile(r"^(.*?\bexperts)\.(\d+)\.([^.]+)(?:\.weight)?$")
 # projections of one expert that always see the same input (gate/up; Mixtral w1/w3)
 _SAME_INPUT = {"up_proj": "gate_proj", "w3": "w1"}
@@ -227,29 +229,31 @@ def route(logits: torch.Tensor, top_k: int, scores: str = "softmax", bias: torch
     score, over the sum of the chosen ones with ``renormalise`` (at least 1e-20), times ``scale``.  A logit or a bias that is ``-inf`` or NaN
     closes its expert for the row (it takes no part in the softmax either); slots that no open expert is left for (all of them, in a row without any) get index
     -1 and weight 0, which :func:`stored_experts` passes over.  At most 1024 experts, 32 groups and ``top_k`` 32."""
-    if scores not in ("softmax", "sigmoid"):
+    sigmoid = _SCORES.get(scores)
+    if sigmoid is None:
         raise ValueError(f"route: scores must be 'softmax' or 'sigmoid', not {scores!r}")
-    from .linear import _rows_of
-
     if logits.dim() < 1:
         raise ValueError("route: logits must have a dimension of experts")
     experts = logits.shape[-1]
-    rows = _rows_of(logits, experts, "route")
-    dev = _lib.need_cuda(logits, bias)
-    if bias is not None and (tuple(bias.shape) != (experts,) or bias.dtype != torch.float32):
-        raise ValueError(f"route: bias must be a float32 tensor of shape ({experts},)")
-    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
-        raise ValueError("route: there is no gradient; call it under torch.no_grad()")
-    shape = (*logits.shape[:-1], int(top_k))
+    rows, dtype = rows_of(logits, experts, "route")
+    dev = logits.device
+    if not logits.is_cuda or bias is not None:
+        _lib.need_cuda(logits, bias)
+    no_gradient("route", logits, bias)
+    top_k = int(top_k)
     if top_k < 1 or top_k > experts:
         raise ValueError(f"route: top_k={top_k} of {experts} experts")
+    bias_ptr = None
+    if bias is not None:
+        if bias.shape != (experts,) or bias.dtype != torch.float32:
+            raise ValueError(f"route: bias must be a float32 tensor of shape ({experts},)")
+        bias = bias.contiguous()
+        bias_ptr = bias.data_ptr()
+    shape = (*logits.shape[:-1], top_k)
     index = torch.empty(shape, dtype=torch.int64, device=dev)
     weight = torch.empty(shape, dtype=torch.float32, device=dev)
-    if bias is not None:
-        bias = bias.contiguous()
-    _lib.call("hi2_route", rows.data_ptr(), _lib.DTYPES[rows.dtype], rows.shape[0], experts, rows.stride(0), int(top_k),
-              1 if scores == "sigmoid" else 0, _lib.ptr(bias), int(groups), int(groups if top_groups is None else top_groups),
-              1 if renormalise else 0, float(scale), index.data_ptr(), weight.data_ptr(), _lib.stream(dev))
+    _lib.launch("hi2_route", dev.index, rows.data_ptr(), dtype, rows.shape[0], experts, rows.stride(0), top_k, sigmoid, bias_ptr, groups,
+                groups if top_groups is None else top_groups, 1 if renormalise else 0, scale, index.data_ptr(), weight.data_ptr())
     return index, weight
 
 
@@ -261,33 +265,34 @@ def stored_experts(x: torch.Tensor, index: torch.Tensor, weight: torch.Tensor, g
     ``[..., top_k]`` as :func:`route` gives them; a slot whose index is not an expert's (-1) adds nothing.  The
     slots of a token are added in their order: equal inputs give equal bits.  Queued on the current stream; nothing
     is read back."""
-    from .linear import _DTYPES, _activation, _output, _rows_of
-
     if len(gate_up.shape) != 3 or len(down.shape) != 3 or gate_up.experts != down.experts or gate_up.k != down.rows or (
             gate_up.rows != 2 * down.k):
         raise ValueError(f"stored_experts: stacks {gate_up.shape} and {down.shape} are not the gate/up and down of one layer")
-    act = _activation(activation)
-    rows = _rows_of(x, gate_up.k, "stored_experts")
-    dev = _lib.need_cuda(x, index, weight, out)
-    if dev != gate_up.device or dev != down.device:
-        raise RuntimeError(f"tensors on different devices: {dev}, {gate_up.device} and {down.device}")
+    act = activation_number(activation)
+    rows, dtype = rows_of(x, gate_up.k, "stored_experts")
+    dev = gate_up.device
+    on_device("stored_experts", dev, x, index, weight, out)
+    if down.device != dev:
+        raise RuntimeError(f"tensors on different devices: {dev} and {down.device}")
     if index.shape != weight.shape or index.dim() != x.dim() or index.shape[:-1] != x.shape[:-1] or index.shape[-1] < 1:
         raise ValueError("stored_experts: index and weight must be [..., top_k] over the rows of x")
-    if index.dtype not in (torch.int64, torch.int32) or weight.dtype not in _DTYPES:
+    if index.dtype not in (torch.int64, torch.int32) or weight.dtype not in DTYPES:
         raise ValueError("stored_experts: index must hold integers, weight fp32, fp16 or bf16")
-    if weight.requires_grad and torch.is_grad_enabled():
-        raise ValueError("stored_experts: there is no gradient; call it under torch.no_grad()")
-    y, y_rows = _output(out, tuple(x.shape), x, "stored_experts")
+    no_gradient("stored_experts", x, weight, out)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        ld_out = down.rows
+    else:
+        ld_out = output_rows(out, x.shape, x, "stored_experts").stride(0)
     tokens, top_k = rows.shape[0], index.shape[-1]
     if tokens == 0:
-        return y
+        return out
     index, weight = index.to(torch.int64).contiguous(), weight.to(torch.float32).contiguous()
-    dtype = _DTYPES[x.dtype]
     need = _lib.load().hi2_stored_experts_workspace_bytes(gate_up.arg, dtype, tokens, top_k)
-    space = torch.empty(need, dtype=torch.uint8, device=dev)
-    _lib.call("hi2_stored_experts", gate_up.arg, down.arg, rows.data_ptr(), dtype, tokens, rows.stride(0), index.data_ptr(),
-              weight.data_ptr(), top_k, act, y_rows.data_ptr(), y_rows.stride(0), space.data_ptr(), need, _lib.stream(dev))
-    return y
+    space, at = workspace(need, dev)
+    _lib.launch("hi2_stored_experts", dev.index, gate_up.arg, down.arg, rows.data_ptr(), dtype, tokens, rows.stride(0), index.data_ptr(),
+                weight.data_ptr(), top_k, act, out.data_ptr(), ld_out, at, need)
+    return out
 
 
 class StoredExperts(nn.Module):
