@@ -51,21 +51,20 @@ lay_out_kernel(const hi2_stored_weight w, const int32_t* __restrict__ src_row, c
 
 // ---- activations of wide products ---------------------------------------------------------------------
 // A team of warps per activation row: largest value, then the fp16 parts relative to its power of two.  A
-// lane keeps up to HOLD pieces of 16 columns in registers; HOLD = 0 forms them twice.
-constexpr int PREP_THREADS = 128;
-
-template <int WARPS, int HOLD>
-__global__ void __launch_bounds__(PREP_THREADS)
+// lane keeps HOLD pieces of 16 columns in registers; HOLD = 0 forms them twice.
+template <int THREADS, int WARPS, int HOLD, int PARTS>
+__global__ void __launch_bounds__(THREADS)
 prepare_kernel(const Product p, const int32_t* __restrict__ used) {
   constexpr int TEAM = WARPS * 32;
   const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
-  const int64_t row = (int64_t)blockIdx.x * (PREP_THREADS / TEAM) + team;
+  const int64_t row = (int64_t)blockIdx.x * (THREADS / TEAM) + team;
   if (row >= (used == nullptr ? p.tiles.rows : (int64_t)*used)) return;  // a team of several warps is the whole block
-  int64_t from = row, expert = 0;
+  int64_t from = row;
+  int expert = 0;
   if (p.tiles.index != nullptr) {
-    const int64_t pair = p.tiles.pair(row);
-    expert = p.tiles.index[pair];
-    if (p.from.kind != FROM_GATED) from = pair / p.from.top_k;
+    const int pair = (int)p.tiles.pair(row);
+    expert = (int)p.tiles.index[pair];
+    if (p.from.kind != FROM_GATED) from = (uint32_t)pair / (uint32_t)p.from.top_k;
   }
   const int groups = (int)(p.w.k / 16);
   constexpr int KEEP = HOLD == 0 ? 1 : HOLD;
@@ -97,10 +96,10 @@ prepare_kernel(const Product p, const int32_t* __restrict__ used) {
   if (lane == 0) p.row_scale[row] = power.back;
   auto store = [&](int g, const float (&x)[16]) {
     uint4 hi[2], lo[2];
-    split16(x, power.to, hi, lo);
+    split16<PARTS>(x, power.to, hi, lo);
     uint4* dst = reinterpret_cast<uint4*>(p.xs + row * p.w.k + (int64_t)g * 16);
     dst[0] = hi[0], dst[1] = hi[1];
-    if (p.parts == 2) {
+    if (PARTS == 2) {
       dst = reinterpret_cast<uint4*>(p.xs + (p.tiles.rows + row) * p.w.k + (int64_t)g * 16);
       dst[0] = lo[0], dst[1] = lo[1];
     }
@@ -117,58 +116,59 @@ prepare_kernel(const Product p, const int32_t* __restrict__ used) {
   }
 }
 
+template <int THREADS, int WARPS, int HOLD>
+void launch_prepare(const Product& p, const int32_t* used, cudaStream_t stream) {
+  const unsigned grid = (unsigned)ceil_div(p.tiles.rows, (int64_t)(THREADS / 32 / WARPS));
+  if (p.parts == 1) prepare_kernel<THREADS, WARPS, HOLD, 1><<<grid, THREADS, 0, stream>>>(p, used);
+  else prepare_kernel<THREADS, WARPS, HOLD, 2><<<grid, THREADS, 0, stream>>>(p, used);
+}
+// Two warps per row where the rows fill the machine (32768 rows of 2048: 65 us; one warp with four pieces per lane 80); else a
+// block per row, one piece per thread
+// as far as that goes (32 rows of 11008 columns: 14 us with 128 threads, which form everything twice).
 int prepare(const Product& p, const int32_t* used, cudaStream_t stream) {
-  const int64_t rows = p.tiles.rows;
-  if (p.w.k <= 32 * 4 * 16) prepare_kernel<1, 4><<<(unsigned)ceil_div(rows, (int64_t)4), PREP_THREADS, 0, stream>>>(p, used);
-  else if (p.w.k <= 128 * 4 * 16) prepare_kernel<4, 4><<<(unsigned)rows, PREP_THREADS, 0, stream>>>(p, used);
-  else prepare_kernel<4, 0><<<(unsigned)rows, PREP_THREADS, 0, stream>>>(p, used);
+  const int64_t pieces = p.w.k / 16;
+  if (pieces <= 128 && p.tiles.rows >= 148 * 16) launch_prepare<64, 2, 2>(p, used, stream);
+  else if (pieces <= 128) launch_prepare<128, 4, 1>(p, used, stream);
+  else if (pieces <= 512) launch_prepare<512, 16, 1>(p, used, stream);
+  else if (pieces <= 1024) launch_prepare<512, 16, 2>(p, used, stream);
+  else launch_prepare<512, 16, 0>(p, used, stream);
   return check_launch("stored: activations");
 }
 
 // ---- dispatch -----------------------------------------------------------------------------------------
-// Stable counting sort of the (token, slot) pairs by expert in one block: every warp counts its stretch of
-// the pairs, the counts are summed over the warps and experts, and every warp places its stretch in order
-// (lanes that name the same expert find each other by a match).  Also the list of token tiles.
-constexpr int SORT_WARPS = 32, SORT_BATCH = 8;
+// Counting sort of the (token, slot) pairs by expert in one block, and the list of token tiles.  Pairs of one expert come
+// in no particular order: a row's result does not depend on its place, so the outputs are the same every time.
+// (Keeping the order, by matching the lanes of a warp that name the same expert, took 36 us for 32768 pairs.)
+constexpr int SORT_THREADS = 1024, SORT_BATCH = 8;
 constexpr int MAX_EXPERTS = 1024;
 
-__global__ void __launch_bounds__(SORT_WARPS * 32)
+__global__ void __launch_bounds__(SORT_THREADS)
 dispatch_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, int tile_width, int32_t* __restrict__ pair_of,
                 int32_t* __restrict__ row_of, int32_t* __restrict__ used, int32_t* __restrict__ tile_count,
                 TokenTile* __restrict__ tiles) {
-  extern __shared__ int32_t counts[];  // [warps][experts]
-  __shared__ int32_t warp_sums[2][SORT_WARPS];
+  __shared__ int32_t next[MAX_EXPERTS];  // counts, then the next row of every expert
+  __shared__ int32_t warp_sums[2][SORT_THREADS / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < SORT_WARPS * experts; i += blockDim.x) counts[i] = 0;
+  next[threadIdx.x] = 0;
   __syncthreads();
-  int32_t* mine = counts + warp * experts;
-  const int64_t per = ceil_div(ceil_div(pairs, (int64_t)SORT_WARPS), (int64_t)32) * 32;
-  const int64_t first = warp * per, last = first + per < pairs ? first + per : pairs;
-  auto load = [&](int64_t i, int64_t (&e)[SORT_BATCH]) {  // several at a time: a load takes most of a microsecond
+  auto load = [&](int64_t i, int (&e)[SORT_BATCH]) {  // several at a time: a load takes most of a microsecond
 #pragma unroll
     for (int b = 0; b < SORT_BATCH; ++b) {
-      const int64_t at = i + 32 * b + lane;
-      e[b] = at < last ? index[at] : -1;
-      if (e[b] < 0 || e[b] >= experts) e[b] = -1;
+      const int64_t at = i + (int64_t)SORT_THREADS * b + threadIdx.x, v = at < pairs ? index[at] : -1;
+      e[b] = v >= 0 && v < experts ? (int)v : -1;
     }
   };
-  for (int64_t i = first; i < last; i += 32 * SORT_BATCH) {
-    int64_t e[SORT_BATCH];
+  for (int64_t i = 0; i < pairs; i += SORT_THREADS * SORT_BATCH) {
+    int e[SORT_BATCH];
     load(i, e);
 #pragma unroll
     for (int b = 0; b < SORT_BATCH; ++b)
-      if (e[b] >= 0) atomicAdd(mine + e[b], 1);  // a count: the order of the additions does not matter
+      if (e[b] >= 0) atomicAdd(next + e[b], 1);
   }
   __syncthreads();
   // thread e: the expert's total, its first row and its first tile (exclusive sums over the experts)
   const int e = threadIdx.x;
-  int32_t total = 0;
-  if (e < experts)
-    for (int v = 0; v < SORT_WARPS; ++v) {
-      const int32_t c = counts[v * experts + e];
-      counts[v * experts + e] = total;
-      total += c;
-    }
+  const int32_t total = next[e];
   const int32_t own_tiles = (total + tile_width - 1) / tile_width;
   int32_t rows_to = total, tiles_to = own_tiles;
 #pragma unroll
@@ -179,33 +179,26 @@ dispatch_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, i
   if (lane == 31) warp_sums[0][warp] = rows_to, warp_sums[1][warp] = tiles_to;
   __syncthreads();
   for (int v = 0; v < warp; ++v) rows_to += warp_sums[0][v], tiles_to += warp_sums[1][v];
-  if (threadIdx.x == blockDim.x - 1) *used = rows_to, *tile_count = tiles_to;
-  if (e < experts) {
-    const int32_t begin = rows_to - total;
-    for (int v = 0; v < SORT_WARPS; ++v) counts[v * experts + e] += begin;
-    for (int t = 0; t < own_tiles; ++t) {
-      const int b = begin + t * tile_width;
-      tiles[tiles_to - own_tiles + t] = TokenTile{e, b, b + tile_width < rows_to ? b + tile_width : rows_to};
-    }
+  if (threadIdx.x == SORT_THREADS - 1) *used = rows_to, *tile_count = tiles_to;
+  const int32_t begin = rows_to - total;
+  next[e] = begin;
+  for (int t = 0; t < own_tiles; ++t) {
+    const int b = begin + t * tile_width;
+    tiles[tiles_to - own_tiles + t] = TokenTile{e, b, b + tile_width < rows_to ? b + tile_width : rows_to};
   }
   __syncthreads();
-  for (int64_t i = first; i < last; i += 32 * SORT_BATCH) {
-    int64_t e[SORT_BATCH];
+  for (int64_t i = 0; i < pairs; i += SORT_THREADS * SORT_BATCH) {
+    int e[SORT_BATCH];
     load(i, e);
 #pragma unroll
     for (int b = 0; b < SORT_BATCH; ++b) {
-      const int64_t at = i + 32 * b + lane;
-      const int x = (int)e[b];
-      const uint32_t same = __match_any_sync(0xffffffffu, x);
+      const int64_t at = i + (int64_t)SORT_THREADS * b + threadIdx.x;
       int32_t row = -1;
-      if (x >= 0) {
-        row = mine[x] + __popc(same & ((1u << lane) - 1u));
+      if (e[b] >= 0) {
+        row = atomicAdd(next + e[b], 1);
         pair_of[row] = (int32_t)at;
       }
-      if (at < last) row_of[at] = row;
-      __syncwarp();
-      if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
-      __syncwarp();
+      if (at < pairs) row_of[at] = row;
     }
   }
 }
@@ -248,12 +241,12 @@ struct Carver {
 };
 
 // Which kernel takes a product.
-inline bool few(int64_t tokens) { return tokens <= FEW_WIDTH; }
+inline bool few(int64_t tokens) { return tokens <= 2 * FEW_WIDTH; }
 inline int64_t rows_per_expert(int64_t experts, int64_t pairs) {  // with half as many again as on average
   const int64_t busy = ceil_div(3 * pairs, 2 * experts);
   return busy < pairs ? busy : pairs;
 }
-inline bool few_experts(int64_t experts, int64_t pairs) { return rows_per_expert(experts, pairs) <= FEW_WIDTH; }
+inline bool few_experts(int64_t experts, int64_t pairs) { return rows_per_expert(experts, pairs) <= 2 * FEW_WIDTH; }
 inline bool apart(int64_t pairs) { return pairs <= FEW_WIDTH; }  // every pair a tile of its own
 
 inline int parts_of(int dtype) { return dtype == HI2_BF16 ? 1 : 2; }
@@ -398,11 +391,7 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
     const int64_t busy = rows_per_expert(experts, pairs);
     tiles = Tiles{index, space.pair_of, space.tile_count, space.tiles, pairs, experts, small ? FEW_WIDTH : wide_width(busy)};
     max_tiles = pairs / tiles.width + experts + 1;
-    const size_t smem = (size_t)SORT_WARPS * experts * sizeof(int32_t);
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(dispatch_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-      return fail(HI2_ERR_LAUNCH, "stored_experts: cannot reserve shared memory");
-    dispatch_kernel<<<1, SORT_WARPS * 32, smem, s>>>(index, pairs, experts, tiles.width, space.pair_of, space.row_of, space.used,
+    dispatch_kernel<<<1, SORT_THREADS, 0, s>>>(index, pairs, experts, tiles.width, space.pair_of, space.row_of, space.used,
                                                     space.tile_count, space.tiles);
     if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
   }

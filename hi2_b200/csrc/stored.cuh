@@ -251,6 +251,7 @@ __device__ __forceinline__ PowerOfTwo power_for(float top) {
   return PowerOfTwo{__uint_as_float((uint32_t)(127 - e) << 23), __uint_as_float((uint32_t)(127 + e) << 23)};
 }
 // The fp16 parts of 16 values times `to`, as two 16-byte words each.
+template <int PARTS>
 __device__ __forceinline__ void split16(const float (&v)[16], float to, uint4 (&hi)[2], uint4 (&lo)[2]) {
   uint32_t h[8], l[8];
 #pragma unroll
@@ -258,7 +259,7 @@ __device__ __forceinline__ void split16(const float (&v)[16], float to, uint4 (&
     const float a = v[2 * i] * to, b = v[2 * i + 1] * to;
     const __half2 both = __floats2half2_rn(a, b);
     h[i] = bits(both);
-    l[i] = bits(__floats2half2_rn(a - __low2float(both), b - __high2float(both)));
+    l[i] = PARTS == 1 ? 0u : bits(__floats2half2_rn(a - __low2float(both), b - __high2float(both)));
   }
   hi[0] = make_uint4(h[0], h[1], h[2], h[3]), hi[1] = make_uint4(h[4], h[5], h[6], h[7]);
   lo[0] = make_uint4(l[0], l[1], l[2], l[3]), lo[1] = make_uint4(l[4], l[5], l[6], l[7]);
@@ -308,6 +309,13 @@ struct Tiles {
     }
     out = TokenTile{(int)e, (int)b, (int)(b + width < rows ? b + width : rows)};
     return true;
+  }
+  // With a list, or of one tensor: how many there are, and one of them.
+  __device__ __forceinline__ int64_t number() const { return count != nullptr ? *count : (rows + width - 1) / width; }
+  __device__ __forceinline__ TokenTile at(int64_t t) const {
+    if (count != nullptr) return list[t];
+    const int64_t b = t * width;
+    return TokenTile{0, (int)b, (int)(b + width < rows ? b + width : rows)};
   }
   __device__ __forceinline__ int64_t pair(int64_t row) const { return pair_of == nullptr ? row : pair_of[row]; }
 };

@@ -150,6 +150,13 @@ few_kernel(const Product p, const int split) {
   const int slab = form.slab_bytes(), copy_shift = 3 - form.width(), per_copy = 1 << copy_shift;  // 4, 2, 1 chunks
   const uint8_t* const data = static_cast<const uint8_t*>(p.w.data) + (int64_t)form.base * 16;
   const int copies = form.width() == 0 ? 0 : (mine + per_copy - 1) >> copy_shift;
+  // What the activations need is asked for ahead of the packed data: behind it, it waited 3 us for its turn at the memory.
+  {
+    const int64_t first = (int64_t)tile.expert * p.w.k + (int64_t)c0 * CHUNK, columns = (int64_t)n * CHUNK;
+    if (p.w.inv_scale != nullptr)
+      for (int64_t i = 32 * threadIdx.x; i < columns; i += 32 * THREADS) prefetch_l2(p.w.inv_scale + first + i);
+    for (int64_t i = 2048 * threadIdx.x; i < columns; i += 2048 * THREADS) prefetch_l2(p.w.had + (first + i) / 16);
+  }
   auto issue = [&](int copy, int stage) {  // by one lane
     const int j = copy << copy_shift, b = j / HALF_CHUNKS, count = min(per_copy, mine - j);
     const int chunk = c0 + b * BLOCK_CHUNKS + (half == 0 ? 0 : b == blocks - 1 ? last_half0 : HALF_CHUNKS) + j % HALF_CHUNKS;
@@ -200,7 +207,7 @@ few_kernel(const Product p, const int split) {
       const int piece = (second ? 4 * half0 : 0) + lane;
       const bool in = piece < 4 * (second ? chunks : half0);
       int64_t from = tile.begin + r;
-      if (p.tiles.index != nullptr && p.from.kind != FROM_GATED) from = p.tiles.pair(from) / p.from.top_k;
+      if (p.tiles.index != nullptr && p.from.kind != FROM_GATED) from = (uint32_t)p.tiles.pair(from) / (uint32_t)p.from.top_k;
       float v[16];
       float top = 0.0f;
       if (in) {
@@ -213,7 +220,7 @@ few_kernel(const Product p, const int split) {
       if (lane == 0) sm.scale[b & 1][second][r] = power.back;
       if (in) {
         uint4 hi[2], lo[2];
-        split16(v, power.to, hi, lo);
+        split16<PARTS>(v, power.to, hi, lo);
         uint4* dst = reinterpret_cast<uint4*>(xs + r * X_PITCH + piece * 16);
         dst[0] = hi[0], dst[1] = hi[1];
         if (PARTS == 2) {

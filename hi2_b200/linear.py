@@ -21,7 +21,7 @@ from .format import GROUP, HI2Tensor
 from .stack import MARK, stack_dims
 
 CHUNK = 64  # columns that a row's codes are dealt out by
-FEW_TOKENS = 8  # up to here a product needs no workspace
+FEW_TOKENS = 16  # up to here a product needs no workspace
 _GROUP_ROWS, _TILE_GROUPS = 32, 4
 
 
