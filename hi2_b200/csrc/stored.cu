@@ -207,6 +207,7 @@ dispatch_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, i
 __global__ void __launch_bounds__(256)
 combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ row_of, const int64_t* __restrict__ index, int experts, int64_t tokens, int top_k, int64_t hidden,
                void* __restrict__ out, int dtype, int64_t ld_out) {
+  chain_wait();
   const int64_t quads = hidden / 4, total = tokens * quads;
   for (int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; id < total; id += (int64_t)gridDim.x * blockDim.x) {
     const int64_t t = id / quads, c = id % quads * 4;
@@ -352,7 +353,7 @@ extern "C" int hi2_stored_linear(const hi2_stored_weight* w, const void* x, int 
   const bool small = few(tokens);
   const Product p{*w, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), 1},
                   Tiles{nullptr, nullptr, nullptr, nullptr, tokens, 1, space.width}, space.max_tiles, parts_of(dtype),
-                  Epilogue{nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}, space.xs, space.scale, space.partial};
+                  Epilogue{nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}, false, space.xs, space.scale, space.partial};
   if (small) return product_few(p, s, "stored_linear");
   const int rc = prepare(p, nullptr, s);
   return rc != HI2_OK ? rc : product_wide(p, s, "stored_linear");
@@ -396,9 +397,9 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
     if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
   }
   const Product up{*gate_up, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), top_k}, tiles, max_tiles, parts,
-                   Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, space.xs, space.scale, nullptr};
+                   Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, false, space.xs, space.scale, nullptr};
   const Product dn{*down, Source{space.z, 2 * inner, FROM_GATED, act, true, top_k}, tiles, max_tiles, parts,
-                   Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, space.xs, space.scale, nullptr};
+                   Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, true, space.xs, space.scale, nullptr};
   for (const Product* p : {&up, &dn}) {
     if (small) {
       rc = product_few(*p, s, "stored_experts");
@@ -410,6 +411,6 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   }
   int64_t blocks = ceil_div(tokens * (hidden / 4), (int64_t)256);
   if (blocks > 148 * 16) blocks = 148 * 16;
-  combine_kernel<<<(unsigned)blocks, 256, 0, s>>>(space.y, space.row_of, index, experts, tokens, top_k, hidden, out, dtype, ld_out);
+  launch_link(combine_kernel, dim3((unsigned)blocks), dim3(256), 0, s, space.y, space.row_of, index, experts, tokens, top_k, hidden, out, dtype, ld_out);
   return check_launch("stored_experts: combine");
 }

@@ -328,6 +328,7 @@ struct Product {
   int64_t max_tiles;
   int parts;               // fp16 parts of an activation: 2 where the second holds what the first one's rounding lost
   Epilogue out;
+  bool settled;            // index and tile list were complete before the kernel ahead of this one set out
   // wide products only: the prepared activations fp16 [parts, rows, k], the powers of two they were divided by, and the
   // sums of the slices fp32 [wide_splits, rows, rows of the tensor] where there are several
   __half* xs;

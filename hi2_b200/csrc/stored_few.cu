@@ -35,7 +35,7 @@ struct Shared {
     uint8_t ring[WARPS][RING_STAGES][RING_BYTES];
     float sums[2][FEW_WIDTH][SUM_PITCH];  // of the two halves, once the rings are done with
   };
-  float scale[2][2][FEW_WIDTH];         // of the block being multiplied and of the one before; of each half
+  float scale[2][FEW_WIDTH];            // of each half and row (of a block: below)
   uint32_t out_row[TILE_ROWS];
   unsigned long long full[WARPS][RING_STAGES];
   volatile uint32_t abort;
@@ -129,7 +129,7 @@ few_kernel(const Product p, const int split) {
   const int row_tile = (int)(blockIdx.x / split) % row_tiles;
   int32_t* const status = p.w.status;
   TokenTile tile;
-  if (p.tiles.index != nullptr) chain_wait();  // which expert comes from an earlier kernel
+  if (p.tiles.index != nullptr && !p.settled) chain_wait();  // which expert comes from an earlier kernel
   if (!p.tiles.get(blockIdx.x / split / row_tiles, tile)) return;  // the same for all blocks of a cluster
   const int tokens = tile.end - tile.begin;
 
@@ -189,6 +189,7 @@ few_kernel(const Product p, const int split) {
     for (int i = 0; i < 4; ++i) total[m][i] = 0.0f;
 
   chain_wait();  // the activations
+  chain_next();
   bool ok = true;
   Ring ring{&sm.ring[warp][0][0], &sm.full[warp][0], slab, 0, 0};
   int next_copy = RING_STAGES;
@@ -197,13 +198,15 @@ few_kernel(const Product p, const int split) {
     ++next_copy;
     __syncwarp();
   };
-  for (int b = 0; b < blocks; ++b) {
-    const int chunks = b == blocks - 1 ? last_chunks : BLOCK_CHUNKS;
-    const int half0 = b == blocks - 1 ? last_half0 : HALF_CHUNKS;
-    // ---- the block's activations, a warp per row and half: up to 32 pieces of 16 columns, one per lane
-    __syncthreads();  // nobody reads the block before any more (and the barriers' words are set)
-    for (int u = warp; u < 2 * tokens; u += WARPS) {
-      const int r = u >> 1, second = u & 1;
+  // Shared memory holds eight rows of a block; fewer rows leave room for several blocks, which are prepared together.
+  const int together = FEW_WIDTH / tokens;
+  for (int b0 = 0; b0 < blocks; b0 += together) {
+    const int here = min(together, blocks - b0);
+    // ---- the activations, a warp per block, row and half: up to 32 pieces of 16 columns, one per lane
+    __syncthreads();  // nobody reads the blocks before any more (and the barriers' words are set)
+    for (int u = warp; u < 2 * tokens * here; u += WARPS) {
+      const int second = u & 1, place = u >> 1, b = b0 + place / tokens, r = place % tokens;
+      const int chunks = b == blocks - 1 ? last_chunks : BLOCK_CHUNKS, half0 = b == blocks - 1 ? last_half0 : HALF_CHUNKS;
       const int piece = (second ? 4 * half0 : 0) + lane;
       const bool in = piece < 4 * (second ? chunks : half0);
       int64_t from = tile.begin + r;
@@ -217,44 +220,47 @@ few_kernel(const Product p, const int split) {
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
       const PowerOfTwo power = power_for(top);
-      if (lane == 0) sm.scale[b & 1][second][r] = power.back;
+      if (lane == 0) sm.scale[second][place] = power.back;
       if (in) {
         uint4 hi[2], lo[2];
         split16<PARTS>(v, power.to, hi, lo);
-        uint4* dst = reinterpret_cast<uint4*>(xs + r * X_PITCH + piece * 16);
+        uint4* dst = reinterpret_cast<uint4*>(xs + place * X_PITCH + piece * 16);
         dst[0] = hi[0], dst[1] = hi[1];
         if (PARTS == 2) {
-          dst = reinterpret_cast<uint4*>(xs + (FEW_WIDTH + r) * X_PITCH + piece * 16);
+          dst = reinterpret_cast<uint4*>(xs + (FEW_WIDTH + place) * X_PITCH + piece * 16);
           dst[0] = lo[0], dst[1] = lo[1];
         }
       }
     }
     __syncthreads();
-    // ---- this warp's chunks of the block
-    float acc[2][4];
+    for (int sub = 0; sub < here; ++sub) {
+      const int chunks = b0 + sub == blocks - 1 ? last_chunks : BLOCK_CHUNKS, half0 = b0 + sub == blocks - 1 ? last_half0 : HALF_CHUNKS;
+      // ---- this warp's chunks of a block; lanes without a row of their own read the last one's
+      float acc[2][4];
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
-    const int first = half == 0 ? 0 : half0, count = half == 0 ? half0 : chunks - half0;
-    if (ok) {  // one loop per code width
-      const __half* x = xs + g * X_PITCH + first * CHUNK + 16 * t;
-      const auto run = [&](auto nbits, auto small) {
-        return multiply<PARTS, decltype(nbits)::value, decltype(small)::value>(ring, x, count, first_word, pair_unit, rows, acc, &sm.abort,
-                                                                                   status, refill);
-      };
-      typedef std::integral_constant<int, 2> Int2;
-      typedef std::integral_constant<int, 4> Int4;
-      typedef std::integral_constant<int, 8> Int8;
-      if (form.width() == 1) ok = form.small_steps() ? run(Int2(), std::true_type()) : run(Int2(), std::false_type());
-      else if (form.width() == 2) ok = form.small_steps() ? run(Int4(), std::true_type()) : run(Int4(), std::false_type());
-      else if (form.width() == 3) ok = form.small_steps() ? run(Int8(), std::true_type()) : run(Int8(), std::false_type());
-    }
-    const float s0 = sm.scale[b & 1][half][2 * t], s1 = sm.scale[b & 1][half][2 * t + 1];
+        for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
+      const int first = half == 0 ? 0 : half0, count = half == 0 ? half0 : chunks - half0;
+      if (ok) {  // one loop per code width
+        const __half* x = xs + (sub * tokens + min(g, tokens - 1)) * X_PITCH + first * CHUNK + 16 * t;
+        const auto run = [&](auto nbits, auto small) {
+          return multiply<PARTS, decltype(nbits)::value, decltype(small)::value>(ring, x, count, first_word, pair_unit, rows, acc, &sm.abort,
+                                                                                     status, refill);
+        };
+        typedef std::integral_constant<int, 2> Int2;
+        typedef std::integral_constant<int, 4> Int4;
+        typedef std::integral_constant<int, 8> Int8;
+        if (form.width() == 1) ok = form.small_steps() ? run(Int2(), std::true_type()) : run(Int2(), std::false_type());
+        else if (form.width() == 2) ok = form.small_steps() ? run(Int4(), std::true_type()) : run(Int4(), std::false_type());
+        else if (form.width() == 3) ok = form.small_steps() ? run(Int8(), std::true_type()) : run(Int8(), std::false_type());
+      }
+      const float s0 = sm.scale[half][sub * tokens + min(2 * t, tokens - 1)], s1 = sm.scale[half][sub * tokens + min(2 * t + 1, tokens - 1)];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      total[m][0] += acc[m][0] * s0, total[m][1] += acc[m][1] * s1;
-      total[m][2] += acc[m][2] * s0, total[m][3] += acc[m][3] * s1;
+      for (int m = 0; m < 2; ++m) {
+        total[m][0] += acc[m][0] * s0, total[m][1] += acc[m][1] * s1;
+        total[m][2] += acc[m][2] * s0, total[m][3] += acc[m][3] * s1;
+      }
     }
   }
   if (__syncthreads_or(!ok)) let_copies_land();
