@@ -60,13 +60,14 @@ __device__ __forceinline__ __half2 half2_of(uint32_t v) { return *reinterpret_ca
 // A ladder as (lo, lo), and (step, step) times the powers of two that the decoder below asks for.  The format
 // defines lo = fp16(fma_f32(u, lo_scale, lo_min)) and step = fp16(u * step_scale).
 struct Ladder {
-  __half2 lo, step[3];
+  __half2 lo, step[2];
 };
 // Two codes of neighbouring columns at bit `AT` of both halves of w -> fp16(lo + code * step).
 //
-// SMALL steps (of all rows of the group: at most 65504 / 2^20, for 8-bit codes 65504 / 2^22): the field by itself is
-// the fp16 subnormal code * 2^(AT - 24), and one fused multiply-add with step * 2^(24 - AT), an fp16 number for the
-// fields' bits 4, 6 and 8 (2-bit codes), 4 (4-bit), 2 (8-bit), forms the weight with the format's single rounding.
+// SMALL steps (of all rows of the group: at most 65504 / 2^18 with 2-bit codes, 2^20 with 4-bit, 2^22 with 8-bit ones):
+// the field by itself is the fp16 subnormal code * 2^(AT - 24), and one fused multiply-add with step * 2^(24 - AT), an
+// fp16 number for fields at bits 6 and 8 (2-bit codes), 4 (4-bit), 2 (8-bit), forms the weight with the format's single
+// rounding.
 // Any step: 1024 + code * 2^AT is an fp16 number with the code in its mantissa; a fused multiply-add takes
 // it to the code (exact), a second one forms the weight.  fp16 arithmetic issues every other clock and shares its pipe
 // with the warp-level products: 2048 INT2 weights and their products take a scheduler 172 clocks with small
@@ -92,16 +93,16 @@ __device__ __forceinline__ void ladders(uint32_t pairs, const float (&lo_min)[2]
   const float v = __uint_as_float(__byte_perm(pairs, 0x4b000000u, 0x7442)) - 8388608.0f;
   const __half2 lo = __floats2half2_rn(fmaf(u, lo_scale[0], lo_min[0]), fmaf(v, lo_scale[1], lo_min[1]));
   const __half2 steps = __hadd2(half2_of(__byte_perm(pairs, 0x64646464u, 0x4341)), half2_of(0xe400e400u));
-  __half2 step[3];
+  __half2 step[2];
   step[0] = __hmul2(steps, step_scale);
-  if (SMALL) {  // 2^10, then 2^6, 2^8, 2^10 or 2^12 (2^20 and 2^22 are no fp16 numbers)
+  if (SMALL) {  // 2^10, then 2^6 and 2^8, 2^10 or 2^12 (2^16 is no fp16 number)
     const __half2 up = __hmul2(step[0], half2_of(0x64006400u));
-    if (NBITS == 2) step[0] = __hmul2(up, half2_of(0x54005400u)), step[1] = __hmul2(up, half2_of(0x5c005c00u)), step[2] = __hmul2(up, half2_of(0x64006400u));
-    else step[0] = __hmul2(up, half2_of(NBITS == 4 ? 0x64006400u : 0x6c006c00u));
+    step[0] = __hmul2(up, half2_of(NBITS == 2 ? 0x54005400u : NBITS == 4 ? 0x64006400u : 0x6c006c00u));
+    if (NBITS == 2) step[1] = __hmul2(up, half2_of(0x5c005c00u));
   }
   a.lo = __low2half2(lo), b.lo = __high2half2(lo);
 #pragma unroll
-  for (int i = 0; i < (SMALL && NBITS == 2 ? 3 : 1); ++i) a.step[i] = __low2half2(step[i]), b.step[i] = __high2half2(step[i]);
+  for (int i = 0; i < (SMALL && NBITS == 2 ? 2 : 1); ++i) a.step[i] = __low2half2(step[i]), b.step[i] = __high2half2(step[i]);
 }
 
 // Word h of a 16-column piece -> its pairs of neighbouring columns.
@@ -109,10 +110,11 @@ template <int NBITS, bool SMALL>
 __device__ __forceinline__ void decode_word(uint32_t w, const Ladder& l, uint32_t* out) {
   const __half2 lo = l.lo, st = l.step[0];
   if (NBITS == 2 && SMALL) {
-    const uint32_t up = w << 6, down = w >> 6;
-    out[0] = weight_pair<6, 2, true>(up, lo, l.step[1]), out[1] = weight_pair<8, 2, true>(up, lo, st);
-    out[2] = weight_pair<4, 2, true>(w, lo, l.step[2]), out[3] = weight_pair<6, 2, true>(w, lo, l.step[1]), out[4] = weight_pair<8, 2, true>(w, lo, st);
-    out[5] = weight_pair<4, 2, true>(down, lo, l.step[2]), out[6] = weight_pair<6, 2, true>(down, lo, l.step[1]), out[7] = weight_pair<8, 2, true>(down, lo, st);
+    const uint32_t up = w << 4, down = w >> 4;
+    out[0] = weight_pair<8, 2, true>(w << 8, lo, st), out[1] = weight_pair<6, 2, true>(up, lo, l.step[1]);
+    out[2] = weight_pair<8, 2, true>(up, lo, st), out[3] = weight_pair<6, 2, true>(w, lo, l.step[1]);
+    out[4] = weight_pair<8, 2, true>(w, lo, st), out[5] = weight_pair<6, 2, true>(down, lo, l.step[1]);
+    out[6] = weight_pair<8, 2, true>(down, lo, st), out[7] = weight_pair<8, 2, true>(w >> 6, lo, st);
   } else if (NBITS == 2) {
     out[0] = weight_pair<0, 2, false>(w, lo, st), out[1] = weight_pair<2, 2, false>(w, lo, st), out[2] = weight_pair<4, 2, false>(w, lo, st);
     out[3] = weight_pair<6, 2, false>(w, lo, st), out[4] = weight_pair<8, 2, false>(w, lo, st);

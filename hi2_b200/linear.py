@@ -123,7 +123,7 @@ def _lay_out_on(f: dict, experts: int, rows: int, k: int, stacked: bool, dev: to
     at = lead.clamp_min(0)
     live = lead >= 0
     # groups whose largest step, times the power of two that its codes are read with, is still an fp16 number
-    limit = torch.where(nbits == 8, 65504.0 / 2**22, 65504.0 / 2**20)
+    limit = 65504.0 / 2.0 ** (16 + 2 * torch.log2(nbits.double()).round())  # 2^18, 2^20, 2^22
     step = 255 * consts[:, 2].float()
     small = ((step >= 0) & (step <= limit))[src.clamp_min(0)] | (src < 0)
     small = small.view(-1, _GROUP_ROWS).all(1).long()

@@ -334,8 +334,8 @@ int hi2_allocate_bits(const double* cost, const double* bits, int n_cand, int64_
  * (hi2_lay_out_rows).  This struct lives in HOST memory; its pointers are device pointers.  `rows` holds
  * four words per sorted row (output row, fp16 lo_min and lo_scale, fp16 step scale, 0), `groups` two per 32
  * sorted rows, which share one format (first 16-byte unit of the group's data; log2 of the code width, 0 for
- * padding, log2(block / 16) << 2, and 1 << 4 where 255 * step scale of every row is at most 65504 / 2^20, for
- * 8-bit codes 65504 / 2^22); groups_per_expert is a multiple of 4.  had [experts, k/16], inv_scale fp32 [experts, k] (reciprocal smoothing vector; null: none).
+ * padding, log2(block / 16) << 2, and 1 << 4 where 255 * step scale of every row is at most 65504 / 2^18,
+ * 2^20 or 2^22 for 2-, 4- and 8-bit codes); groups_per_expert is a multiple of 4.  had [experts, k/16], inv_scale fp32 [experts, k] (reciprocal smoothing vector; null: none).
  * status: a device int that a bounded wait which ran out raises and nothing clears. */
 typedef struct {
   const void* data;
