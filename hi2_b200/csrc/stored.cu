@@ -136,39 +136,38 @@ int prepare(const Product& p, const int32_t* used, cudaStream_t stream) {
 }
 
 // ---- dispatch -----------------------------------------------------------------------------------------
-// Counting sort of the (token, slot) pairs by expert in one block, and the list of token tiles.  Pairs of one expert come
-// in no particular order: a row's result does not depend on its place, so the outputs are the same every time.
-// (Keeping the order, by matching the lanes of a warp that name the same expert, took 36 us for 32768 pairs.)
+// Counting sort of the (token, slot) pairs by expert: one block counts and makes the list of token tiles, then many place
+// the pairs.  Pairs of one expert come in no particular order: a row's result does not depend on its place, so the outputs
+// are the same every time.  (One block for both, keeping the order by matching the lanes of a warp, took 36 us for 32768
+// pairs, without the order 26 us: its scattered stores all go through one SM.)
 constexpr int SORT_THREADS = 1024, SORT_BATCH = 8;
 constexpr int MAX_EXPERTS = 1024;
 
+__device__ __forceinline__ int expert_of(const int64_t* index, int64_t pair, int64_t pairs, int experts) {
+  const int64_t e = pair < pairs ? index[pair] : -1;
+  return e >= 0 && e < experts ? (int)e : -1;
+}
+
 __global__ void __launch_bounds__(SORT_THREADS)
-dispatch_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, int tile_width, int32_t* __restrict__ pair_of,
-                int32_t* __restrict__ row_of, int32_t* __restrict__ used, int32_t* __restrict__ tile_count,
-                TokenTile* __restrict__ tiles) {
-  __shared__ int32_t next[MAX_EXPERTS];  // counts, then the next row of every expert
+count_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, int tile_width, int32_t* __restrict__ next_row,
+             int32_t* __restrict__ used, int32_t* __restrict__ tile_count, TokenTile* __restrict__ tiles) {
+  __shared__ int32_t counts[MAX_EXPERTS];
   __shared__ int32_t warp_sums[2][SORT_THREADS / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  next[threadIdx.x] = 0;
+  counts[threadIdx.x] = 0;
   __syncthreads();
-  auto load = [&](int64_t i, int (&e)[SORT_BATCH]) {  // several at a time: a load takes most of a microsecond
+  for (int64_t i = threadIdx.x; i < pairs; i += SORT_THREADS * SORT_BATCH) {
+    int e[SORT_BATCH];  // several at a time: a load takes most of a microsecond
 #pragma unroll
-    for (int b = 0; b < SORT_BATCH; ++b) {
-      const int64_t at = i + (int64_t)SORT_THREADS * b + threadIdx.x, v = at < pairs ? index[at] : -1;
-      e[b] = v >= 0 && v < experts ? (int)v : -1;
-    }
-  };
-  for (int64_t i = 0; i < pairs; i += SORT_THREADS * SORT_BATCH) {
-    int e[SORT_BATCH];
-    load(i, e);
+    for (int b = 0; b < SORT_BATCH; ++b) e[b] = expert_of(index, i + SORT_THREADS * b, pairs, experts);
 #pragma unroll
     for (int b = 0; b < SORT_BATCH; ++b)
-      if (e[b] >= 0) atomicAdd(next + e[b], 1);
+      if (e[b] >= 0) atomicAdd(counts + e[b], 1);
   }
   __syncthreads();
   // thread e: the expert's total, its first row and its first tile (exclusive sums over the experts)
   const int e = threadIdx.x;
-  const int32_t total = next[e];
+  const int32_t total = counts[e];
   const int32_t own_tiles = (total + tile_width - 1) / tile_width;
   int32_t rows_to = total, tiles_to = own_tiles;
 #pragma unroll
@@ -181,25 +180,39 @@ dispatch_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, i
   for (int v = 0; v < warp; ++v) rows_to += warp_sums[0][v], tiles_to += warp_sums[1][v];
   if (threadIdx.x == SORT_THREADS - 1) *used = rows_to, *tile_count = tiles_to;
   const int32_t begin = rows_to - total;
-  next[e] = begin;
+  if (e < experts) next_row[e] = begin;
   for (int t = 0; t < own_tiles; ++t) {
     const int b = begin + t * tile_width;
     tiles[tiles_to - own_tiles + t] = TokenTile{e, b, b + tile_width < rows_to ? b + tile_width : rows_to};
   }
+}
+
+// A block reserves rows for its pairs of every expert at once, and hands them out.
+constexpr int PLACE_PAIRS = 2048;
+__global__ void __launch_bounds__(SORT_THREADS)
+place_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, int32_t* __restrict__ next_row, int32_t* __restrict__ pair_of,
+             int32_t* __restrict__ row_of) {
+  __shared__ int32_t next[MAX_EXPERTS];
+  constexpr int EACH = PLACE_PAIRS / SORT_THREADS;
+  const int64_t first = (int64_t)blockIdx.x * PLACE_PAIRS + threadIdx.x;
+  next[threadIdx.x] = 0;
   __syncthreads();
-  for (int64_t i = 0; i < pairs; i += SORT_THREADS * SORT_BATCH) {
-    int e[SORT_BATCH];
-    load(i, e);
+  chain_wait();
+  int e[EACH], place[EACH];
 #pragma unroll
-    for (int b = 0; b < SORT_BATCH; ++b) {
-      const int64_t at = i + (int64_t)SORT_THREADS * b + threadIdx.x;
-      int32_t row = -1;
-      if (e[b] >= 0) {
-        row = atomicAdd(next + e[b], 1);
-        pair_of[row] = (int32_t)at;
-      }
-      if (at < pairs) row_of[at] = row;
-    }
+  for (int b = 0; b < EACH; ++b) e[b] = expert_of(index, first + SORT_THREADS * b, pairs, experts);
+#pragma unroll
+  for (int b = 0; b < EACH; ++b) place[b] = e[b] >= 0 ? atomicAdd(next + e[b], 1) : 0;
+  __syncthreads();
+  if (next[threadIdx.x] > 0) next[threadIdx.x] = atomicAdd(next_row + threadIdx.x, next[threadIdx.x]);
+  __syncthreads();
+#pragma unroll
+  for (int b = 0; b < EACH; ++b) {
+    const int64_t at = first + SORT_THREADS * b;
+    if (at >= pairs) continue;
+    const int32_t row = e[b] >= 0 ? next[e[b]] + place[b] : -1;
+    if (row >= 0) pair_of[row] = (int32_t)at;
+    row_of[at] = row;
   }
 }
 
@@ -280,7 +293,7 @@ struct LinearSpace {
 struct ExpertSpace {
   __half* xs = nullptr;  // of the gate/up product, then of the down product
   float *scale = nullptr, *z, *y;
-  int32_t *pair_of = nullptr, *row_of = nullptr, *used = nullptr, *tile_count = nullptr;
+  int32_t *pair_of = nullptr, *row_of = nullptr, *next_row = nullptr, *used = nullptr, *tile_count = nullptr;
   TokenTile* tiles = nullptr;
   size_t bytes;
   ExpertSpace(void* ws, const hi2_stored_weight& gate_up, int dtype, int64_t tokens, int top_k) {
@@ -293,6 +306,7 @@ struct ExpertSpace {
       tile_count = used == nullptr ? nullptr : used + 32;
       pair_of = c.take<int32_t>(pairs);
       row_of = c.take<int32_t>(pairs);
+      next_row = c.take<int32_t>(gate_up.experts);
       tiles = c.take<TokenTile>(pairs / 8 + gate_up.experts + 1);
     }
     if (!few_experts(gate_up.experts, pairs)) {
@@ -392,8 +406,10 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
     const int64_t busy = rows_per_expert(experts, pairs);
     tiles = Tiles{index, space.pair_of, space.tile_count, space.tiles, pairs, experts, small ? FEW_WIDTH : wide_width(busy)};
     max_tiles = pairs / tiles.width + experts + 1;
-    dispatch_kernel<<<1, SORT_THREADS, 0, s>>>(index, pairs, experts, tiles.width, space.pair_of, space.row_of, space.used,
-                                                    space.tile_count, space.tiles);
+    count_kernel<<<1, SORT_THREADS, 0, s>>>(index, pairs, experts, tiles.width, space.next_row, space.used, space.tile_count, space.tiles);
+    if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
+    launch_link(place_kernel, dim3((unsigned)ceil_div(pairs, (int64_t)PLACE_PAIRS)), dim3(SORT_THREADS), 0, s, index, pairs, experts,
+                space.next_row, space.pair_of, space.row_of);
     if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
   }
   const Product up{*gate_up, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), top_k}, tiles, max_tiles, parts,

@@ -103,11 +103,11 @@ def _lay_out_on(f: dict, experts: int, rows: int, k: int, stacked: bool, dev: to
     if not all(good[1:]):
         raise ValueError("lay_out: the row offsets do not fit the buffers")
 
-    # Rows by (block, width), a stable order.  Every format's rows fill groups of 32; the last one of each is
+    # Rows by (width, block), a stable order.  Every format's rows fill groups of 32; the last one of each is
     # filled up with padding, and so are the groups of an expert to whole tiles.
     shift = torch.log2(block.double()).round().long() - 4       # 0, 1, 2
     width = torch.log2(nbits.double()).round().long()           # 1, 2, 3
-    key = (3 * shift + width - 1).view(experts, rows)
+    key = (3 * (width - 1) + shift).view(experts, rows)
     counts = torch.zeros(experts, 9, dtype=torch.int64, device=dev).scatter_add_(1, key, torch.ones_like(key))
     groups = (counts + _GROUP_ROWS - 1) // _GROUP_ROWS
     first = groups.cumsum(1) - groups                           # first group of every format
