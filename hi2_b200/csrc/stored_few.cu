@@ -25,24 +25,24 @@ namespace {
 constexpr int WARPS = 8, THREADS = 256;
 constexpr int BLOCK_CHUNKS = 16, BLOCK_COLUMNS = BLOCK_CHUNKS * CHUNK;
 constexpr int HALF_CHUNKS = BLOCK_CHUNKS / 2;
-constexpr int RING_STAGES = 3, RING_BYTES = 3072;  // a stage: four chunks of INT2, two of INT4, one of INT8
+constexpr int RING_STAGES = 2, RING_BYTES = 3072;  // a stage: four chunks of INT2, two of INT4, one of INT8
 constexpr int X_PITCH = BLOCK_COLUMNS + 8;         // halves; the extra 16 bytes keep 128-bit reads of eight rows apart
 constexpr int SUM_PITCH = TILE_ROWS + 4;
 constexpr int MAX_SPLIT = 8;
+template <int PARTS>
+constexpr int PLACES = PARTS == 1 ? 16 : 8;        // of a row's 1024 columns in shared memory; at least FEW_WIDTH
 
 struct Shared {
-  union {
-    uint8_t ring[WARPS][RING_STAGES][RING_BYTES];
-    float sums[2][FEW_WIDTH][SUM_PITCH];  // of the two halves, once the rings are done with
-  };
-  float scale[2][FEW_WIDTH];            // of each half and row (of a block: below)
+  uint8_t ring[WARPS][RING_STAGES][RING_BYTES];
+  float sums[2][FEW_WIDTH][SUM_PITCH];  // of the two halves
+  float scale[2][16];                   // of each half and place
   uint32_t out_row[TILE_ROWS];
   unsigned long long full[WARPS][RING_STAGES];
   volatile uint32_t abort;
 };
 template <int PARTS>
 constexpr size_t smem_bytes() {
-  return sizeof(Shared) + (size_t)PARTS * FEW_WIDTH * X_PITCH * sizeof(__half) + 16;
+  return sizeof(Shared) + (size_t)PARTS * PLACES<PARTS> * X_PITCH * sizeof(__half) + 16;
 }
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -99,7 +99,7 @@ __device__ __forceinline__ bool multiply(Ring& ring, const __half* x, int count,
       decode_rows<NBITS, SMALL>(slab, first_word, pair_unit, rows, w);
 #pragma unroll
       for (int part = 0; part < PARTS; ++part) {
-        const __half* from = x + part * FEW_WIDTH * X_PITCH;
+        const __half* from = x + part * PLACES<PARTS> * X_PITCH;
         const uint4 x0 = *reinterpret_cast<const uint4*>(from), x1 = *reinterpret_cast<const uint4*>(from + 8);
         const uint32_t k[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
@@ -119,18 +119,20 @@ __device__ __forceinline__ bool multiply(Ring& ring, const __half* x, int count,
 
 template <int PARTS>
 __global__ void __launch_bounds__(THREADS, 2)
-few_kernel(const Product p, const int split) {
+few_kernel(const Product p, const int split, const int run) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared& sm = *reinterpret_cast<Shared*>(raw);
   __half* const xs = reinterpret_cast<__half*>((reinterpret_cast<uintptr_t>(raw) + sizeof(Shared) + 15) & ~(uintptr_t)15);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int row_tiles = (int)(p.w.groups_per_expert / 4), runs = (row_tiles + run - 1) / run;
   const int rank = (int)(blockIdx.x % split);
-  const int row_tiles = (int)(p.w.groups_per_expert / 4);
-  const int row_tile = (int)(blockIdx.x / split) % row_tiles;
+  const uint32_t which = blockIdx.x / split;
+  int row_tile = (int)(which % runs) * run;
+  const int last_tile = min(row_tile + run, row_tiles) - 1;
   int32_t* const status = p.w.status;
   TokenTile tile;
   if (p.tiles.index != nullptr && !p.settled) chain_wait();  // which expert comes from an earlier kernel
-  if (!p.tiles.get(blockIdx.x / split / row_tiles, tile)) return;  // the same for all blocks of a cluster
+  if (!p.tiles.get(which / runs, tile)) return;  // the same for all blocks of a cluster
   const int tokens = tile.end - tile.begin;
 
   // ---- this warp's stream of packed data
@@ -142,14 +144,14 @@ few_kernel(const Product p, const int split) {
   const int last_half0 = (last_chunks + 1) / 2;
   const int last_mine = half == 0 ? last_half0 : last_chunks - last_half0;
   const int mine = (blocks - 1) * HALF_CHUNKS + last_mine;
-  const int64_t group = (int64_t)tile.expert * p.w.groups_per_expert + row_tile * 4 + quarter;
-  const GroupForm form = load_group(p.w.groups, group);
+  const int64_t first_group = (int64_t)tile.expert * p.w.groups_per_expert + quarter;
+  GroupForm form = load_group(p.w.groups, first_group + row_tile * 4);
   RowConsts consts[4];
+  auto load_rows = [&](int tile_of_rows) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) consts[r] = load_row(p.w.rows, group * GROUP_ROWS + 8 * r + g);
-  const int slab = form.slab_bytes(), copy_shift = 3 - form.width(), per_copy = 1 << copy_shift;  // 4, 2, 1 chunks
-  const uint8_t* const data = static_cast<const uint8_t*>(p.w.data) + (int64_t)form.base * 16;
-  const int copies = form.width() == 0 ? 0 : (mine + per_copy - 1) >> copy_shift;
+    for (int r = 0; r < 4; ++r) consts[r] = load_row(p.w.rows, (first_group + tile_of_rows * 4) * GROUP_ROWS + 8 * r + g);
+  };
+  load_rows(row_tile);
   // What the activations need is asked for ahead of the packed data: behind it, it waited 3 us for its turn at the memory.
   {
     const int64_t first = (int64_t)tile.expert * p.w.k + (int64_t)c0 * CHUNK, columns = (int64_t)n * CHUNK;
@@ -157,152 +159,179 @@ few_kernel(const Product p, const int split) {
       for (int64_t i = 32 * threadIdx.x; i < columns; i += 32 * THREADS) prefetch_l2(p.w.inv_scale + first + i);
     for (int64_t i = 2048 * threadIdx.x; i < columns; i += 2048 * THREADS) prefetch_l2(p.w.had + (first + i) / 16);
   }
+  Ring ring{&sm.ring[warp][0][0], &sm.full[warp][0], 0, 0, 0};
+  const uint8_t* data;
+  int copy_shift, copies, next_copy;
   auto issue = [&](int copy, int stage) {  // by one lane
-    const int j = copy << copy_shift, b = j / HALF_CHUNKS, count = min(per_copy, mine - j);
+    const int j = copy << copy_shift, b = j / HALF_CHUNKS, count = min(1 << copy_shift, mine - j);
     const int chunk = c0 + b * BLOCK_CHUNKS + (half == 0 ? 0 : b == blocks - 1 ? last_half0 : HALF_CHUNKS) + j % HALF_CHUNKS;
-    bar_expect(&sm.full[warp][stage], (uint32_t)(count * slab));
-    bulk_load(sm.ring[warp][stage], data + (int64_t)chunk * slab, (uint32_t)(count * slab), &sm.full[warp][stage]);
+    bar_expect(&sm.full[warp][stage], (uint32_t)(count * ring.slab));
+    bulk_load(sm.ring[warp][stage], data + (int64_t)chunk * ring.slab, (uint32_t)(count * ring.slab), &sm.full[warp][stage]);
   };
-  if (lane == 0) {
-    for (int s = 0; s < RING_STAGES; ++s) bar_init(&sm.full[warp][s], 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    for (int c = 0; c < RING_STAGES && c < copies; ++c) issue(c, c);
-  }
-  if (threadIdx.x == 0) sm.abort = 0;
-  LaneRows rows;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const RowConsts c = consts[r];
-    rows.lo_min[r] = c.lo_min(), rows.lo_scale[r] = c.lo_scale();
-    const __half s = __ushort_as_half((uint16_t)c.step_scale);
-    if (r & 1) rows.step_scale[r / 2] = __halves2half2(__low2half(rows.step_scale[r / 2]), s);
-    else rows.step_scale[r / 2] = __half2half2(s);
-    if (half == 0 && t == 0) sm.out_row[quarter * 32 + 8 * r + g] = c.out_row;
-  }
-  const int pair_unit = (4 >> form.shift()) * g + (t >> form.shift()), first_word = code_word(g, t);
-
-  float total[2][4];
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) total[m][i] = 0.0f;
-
-  chain_wait();  // the activations
-  chain_next();
-  bool ok = true;
-  Ring ring{&sm.ring[warp][0][0], &sm.full[warp][0], slab, 0, 0};
-  int next_copy = RING_STAGES;
+  auto begin_stream = [&]() {  // of the tile of packed rows that `form` belongs to
+    ring.slab = form.slab_bytes(), copy_shift = 3 - form.width();                 // 4, 2, 1 chunks
+    data = static_cast<const uint8_t*>(p.w.data) + (int64_t)form.base * 16;
+    copies = form.width() == 0 ? 0 : (mine + (1 << copy_shift) - 1) >> copy_shift;
+    next_copy = RING_STAGES;
+    if (lane == 0)
+      for (int c = 0; c < RING_STAGES && c < copies; ++c) issue(c, (ring.stage + c) % RING_STAGES);
+    __syncwarp();
+  };
   auto refill = [&](int stage) {
     if (lane == 0 && next_copy < copies) issue(next_copy, stage);
     ++next_copy;
     __syncwarp();
   };
-  // Shared memory holds eight rows of a block; fewer rows leave room for several blocks, which are prepared together.
-  const int together = FEW_WIDTH / tokens;
-  for (int b0 = 0; b0 < blocks; b0 += together) {
-    const int here = min(together, blocks - b0);
-    // ---- the activations, a warp per block, row and half: up to 32 pieces of 16 columns, one per lane
-    __syncthreads();  // nobody reads the blocks before any more (and the barriers' words are set)
-    for (int u = warp; u < 2 * tokens * here; u += WARPS) {
-      const int second = u & 1, place = u >> 1, b = b0 + place / tokens, r = place % tokens;
-      const int chunks = b == blocks - 1 ? last_chunks : BLOCK_CHUNKS, half0 = b == blocks - 1 ? last_half0 : HALF_CHUNKS;
-      const int piece = (second ? 4 * half0 : 0) + lane;
-      const bool in = piece < 4 * (second ? chunks : half0);
-      int64_t from = tile.begin + r;
-      if (p.tiles.index != nullptr && p.from.kind != FROM_GATED) from = (uint32_t)p.tiles.pair(from) / (uint32_t)p.from.top_k;
-      float v[16];
-      float top = 0.0f;
-      if (in) {
-        stored_basis(p.from, p.w, from, tile.expert, (int64_t)(c0 + b * BLOCK_CHUNKS) * 4 + piece, v);
-        top = largest(v);
-      }
+  if (lane == 0) {
+    for (int s = 0; s < RING_STAGES; ++s) bar_init(&sm.full[warp][s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncwarp();
+  begin_stream();
+  if (threadIdx.x == 0) sm.abort = 0;
+  const int first_word = code_word(g, t);
+
+  chain_wait();  // the activations
+  chain_next();
+  bool ok = true, prepared = false;
+  for (;; ++row_tile) {
+    LaneRows rows;
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const PowerOfTwo power = power_for(top);
-      if (lane == 0) sm.scale[second][place] = power.back;
-      if (in) {
-        uint4 hi[2], lo[2];
-        split16<PARTS>(v, power.to, hi, lo);
-        uint4* dst = reinterpret_cast<uint4*>(xs + place * X_PITCH + piece * 16);
-        dst[0] = hi[0], dst[1] = hi[1];
-        if (PARTS == 2) {
-          dst = reinterpret_cast<uint4*>(xs + (FEW_WIDTH + place) * X_PITCH + piece * 16);
-          dst[0] = lo[0], dst[1] = lo[1];
+    for (int r = 0; r < 4; ++r) {
+      const RowConsts c = consts[r];
+      rows.lo_min[r] = c.lo_min(), rows.lo_scale[r] = c.lo_scale();
+      const __half s = __ushort_as_half((uint16_t)c.step_scale);
+      if (r & 1) rows.step_scale[r / 2] = __halves2half2(__low2half(rows.step_scale[r / 2]), s);
+      else rows.step_scale[r / 2] = __half2half2(s);
+      if (half == 0 && t == 0) sm.out_row[quarter * 32 + 8 * r + g] = c.out_row;
+    }
+    const int pair_unit = (4 >> form.shift()) * g + (t >> form.shift());
+    const bool more = row_tile < last_tile;
+    GroupForm next_form{0, 0};
+    if (more) next_form = load_group(p.w.groups, first_group + (row_tile + 1) * 4);
+    float total[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) total[m][i] = 0.0f;
+    // Shared memory holds 8 or 16 rows of a block; fewer rows leave room for several blocks, which are prepared together,
+    // and once for a run of tiles.
+    const int together = PLACES<PARTS> / tokens;
+    for (int b0 = 0; b0 < blocks; b0 += together) {
+      const int here = min(together, blocks - b0);
+      // ---- the activations, a warp per block, row and half: up to 32 pieces of 16 columns, one per lane
+      if (!prepared) {
+        __syncthreads();  // nobody reads the blocks before any more (and the barriers' words are set)
+        for (int u = warp; u < 2 * tokens * here; u += WARPS) {
+          const int second = u & 1, place = u >> 1, b = b0 + place / tokens, r = place % tokens;
+          const int chunks = b == blocks - 1 ? last_chunks : BLOCK_CHUNKS, half0 = b == blocks - 1 ? last_half0 : HALF_CHUNKS;
+          const int piece = (second ? 4 * half0 : 0) + lane;
+          const bool in = piece < 4 * (second ? chunks : half0);
+          int64_t from = tile.begin + r;
+          if (p.tiles.index != nullptr && p.from.kind != FROM_GATED) from = (uint32_t)p.tiles.pair(from) / (uint32_t)p.from.top_k;
+          float v[16];
+          float top = 0.0f;
+          if (in) {
+            stored_basis(p.from, p.w, from, tile.expert, (int64_t)(c0 + b * BLOCK_CHUNKS) * 4 + piece, v);
+            top = largest(v);
+          }
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          const PowerOfTwo power = power_for(top);
+          if (lane == 0) sm.scale[second][place] = power.back;
+          if (in) {
+            uint4 hi[2], lo[2];
+            split16<PARTS>(v, power.to, hi, lo);
+            uint4* dst = reinterpret_cast<uint4*>(xs + place * X_PITCH + piece * 16);
+            dst[0] = hi[0], dst[1] = hi[1];
+            if (PARTS == 2) {
+              dst = reinterpret_cast<uint4*>(xs + (PLACES<PARTS> + place) * X_PITCH + piece * 16);
+              dst[0] = lo[0], dst[1] = lo[1];
+            }
+          }
+        }
+        __syncthreads();
+      }
+      for (int sub = 0; sub < here; ++sub) {
+        const int chunks = b0 + sub == blocks - 1 ? last_chunks : BLOCK_CHUNKS, half0 = b0 + sub == blocks - 1 ? last_half0 : HALF_CHUNKS;
+        // ---- this warp's chunks of a block; lanes without a row of their own read the last one's
+        float acc[2][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
+        const int first = half == 0 ? 0 : half0, count = half == 0 ? half0 : chunks - half0;
+        if (ok) {  // one loop per code width
+          const __half* x = xs + (sub * tokens + min(g, tokens - 1)) * X_PITCH + first * CHUNK + 16 * t;
+          const auto run = [&](auto nbits, auto small) {
+            return multiply<PARTS, decltype(nbits)::value, decltype(small)::value>(ring, x, count, first_word, pair_unit, rows, acc, &sm.abort,
+                                                                                       status, refill);
+          };
+          typedef std::integral_constant<int, 2> Int2;
+          typedef std::integral_constant<int, 4> Int4;
+          typedef std::integral_constant<int, 8> Int8;
+          if (form.width() == 1) ok = form.small_steps() ? run(Int2(), std::true_type()) : run(Int2(), std::false_type());
+          else if (form.width() == 2) ok = form.small_steps() ? run(Int4(), std::true_type()) : run(Int4(), std::false_type());
+          else if (form.width() == 3) ok = form.small_steps() ? run(Int8(), std::true_type()) : run(Int8(), std::false_type());
+        }
+        const float s0 = sm.scale[half][sub * tokens + min(2 * t, tokens - 1)], s1 = sm.scale[half][sub * tokens + min(2 * t + 1, tokens - 1)];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          total[m][0] += acc[m][0] * s0, total[m][1] += acc[m][1] * s1;
+          total[m][2] += acc[m][2] * s0, total[m][3] += acc[m][3] * s1;
         }
       }
     }
-    __syncthreads();
-    for (int sub = 0; sub < here; ++sub) {
-      const int chunks = b0 + sub == blocks - 1 ? last_chunks : BLOCK_CHUNKS, half0 = b0 + sub == blocks - 1 ? last_half0 : HALF_CHUNKS;
-      // ---- this warp's chunks of a block; lanes without a row of their own read the last one's
-      float acc[2][4];
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
-      const int first = half == 0 ? 0 : half0, count = half == 0 ? half0 : chunks - half0;
-      if (ok) {  // one loop per code width
-        const __half* x = xs + (sub * tokens + min(g, tokens - 1)) * X_PITCH + first * CHUNK + 16 * t;
-        const auto run = [&](auto nbits, auto small) {
-          return multiply<PARTS, decltype(nbits)::value, decltype(small)::value>(ring, x, count, first_word, pair_unit, rows, acc, &sm.abort,
-                                                                                     status, refill);
-        };
-        typedef std::integral_constant<int, 2> Int2;
-        typedef std::integral_constant<int, 4> Int4;
-        typedef std::integral_constant<int, 8> Int8;
-        if (form.width() == 1) ok = form.small_steps() ? run(Int2(), std::true_type()) : run(Int2(), std::false_type());
-        else if (form.width() == 2) ok = form.small_steps() ? run(Int4(), std::true_type()) : run(Int4(), std::false_type());
-        else if (form.width() == 3) ok = form.small_steps() ? run(Int8(), std::true_type()) : run(Int8(), std::false_type());
-      }
-      const float s0 = sm.scale[half][sub * tokens + min(2 * t, tokens - 1)], s1 = sm.scale[half][sub * tokens + min(2 * t + 1, tokens - 1)];
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        total[m][0] += acc[m][0] * s0, total[m][1] += acc[m][1] * s1;
-        total[m][2] += acc[m][2] * s0, total[m][3] += acc[m][3] * s1;
-      }
+    prepared = true;  // all of them: a run of several tiles is only made where they fit
+    if (more && ok) {  // the next tile's data sets out while this one's sums are joined
+      form = next_form;
+      begin_stream();
+      load_rows(row_tile + 1);
     }
-  }
-  if (__syncthreads_or(!ok)) let_copies_land();
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sm.sums[half][2 * t + (i & 1)][quarter * 32 + 16 * m + 8 * (i >> 1) + g] = total[m][i];
-  __syncthreads();
-  if (split > 1) cluster_sync();
-  const uint32_t here = s32(&sm.sums[0][0][0]);
-  for (int i = rank * THREADS + threadIdx.x; i < tokens * TILE_ROWS; i += split * THREADS) {
-    const int token = i / TILE_ROWS, row = i % TILE_ROWS;
-    const uint32_t off = (uint32_t)(token * SUM_PITCH + row) * 4, other = FEW_WIDTH * SUM_PITCH * 4;
-    float v[2 * MAX_SPLIT];
-    if (split > 1) {
+      for (int i = 0; i < 4; ++i) sm.sums[half][2 * t + (i & 1)][quarter * 32 + 16 * m + 8 * (i >> 1) + g] = total[m][i];
+    __syncthreads();
+    if (split > 1) cluster_sync();
+    const uint32_t here = s32(&sm.sums[0][0][0]);
+    for (int i = rank * THREADS + threadIdx.x; i < tokens * TILE_ROWS; i += split * THREADS) {
+      const int token = i / TILE_ROWS, row = i % TILE_ROWS;
+      const uint32_t off = (uint32_t)(token * SUM_PITCH + row) * 4, other = FEW_WIDTH * SUM_PITCH * 4;
+      float v[2 * MAX_SPLIT];
+      if (split > 1) {
+#pragma unroll
+        for (int q = 0; q < MAX_SPLIT; ++q)
+          if (q < split) {
+            const uint32_t there = in_rank(here, q) + off;
+            v[2 * q] = load_cluster(there), v[2 * q + 1] = load_cluster(there + other);
+          }
+      } else {
+        v[0] = sm.sums[0][token][row], v[1] = sm.sums[1][token][row];
+      }
+      float sum = 0.0f;
 #pragma unroll
       for (int q = 0; q < MAX_SPLIT; ++q)
-        if (q < split) {
-          const uint32_t there = in_rank(here, q) + off;
-          v[2 * q] = load_cluster(there), v[2 * q + 1] = load_cluster(there + other);
-        }
-    } else {
-      v[0] = sm.sums[0][token][row], v[1] = sm.sums[1][token][row];
+        if (q < split) sum += v[2 * q] + v[2 * q + 1];
+      const int64_t at = tile.begin + token;
+      if (p.out.pair_weight != nullptr) sum *= p.out.pair_weight[p.tiles.pair(at)];
+      const uint32_t col = sm.out_row[row];
+      if (col != NO_ROW) p.out.put(at, col, sum);
     }
-    float sum = 0.0f;
-#pragma unroll
-    for (int q = 0; q < MAX_SPLIT; ++q)
-      if (q < split) sum += v[2 * q] + v[2 * q + 1];
-    const int64_t at = tile.begin + token;
-    if (p.out.pair_weight != nullptr) sum *= p.out.pair_weight[p.tiles.pair(at)];
-    const uint32_t col = sm.out_row[row];
-    if (col != NO_ROW) p.out.put(at, col, sum);
+    if (split > 1) cluster_sync();  // nobody reads this block's sums any more
+    else __syncthreads();
+    if (!more) break;
   }
-  if (split > 1) cluster_sync();  // nobody reads this block's sums any more
+  if (__syncthreads_or(!ok)) let_copies_land();
 }
 
 template <int PARTS>
-int launch(const Product& p, int split, cudaStream_t stream, const char* what) {
+int launch(const Product& p, int split, int run, cudaStream_t stream, const char* what) {
   const size_t smem = smem_bytes<PARTS>();
   if (!reserve_smem<few_kernel<PARTS>>())
     return fail(HI2_ERR_LAUNCH, "stored product: cannot reserve shared memory");
-  const int64_t blocks = p.w.groups_per_expert / 4 * p.max_tiles * split;
+  const int64_t blocks = ceil_div(p.w.groups_per_expert / 4, (int64_t)run) * p.max_tiles * split;
   if (blocks >= (int64_t)1 << 31) return fail(HI2_ERR_ARG, "stored product: too many tiles");
   cudaLaunchConfig_t config = {};
   config.gridDim = (unsigned)blocks, config.blockDim = THREADS, config.dynamicSmemBytes = smem, config.stream = stream;
@@ -312,24 +341,29 @@ int launch(const Product& p, int split, cudaStream_t stream, const char* what) {
   attribute[1].id = cudaLaunchAttributeClusterDimension;
   attribute[1].val.clusterDim.x = split, attribute[1].val.clusterDim.y = 1, attribute[1].val.clusterDim.z = 1;
   config.attrs = attribute, config.numAttrs = 2;
-  cudaLaunchKernelEx(&config, few_kernel<PARTS>, p, split);
+  cudaLaunchKernelEx(&config, few_kernel<PARTS>, p, split, run);
   return check_launch(what);
 }
 
 }  // namespace
 
 int product_few(const Product& p, cudaStream_t stream, const char* what) {
-  // Slices of the columns: the number that leaves the fullest SM the least work, with what a block costs
-  // besides its chunks (start, activations, the join) counted as twelve of them; each at least four chunks.
-  const int64_t tiles = p.w.groups_per_expert / 4 * p.max_tiles, chunks = p.w.k / CHUNK;
-  const int64_t room = 148 * 2;
-  int split = 1;
+  // Slices of the columns and tiles per block: what leaves the fullest SM the least work, with what a tile costs besides its
+  // chunks (start of its stream, the join) counted as eight of them and what a block costs (start, activations) as twelve.
+  const int64_t row_tiles = p.w.groups_per_expert / 4, chunks = p.w.k / CHUNK, room = 2 * 148;
+  const int64_t width = p.tiles.width < p.tiles.rows ? p.tiles.width : p.tiles.rows;
+  const int places = p.parts == 1 ? PLACES<1> : PLACES<2>;
+  int split = 1, run = 1;
   int64_t least = INT64_MAX;
   for (int s = 1; s <= MAX_SPLIT && (s == 1 || chunks >= 4 * s); ++s) {
-    const int64_t cost = ceil_div(tiles * s, room) * (ceil_div(chunks, (int64_t)s) + 12);
-    if (cost < least) least = cost, split = s;
+    const int64_t slice = ceil_div(chunks, (int64_t)s);
+    const bool fits = width * ceil_div(slice, (int64_t)BLOCK_CHUNKS) <= places;  // activations stay for a run of tiles
+    for (int r = 1; r == 1 || (fits && r <= 16 && r <= row_tiles); ++r) {
+      const int64_t cost = ceil_div(ceil_div(row_tiles, (int64_t)r) * p.max_tiles * s, room) * (r * (slice + 8) + 12);
+      if (cost < least) least = cost, split = s, run = r;
+    }
   }
-  return p.parts == 1 ? launch<1>(p, split, stream, what) : launch<2>(p, split, stream, what);
+  return p.parts == 1 ? launch<1>(p, split, run, stream, what) : launch<2>(p, split, run, stream, what);
 }
 
 }  // namespace stored

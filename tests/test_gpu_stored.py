@@ -63,6 +63,44 @@ def test_epilogue(activation, dtype, tokens):
     _check(t, x, dt, None, activation, residual)
 
 
+@pytest.mark.parametrize("rows,k,tokens,dtype", [(40000, 128, 1, "bf16"), (40000, 192, 5, "f32"), (39000, 64, 8, "f16"), (20000, 1088, 9, "bf16"),
+                                                 (96, 34816, 2, "bf16"), (64, 65536, 8, "f32"), (64, 65536, 8, "bf16"), (130, 16448, 20, "bf16"),
+                                                 (40000, 64, 200, "bf16"), (700, 9024, 16, "f16")])
+def test_many_rows_and_many_columns(rows, k, tokens, dtype):
+    t = packed(rows, k, rows + tokens)
+    _check(t, _x(tokens, k, DTYPES[dtype], 1), DTYPES[dtype])
+
+
+@pytest.mark.parametrize("tokens", [8, 17, 40])
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_epilogue_behind_a_sum_of_slices(tokens, dtype):
+    dt = DTYPES[dtype]
+    t = packed(200, 4224, 13)
+    bias, buf = _x(1, 200, dt, 1)[0], _x(tokens, 210, dt, 2)
+    x = _x(tokens, 4224, dt, 5, 0.3)
+    before = buf.clone()
+    _check(t, x, dt, bias, "silu", buf[:, 3:203], out=buf[:, 3:203])
+    assert torch.equal(buf[:, :3], before[:, :3]) and torch.equal(buf[:, 203:], before[:, 203:])
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0, 5.0, 20.0, 3e3])
+def test_steps_on_both_sides_of_the_short_decoding(scale):
+    """Groups whose steps (times a power of two) are fp16 numbers are decoded by one operation, others by two."""
+    t = packed(400, 192, 17)
+    t.row_consts = (t.row_consts.float() * torch.where(torch.arange(400) % 3 == 0, scale, 1.0)[:, None]).half()
+    for tokens in (2, 50):
+        _check(t, _x(tokens, 192, torch.float32, 3), torch.float32)
+    # every weight of a one-hot product is the stored one, to the bit
+    eye = torch.eye(192, device=DEV)
+    t.had.zero_()
+    t.col_scale = None
+    w = linear.lay_out(t, DEV)
+    v = dequantize_stored(t, DEV, torch.float32)
+    for lo in range(0, 192, 8):
+        assert torch.equal(linear.stored_linear(eye[lo : lo + 8], w), v[:, lo : lo + 8].T)
+    assert torch.equal(linear.stored_linear(eye, w), v.T)
+
+
 def test_agrees_with_the_reference_product():
     t = packed(300, 512, 21)
     x = _x(9, 512, torch.float32, 8)
@@ -165,7 +203,8 @@ def _stacks(experts, hidden, inner, seed, formats=None):
 
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 @pytest.mark.parametrize("experts,top_k,hidden,inner,tokens", [(1, 1, 64, 64, 1), (5, 3, 128, 192, 1), (5, 3, 320, 64, 37),
-                                                               (8, 2, 256, 128, 300), (40, 8, 64, 64, 64), (3, 3, 192, 320, 130)])
+                                                               (8, 2, 256, 128, 300), (40, 8, 64, 64, 64), (3, 3, 192, 320, 130),
+                                                               (24, 2, 1088, 576, 96), (6, 2, 2112, 64, 3)])
 def test_experts_sizes_and_types(experts, top_k, hidden, inner, tokens, dtype):
     dt = DTYPES[dtype]
     gu, dn, gate_up, down = _stacks(experts, hidden, inner, 100 * experts + tokens)
