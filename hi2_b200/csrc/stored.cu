@@ -283,7 +283,7 @@ struct LinearSpace {
     }
     max_tiles = ceil_div(tokens, (int64_t)width);
     if (!few(tokens)) {
-      const int splits = wide_splits(w, Tiles{}, max_tiles);
+      const int splits = wide_splits(w.k, w.rows_per_expert, tokens, max_tiles, false, dtype == HI2_F32);
       if (splits > 1) partial = c.take<float>((size_t)splits * tokens * w.rows_per_expert);
     }
     bytes = c.used;
@@ -292,7 +292,7 @@ struct LinearSpace {
 
 struct ExpertSpace {
   __half* xs = nullptr;  // of the gate/up product, then of the down product
-  float *scale = nullptr, *z, *y;
+  float *scale = nullptr, *partial = nullptr, *z, *y;
   int32_t *pair_of = nullptr, *row_of = nullptr, *next_row = nullptr, *used = nullptr, *tile_count = nullptr;
   TokenTile* tiles = nullptr;
   size_t bytes;
@@ -312,6 +312,10 @@ struct ExpertSpace {
     if (!few_experts(gate_up.experts, pairs)) {
       xs = c.take<__half>(pairs * (hidden > inner ? hidden : inner) * parts_of(dtype));
       scale = c.take<float>(pairs);
+      const bool exact = dtype == HI2_F32;
+      const size_t up = wide_splits(hidden, 2 * inner, pairs, 1, true, exact), dn = wide_splits(inner, hidden, pairs, 1, true, exact);
+      const size_t most = 2 * inner * (up > 1 ? up : 0) > hidden * (dn > 1 ? dn : 0) ? 2 * inner * up : hidden * (dn > 1 ? dn : 0);
+      if (most > 0) partial = c.take<float>(pairs * most);
     }
     bytes = c.used;
   }
@@ -367,7 +371,7 @@ extern "C" int hi2_stored_linear(const hi2_stored_weight* w, const void* x, int 
   const bool small = few(tokens);
   const Product p{*w, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), 1},
                   Tiles{nullptr, nullptr, nullptr, nullptr, tokens, 1, space.width}, space.max_tiles, parts_of(dtype),
-                  Epilogue{nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}, false, space.xs, space.scale, space.partial};
+                  Epilogue{nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}, dtype == HI2_F32, false, space.xs, space.scale, space.partial};
   if (small) return product_few(p, s, "stored_linear");
   const int rc = prepare(p, nullptr, s);
   return rc != HI2_OK ? rc : product_wide(p, s, "stored_linear");
@@ -413,9 +417,9 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
     if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
   }
   const Product up{*gate_up, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), top_k}, tiles, max_tiles, parts,
-                   Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, false, space.xs, space.scale, nullptr};
+                   Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, dtype == HI2_F32, false, space.xs, space.scale, space.partial};
   const Product dn{*down, Source{space.z, 2 * inner, FROM_GATED, act, true, top_k}, tiles, max_tiles, parts,
-                   Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, true, space.xs, space.scale, nullptr};
+                   Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, dtype == HI2_F32, true, space.xs, space.scale, space.partial};
   for (const Product* p : {&up, &dn}) {
     if (small) {
       rc = product_few(*p, s, "stored_experts");

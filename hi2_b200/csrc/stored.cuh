@@ -330,6 +330,7 @@ struct Product {
   int64_t max_tiles;
   int parts;               // fp16 parts of an activation: 2 where the second holds what the first one's rounding lost
   Epilogue out;
+  bool exact;              // fp32 results
   bool settled;            // index and tile list were complete before the kernel ahead of this one set out
   // wide products only: the prepared activations fp16 [parts, rows, k], the powers of two they were divided by, and the
   // sums of the slices fp32 [wide_splits, rows, rows of the tensor] where there are several
@@ -343,7 +344,7 @@ constexpr int FEW_WIDTH = 8;
 int product_few(const Product& p, cudaStream_t stream, const char* what);
 // Wide tiles, from prepared activations.
 int wide_width(int64_t rows);
-int wide_splits(const hi2_stored_weight& w, const Tiles& tiles, int64_t max_tiles);
+int wide_splits(int64_t k, int64_t rows_of_tensor, int64_t rows, int64_t max_tiles, bool stack, bool exact);
 int product_wide(const Product& p, cudaStream_t stream, const char* what);
 
 }  // namespace stored

@@ -97,17 +97,28 @@ __device__ __forceinline__ bool multiply(Ring& ring, const __half* x, int count,
     for (int i = 0; i < here; ++i, x += CHUNK, slab += ring.slab) {
       uint32_t w[4][8];
       decode_rows<NBITS, SMALL>(slab, first_word, pair_unit, rows, w);
+      // With two parts a chunk's sum is formed by itself, small parts first, and added in fp32: the tensor cores' accumulator
+      // drops what does not fit it at every step, which over 512 columns would cost 1e-6 of a result, always towards zero.
+      float sum[2][4];
 #pragma unroll
-      for (int part = 0; part < PARTS; ++part) {
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum[m][q] = PARTS == 1 ? acc[m][q] : 0.0f;
+#pragma unroll
+      for (int part = PARTS - 1; part >= 0; --part) {
         const __half* from = x + part * PLACES<PARTS> * X_PITCH;
         const uint4 x0 = *reinterpret_cast<const uint4*>(from), x1 = *reinterpret_cast<const uint4*>(from + 8);
         const uint32_t k[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          mma(acc[0], w[0][2 * s], w[1][2 * s], w[0][2 * s + 1], w[1][2 * s + 1], k[2 * s], k[2 * s + 1]);
-          mma(acc[1], w[2][2 * s], w[3][2 * s], w[2][2 * s + 1], w[3][2 * s + 1], k[2 * s], k[2 * s + 1]);
+          mma(sum[0], w[0][2 * s], w[1][2 * s], w[0][2 * s + 1], w[1][2 * s + 1], k[2 * s], k[2 * s + 1]);
+          mma(sum[1], w[2][2 * s], w[3][2 * s], w[2][2 * s + 1], w[3][2 * s + 1], k[2 * s], k[2 * s + 1]);
         }
       }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) acc[m][q] = PARTS == 1 ? sum[m][q] : acc[m][q] + sum[m][q];
     }
     count -= here;
     __syncwarp();  // every lane has read the stage

@@ -461,15 +461,16 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
         if (!ok) break;
         fence_after();
         if (elected()) {
-          for (int part = 0; part < p.parts; ++part)
+          uint32_t accumulate = i > 0 ? 1u : 0u;
+          for (int part = p.parts - 1; part >= 0; --part) {  // small parts first
 #pragma unroll
-            for (int kk = 0; kk < CHUNK / 16; ++kk)
-              mma_pair(d, a + kk * 8, b + part * box + kk * 2, idesc, i > 0 || part > 0 || kk > 0 ? 1u : 0u);
-          if (i < second)
-            for (int part = 0; part < p.parts; ++part)
+            for (int kk = 0; kk < CHUNK / 16; ++kk) mma_pair(d, a + kk * 8, b + part * box + kk * 2, idesc, kk > 0 ? 1u : accumulate);
+            accumulate = 1;
+            if (i < second) {
 #pragma unroll
-              for (int kk = 0; kk < CHUNK / 16; ++kk)
-                mma_pair(d, a + A_COLUMNS + kk * 8, b + (p.parts + part) * box + kk * 2, idesc, 1u);
+              for (int kk = 0; kk < CHUNK / 16; ++kk) mma_pair(d, a + A_COLUMNS + kk * 8, b + (p.parts + part) * box + kk * 2, idesc, 1u);
+            }
+          }
           commit_both(&ctl->a_empty[slot]);
           commit_both(&ctl->x_empty[stage]);
           if (i == item.count - 1) commit_both(&ctl->d_full[buf]);
@@ -564,16 +565,23 @@ EncodeFn encoder() {
 
 }  // namespace
 
-// Slices of the columns of one tensor, for tiles that are fewer than the SM pairs: the number that leaves the busiest
-// pair the fewest steps, with start and end of an item counted as six of them; each at least four steps.
-int wide_splits(const hi2_stored_weight& w, const Tiles& tiles, int64_t max_tiles) {
-  if (tiles.index != nullptr) return 1;
-  const int64_t items = (w.groups_per_expert / 4 + 1) / 2 * max_tiles, count = (w.k / CHUNK + 1) / 2;
+// Slices of the columns.  Of one tensor, for tiles that are fewer than the SM pairs: the number that leaves the busiest pair
+// the fewest steps, with start and end of an item counted as six of them; each at least four steps.  For fp32 results
+// (`exact`), as far as 1 GiB of partial sums goes, slices of 128 columns, of 256 with many rows: the tensor cores'
+// accumulator drops what does not fit it at every step, always towards zero, which over 2048 columns costs 2e-6 of a result
+// and over 256 3e-7 (small parts are added first).
+int wide_splits(int64_t k, int64_t rows_of_tensor, int64_t rows, int64_t max_tiles, bool stack, bool exact) {
+  const int64_t items = (ceil_div(rows_of_tensor, (int64_t)TILE_ROWS) + 1) / 2 * max_tiles, count = (k / CHUNK + 1) / 2;
   int best = 1;
   int64_t least = INT64_MAX;
-  for (int s = 1; s <= 16 && (s == 1 || count >= 4 * s); ++s) {
+  for (int s = 1; s <= 16 && (s == 1 || (!stack && count >= 4 * s)); ++s) {
     const int64_t cost = ceil_div(items * s, (int64_t)74) * (ceil_div(count, (int64_t)s) + 6);
     if (cost < least) least = cost, best = s;
+  }
+  if (exact) {
+    const int64_t fit = ((int64_t)1 << 30) / (rows * rows_of_tensor * (int64_t)sizeof(float)), want = rows <= 2048 ? count : (count + 1) / 2;
+    const int64_t s = want < fit ? want : fit;
+    if (s > best) best = (int)(s < 256 ? s : 256);
   }
   return best;
 }
@@ -595,13 +603,14 @@ int product_wide(const Product& p, cudaStream_t stream, const char* what) {
   if (s.slots > MAX_SLOTS) s.slots = MAX_SLOTS;
   s.chunks = (int)(p.w.k / CHUNK), s.half0 = (s.chunks + 1) / 2;
   s.row_pairs = (int)((p.w.groups_per_expert / 4 + 1) / 2);
-  s.splits = wide_splits(p.w, p.tiles, p.max_tiles);
+  s.splits = wide_splits(p.w.k, p.w.rows_per_expert, p.tiles.rows, p.max_tiles, p.tiles.index != nullptr, p.exact);
   size_t smem = (size_t)s.x_stages * stage_bytes + DECODE_WARPS * RING_STAGES * RING_BYTES + sizeof(Control) + 1024;
   // A block takes all of an SM's tensor memory: two must never be resident on one SM.
   if (smem < 120 * 1024) smem = 120 * 1024;
   Product q = p;
   if (s.splits > 1) {  // plain sums of the slices; joined below
     q.out = Epilogue{};
+    q.out.pair_weight = p.out.pair_weight;
     q.out.out = p.partial, q.out.ld_out = p.w.rows_per_expert, q.out.dtype = HI2_F32;
   }
 
