@@ -58,6 +58,24 @@ def output_rows(out, shape, like: torch.Tensor, what: str):
     return rows
 
 
+def apart(what: str, name: str, t, out) -> None:
+    """Refuse an ``out`` whose rows share memory with those of the operand ``t`` (``[tokens, n]`` or ``[n]``, unit column stride)."""
+    size, o_size = t.element_size(), out.element_size()
+    a, o = t.data_ptr(), out.data_ptr()
+    rows = t if t.dim() == 2 else t[None]
+    if not rows.numel() or not out.numel():
+        return
+    step, o_step = rows.stride(0) * size, out.stride(0) * o_size
+    width, o_width = rows.shape[1] * size, out.shape[1] * o_size
+    if a + (rows.shape[0] - 1) * step + width <= o or o + (out.shape[0] - 1) * o_step + o_width <= a:
+        return
+    if rows.shape[0] > 1 and out.shape[0] > 1 and step == o_step:  # columns of one buffer
+        off = (o - a) % step
+        if off >= width and off + o_width <= step:
+            return
+    raise ValueError(f"{what}: out shares memory with {name}")
+
+
 def workspace(need: int, dev: torch.device):
     """``(tensor, address)``: fresh for every call, so that calls on several streams or in several graphs share nothing."""
     if need == 0:

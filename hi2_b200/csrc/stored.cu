@@ -122,9 +122,9 @@ void launch_prepare(const Product& p, const int32_t* used, cudaStream_t stream) 
   if (p.parts == 1) prepare_kernel<THREADS, WARPS, HOLD, 1><<<grid, THREADS, 0, stream>>>(p, used);
   else prepare_kernel<THREADS, WARPS, HOLD, 2><<<grid, THREADS, 0, stream>>>(p, used);
 }
-// Two warps per row where the rows fill the machine (32768 rows of 2048: 65 us; one warp with four pieces per lane 80); else a
-// block per row, one piece per thread
-// as far as that goes (32 rows of 11008 columns: 14 us with 128 threads, which form everything twice).
+// Two warps per row where the rows fill the machine (32768 rows of 2048 columns: 65 us, one warp with four pieces per lane
+// 80); else a block per row, one piece per thread as far as that goes (32 rows of 11008 columns: 14 us with 128
+// threads, which form everything twice).
 int prepare(const Product& p, const int32_t* used, cudaStream_t stream) {
   const int64_t pieces = p.w.k / 16;
   if (pieces <= 128 && p.tiles.rows >= 148 * 16) launch_prepare<64, 2, 2>(p, used, stream);
@@ -218,8 +218,8 @@ place_kernel(const int64_t* __restrict__ index, int64_t pairs, int experts, int3
 
 // out[t] = sum of the token's weighted rows in slot order (a fixed order: the same bits every time).
 __global__ void __launch_bounds__(256)
-combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ row_of, const int64_t* __restrict__ index, int experts, int64_t tokens, int top_k, int64_t hidden,
-               void* __restrict__ out, int dtype, int64_t ld_out) {
+combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ row_of, const int64_t* __restrict__ index,
+               int experts, int64_t tokens, int top_k, int64_t hidden, void* __restrict__ out, int dtype, int64_t ld_out) {
   chain_wait();
   const int64_t quads = hidden / 4, total = tokens * quads;
   for (int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; id < total; id += (int64_t)gridDim.x * blockDim.x) {
@@ -254,16 +254,27 @@ struct Carver {
   }
 };
 
-// Which kernel takes a product.
-inline bool few(int64_t tokens) { return tokens <= 2 * FEW_WIDTH; }
+inline int parts_of(int dtype) { return dtype == HI2_BF16 ? 1 : 2; }
+// Which kernel takes a product: the one for few rows up to 16 of them, and as long as its tiles of eight are little work (it
+// is one launch where the other takes three).  Measured, few / wide, us (and cost): 256 tokens x 512 x 512 8.7 / 15.4
+// (24), 77 x 1001 x 1088 in fp32 11.8 / 16.9 (26), 64 x 2048 x 2048 12.8 / 17.4 (36), 24 x 4096 x 4096 19.5 / 19.0 (42),
+// 64 x 4096 x 4096 34 / 22 (84); 111 pairs of 5 experts of 192 x 320 in fp32 25.1 / 32.8 (25).
+constexpr int64_t FEW_COST = 40;
+inline bool few(const hi2_stored_weight& w, int64_t tokens, int parts) {
+  return tokens <= 2 * FEW_WIDTH || few_plan(w.k, w.groups_per_expert / 4, ceil_div(tokens, (int64_t)FEW_WIDTH), FEW_WIDTH, parts).cost <= FEW_COST;
+}
 inline int64_t rows_per_expert(int64_t experts, int64_t pairs) {  // with half as many again as on average
   const int64_t busy = ceil_div(3 * pairs, 2 * experts);
   return busy < pairs ? busy : pairs;
 }
-inline bool few_experts(int64_t experts, int64_t pairs) { return rows_per_expert(experts, pairs) <= 2 * FEW_WIDTH; }
+inline bool few_experts(const hi2_stored_weight& gate_up, int64_t pairs, int parts) {  // both products, or neither
+  if (rows_per_expert(gate_up.experts, pairs) <= 2 * FEW_WIDTH) return true;
+  const int64_t tiles = pairs / FEW_WIDTH + gate_up.experts, hidden = gate_up.k, inner = gate_up.rows_per_expert / 2;
+  return few_plan(hidden, ceil_div(2 * inner, (int64_t)TILE_ROWS), tiles, FEW_WIDTH, parts).cost <= FEW_COST &&
+         few_plan(inner, ceil_div(hidden, (int64_t)TILE_ROWS), tiles, FEW_WIDTH, parts).cost <= FEW_COST;
+}
 inline bool apart(int64_t pairs) { return pairs <= FEW_WIDTH; }  // every pair a tile of its own
 
-inline int parts_of(int dtype) { return dtype == HI2_BF16 ? 1 : 2; }
 inline int64_t size_of(int dtype) { return dtype == HI2_F32 ? 4 : 2; }
 inline bool rows_aligned(const void* p, int64_t ld, int dtype) { return aligned16(p) && ld * size_of(dtype) % 16 == 0; }
 inline int kind_of(int dtype) { return dtype == HI2_BF16 ? FROM_BF16 : dtype == HI2_F16 ? FROM_F16 : FROM_F32; }
@@ -273,16 +284,17 @@ struct LinearSpace {
   float *scale = nullptr, *partial = nullptr;
   int width = FEW_WIDTH;
   int64_t max_tiles;
+  bool small;
   size_t bytes;
-  LinearSpace(void* ws, const hi2_stored_weight& w, int dtype, int64_t tokens) {
+  LinearSpace(void* ws, const hi2_stored_weight& w, int dtype, int64_t tokens) : small(few(w, tokens, parts_of(dtype))) {
     Carver c{static_cast<uint8_t*>(ws)};
-    if (!few(tokens)) {
+    if (!small) {
       xs = c.take<__half>((size_t)tokens * w.k * parts_of(dtype));
       scale = c.take<float>(tokens);
       width = wide_width(tokens);
     }
     max_tiles = ceil_div(tokens, (int64_t)width);
-    if (!few(tokens)) {
+    if (!small) {
       const int splits = wide_splits(w.k, w.rows_per_expert, tokens, max_tiles, false, dtype == HI2_F32);
       if (splits > 1) partial = c.take<float>((size_t)splits * tokens * w.rows_per_expert);
     }
@@ -295,8 +307,10 @@ struct ExpertSpace {
   float *scale = nullptr, *partial = nullptr, *z, *y;
   int32_t *pair_of = nullptr, *row_of = nullptr, *next_row = nullptr, *used = nullptr, *tile_count = nullptr;
   TokenTile* tiles = nullptr;
+  bool small;
   size_t bytes;
-  ExpertSpace(void* ws, const hi2_stored_weight& gate_up, int dtype, int64_t tokens, int top_k) {
+  ExpertSpace(void* ws, const hi2_stored_weight& gate_up, int dtype, int64_t tokens, int top_k)
+      : small(few_experts(gate_up, tokens * top_k, parts_of(dtype))) {
     const size_t pairs = (size_t)tokens * top_k, hidden = gate_up.k, inner = gate_up.rows_per_expert / 2;
     Carver c{static_cast<uint8_t*>(ws)};
     z = c.take<float>(pairs * inner * 2);
@@ -309,7 +323,7 @@ struct ExpertSpace {
       next_row = c.take<int32_t>(gate_up.experts);
       tiles = c.take<TokenTile>(pairs / 8 + gate_up.experts + 1);
     }
-    if (!few_experts(gate_up.experts, pairs)) {
+    if (!small) {
       xs = c.take<__half>(pairs * (hidden > inner ? hidden : inner) * parts_of(dtype));
       scale = c.take<float>(pairs);
       const bool exact = dtype == HI2_F32;
@@ -329,7 +343,6 @@ bool complete(const hi2_stored_weight* w) {
 bool known_dtype(int dtype) { return dtype == HI2_F32 || dtype == HI2_F16 || dtype == HI2_BF16; }
 
 }  // namespace
-
 }  // namespace stored
 }  // namespace hi2
 
@@ -368,11 +381,11 @@ extern "C" int hi2_stored_linear(const hi2_stored_weight* w, const void* x, int 
   if (space.bytes > 0 && (workspace == nullptr || workspace_bytes < space.bytes || !aligned16(workspace)))
     return fail(HI2_ERR_WORKSPACE, "stored_linear: workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool small = few(tokens);
   const Product p{*w, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), 1},
                   Tiles{nullptr, nullptr, nullptr, nullptr, tokens, 1, space.width}, space.max_tiles, parts_of(dtype),
-                  Epilogue{nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}, dtype == HI2_F32, false, space.xs, space.scale, space.partial};
-  if (small) return product_few(p, s, "stored_linear");
+                  Epilogue{nullptr, bias, residual, out, ld_residual, ld_out, act, dtype}, dtype == HI2_F32, false, space.xs, space.scale,
+                  space.partial};
+  if (space.small) return product_few(p, s, "stored_linear");
   const int rc = prepare(p, nullptr, s);
   return rc != HI2_OK ? rc : product_wide(p, s, "stored_linear");
 }
@@ -402,13 +415,12 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t pairs = tokens * top_k, hidden = gate_up->k, inner = down->k;
   const int experts = (int)gate_up->experts, parts = parts_of(dtype);
-  const bool small = few_experts(experts, pairs);
   Tiles tiles{index, nullptr, nullptr, nullptr, pairs, experts, 1};
   int64_t max_tiles = pairs;
   int rc;
   if (!apart(pairs)) {
     const int64_t busy = rows_per_expert(experts, pairs);
-    tiles = Tiles{index, space.pair_of, space.tile_count, space.tiles, pairs, experts, small ? FEW_WIDTH : wide_width(busy)};
+    tiles = Tiles{index, space.pair_of, space.tile_count, space.tiles, pairs, experts, space.small ? FEW_WIDTH : wide_width(busy)};
     max_tiles = pairs / tiles.width + experts + 1;
     count_kernel<<<1, SORT_THREADS, 0, s>>>(index, pairs, experts, tiles.width, space.next_row, space.used, space.tile_count, space.tiles);
     if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
@@ -417,11 +429,13 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
     if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
   }
   const Product up{*gate_up, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), top_k}, tiles, max_tiles, parts,
-                   Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, dtype == HI2_F32, false, space.xs, space.scale, space.partial};
+                   Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, dtype == HI2_F32, false, space.xs,
+                   space.scale, space.partial};
   const Product dn{*down, Source{space.z, 2 * inner, FROM_GATED, act, true, top_k}, tiles, max_tiles, parts,
-                   Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, dtype == HI2_F32, true, space.xs, space.scale, space.partial};
+                   Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, dtype == HI2_F32, true, space.xs,
+                   space.scale, space.partial};
   for (const Product* p : {&up, &dn}) {
-    if (small) {
+    if (space.small) {
       rc = product_few(*p, s, "stored_experts");
     } else {
       rc = prepare(*p, space.used, s);
@@ -431,6 +445,7 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   }
   int64_t blocks = ceil_div(tokens * (hidden / 4), (int64_t)256);
   if (blocks > 148 * 16) blocks = 148 * 16;
-  launch_link(combine_kernel, dim3((unsigned)blocks), dim3(256), 0, s, space.y, space.row_of, index, experts, tokens, top_k, hidden, out, dtype, ld_out);
+  launch_link(combine_kernel, dim3((unsigned)blocks), dim3(256), 0, s, space.y, space.row_of, index, experts, tokens, top_k, hidden,
+              out, dtype, ld_out);
   return check_launch("stored_experts: combine");
 }

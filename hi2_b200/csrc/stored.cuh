@@ -70,8 +70,8 @@ struct Ladder {
 // rounding.
 // Any step: 1024 + code * 2^AT is an fp16 number with the code in its mantissa; a fused multiply-add takes
 // it to the code (exact), a second one forms the weight.  fp16 arithmetic issues every other clock and shares its pipe
-// with the warp-level products: 2048 INT2 weights and their products take a scheduler 172 clocks with small
-// steps (52 fp16 instructions and 8 products), 216 without (70 and 8).
+// with the warp-level products: 2048 INT2 weights and their products, out of registers, take a scheduler 183 clocks with small
+// steps and 216 without; 2048 INT4 weights with small steps 190, INT8 201.
 template <int AT, int NBITS, bool SMALL>
 __device__ __forceinline__ uint32_t weight_pair(uint32_t w, __half2 lo, __half2 step) {
   constexpr uint32_t mask = ((1u << NBITS) - 1u) << AT;
@@ -312,13 +312,6 @@ struct Tiles {
     out = TokenTile{(int)e, (int)b, (int)(b + width < rows ? b + width : rows)};
     return true;
   }
-  // With a list, or of one tensor: how many there are, and one of them.
-  __device__ __forceinline__ int64_t number() const { return count != nullptr ? *count : (rows + width - 1) / width; }
-  __device__ __forceinline__ TokenTile at(int64_t t) const {
-    if (count != nullptr) return list[t];
-    const int64_t b = t * width;
-    return TokenTile{0, (int)b, (int)(b + width < rows ? b + width : rows)};
-  }
   __device__ __forceinline__ int64_t pair(int64_t row) const { return pair_of == nullptr ? row : pair_of[row]; }
 };
 
@@ -341,6 +334,11 @@ struct Product {
 
 // Products with up to 8 activation rows per tile, which prepare their activations themselves.
 constexpr int FEW_WIDTH = 8;
+struct FewPlan {
+  int split, run;  // slices of the columns; tiles of packed rows per block
+  int64_t cost;    // of the fullest SM, in chunks
+};
+FewPlan few_plan(int64_t k, int64_t row_tiles, int64_t tiles, int64_t width, int parts);
 int product_few(const Product& p, cudaStream_t stream, const char* what);
 // Wide tiles, from prepared activations.
 int wide_width(int64_t rows);

@@ -33,8 +33,7 @@ __device__ __forceinline__ void bar_expect(unsigned long long* b, uint32_t bytes
 __device__ __forceinline__ void bar_arrive(unsigned long long* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(b)) : "memory");
 }
-// Sleeps up to 20 us for the phase.  (With the default limit waiting warps came back so often that a third of all
-// instructions of a wide product were their polls.)
+// Sleeps up to 20 us for the phase.
 __device__ __forceinline__ bool bar_try(unsigned long long* b, uint32_t parity) {
   uint32_t ok;
   asm volatile(

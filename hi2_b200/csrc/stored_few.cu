@@ -358,23 +358,27 @@ int launch(const Product& p, int split, int run, cudaStream_t stream, const char
 
 }  // namespace
 
-int product_few(const Product& p, cudaStream_t stream, const char* what) {
-  // Slices of the columns and tiles per block: what leaves the fullest SM the least work, with what a tile costs besides its
-  // chunks (start of its stream, the join) counted as eight of them and what a block costs (start, activations) as twelve.
-  const int64_t row_tiles = p.w.groups_per_expert / 4, chunks = p.w.k / CHUNK, room = 2 * 148;
-  const int64_t width = p.tiles.width < p.tiles.rows ? p.tiles.width : p.tiles.rows;
-  const int places = p.parts == 1 ? PLACES<1> : PLACES<2>;
-  int split = 1, run = 1;
-  int64_t least = INT64_MAX;
+// Slices of the columns and tiles per block: what leaves the fullest SM the least work, with what a tile costs besides its
+// chunks (start of its stream, the join) counted as eight of them and what a block costs (start, activations) as twelve.
+FewPlan few_plan(int64_t k, int64_t row_tiles, int64_t tiles, int64_t width, int parts) {
+  const int64_t chunks = k / CHUNK, room = 2 * 148;
+  const int places = parts == 1 ? PLACES<1> : PLACES<2>;
+  FewPlan plan{1, 1, INT64_MAX};
   for (int s = 1; s <= MAX_SPLIT && (s == 1 || chunks >= 4 * s); ++s) {
     const int64_t slice = ceil_div(chunks, (int64_t)s);
     const bool fits = width * ceil_div(slice, (int64_t)BLOCK_CHUNKS) <= places;  // activations stay for a run of tiles
     for (int r = 1; r == 1 || (fits && r <= 16 && r <= row_tiles); ++r) {
-      const int64_t cost = ceil_div(ceil_div(row_tiles, (int64_t)r) * p.max_tiles * s, room) * (r * (slice + 8) + 12);
-      if (cost < least) least = cost, split = s, run = r;
+      const int64_t cost = ceil_div(ceil_div(row_tiles, (int64_t)r) * tiles * s, room) * (r * (slice + 8) + 12);
+      if (cost < plan.cost) plan = FewPlan{s, r, cost};
     }
   }
-  return p.parts == 1 ? launch<1>(p, split, run, stream, what) : launch<2>(p, split, run, stream, what);
+  return plan;
+}
+
+int product_few(const Product& p, cudaStream_t stream, const char* what) {
+  const int64_t width = p.tiles.width < p.tiles.rows ? p.tiles.width : p.tiles.rows;
+  const FewPlan plan = few_plan(p.w.k, p.w.groups_per_expert / 4, p.max_tiles, width, p.parts);
+  return p.parts == 1 ? launch<1>(p, plan.split, plan.run, stream, what) : launch<2>(p, plan.split, plan.run, stream, what);
 }
 
 }  // namespace stored

@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t cta_rank() {
   return r;
 }
 // What these arrivals order is tensor memory, which the fences before and after them do.  A release at cluster
-// scope would wait for everything else the thread has in flight: 1200 clocks where this takes 250.
+// scope would wait for everything else the thread has in flight: from a step to its products 1200 clocks, so 190.
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }

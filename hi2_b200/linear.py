@@ -16,12 +16,12 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._args import ACTIVATIONS, activation_number, no_gradient, on_device, output_rows, rows_of, workspace
+from ._args import ACTIVATIONS, activation_number, apart, no_gradient, on_device, output_rows, rows_of, workspace
 from .format import GROUP, HI2Tensor
 from .stack import MARK, stack_dims
 
 CHUNK = 64  # columns that a row's codes are dealt out by
-FEW_TOKENS = 16  # up to here a product needs no workspace
+FEW_TOKENS = 16  # up to here a product never needs a workspace
 _GROUP_ROWS, _TILE_GROUPS = 32, 4
 
 
@@ -180,7 +180,7 @@ def stored_linear(x: torch.Tensor, w: StoredWeight, bias: torch.Tensor | None = 
     """``activation(x @ W^T + bias) + residual`` with the packed weight ``w`` (``[rows, K]``), as ``[..., rows]`` in
     the dtype of ``x [..., K]`` (bf16, fp16 or fp32, any strides).  ``activation`` is None, ``"relu"``, ``"silu"``,
     ``"gelu"`` or ``"gelu_tanh"``; ``bias [rows]`` and ``residual [..., rows]`` have the dtype of ``x``.
-    ``out`` may be given, and may be ``residual`` itself.  Queued on the current stream of the weight's device; a token with a
+    ``out`` may be given, and may be ``residual`` itself, but share no memory with the other operands.  Queued on the current stream of the weight's device; a token with a
     non-finite activation gets non-finite sums and leaves the others alone."""
     if len(w.shape) != 2:
         raise ValueError("stored_linear: a stack of experts goes through moe.stored_experts")
@@ -195,7 +195,7 @@ def stored_linear(x: torch.Tensor, w: StoredWeight, bias: torch.Tensor | None = 
         if bias.shape != (n,) or bias.dtype != x.dtype:
             raise ValueError(f"stored_linear: bias must have shape {(n,)} and dtype {x.dtype}")
         bias = bias.contiguous()
-    res_ptr, ld_res = None, 0
+    res, res_ptr, ld_res = None, None, 0
     if residual is not None:
         if residual.shape != shape or residual.dtype != x.dtype:
             raise ValueError(f"stored_linear: residual must have shape {shape} and dtype {x.dtype}")
@@ -208,6 +208,11 @@ def stored_linear(x: torch.Tensor, w: StoredWeight, bias: torch.Tensor | None = 
     else:
         y = output_rows(out, shape, x, "stored_linear")
         ld_out = y.stride(0)
+        apart("stored_linear", "x", rows, y)
+        if bias is not None:
+            apart("stored_linear", "bias", bias, y)
+        if res is not None and (res_ptr != y.data_ptr() or (ld_res != ld_out and tokens > 1)):
+            apart("stored_linear", "residual", res, y)
     if tokens == 0:
         return out
     need = 0

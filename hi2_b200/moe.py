@@ -17,7 +17,7 @@ import torch
 from torch import nn
 
 from . import _lib
-from ._args import DTYPES, activation_number, no_gradient, on_device, output_rows, rows_of, workspace
+from ._args import DTYPES, activation_number, apart, no_gradient, on_device, output_rows, rows_of, workspace
 from .hessian import HessianStats
 from .stats import ColumnStats
 
@@ -263,7 +263,8 @@ def stored_experts(x: torch.Tensor, index: torch.Tensor, weight: torch.Tensor, g
     dtype of ``x [..., hidden]`` (bf16, fp16 or fp32): the call of :class:`ExpertViews` over stacks of packed
     weights (``gate_up``, ``down``: :func:`hi2_b200.linear.lay_out_stack` with 2 and 1 parts).  ``index`` and ``weight`` are
     ``[..., top_k]`` as :func:`route` gives them; a slot whose index is not an expert's (-1) adds nothing.  The
-    slots of a token are added in their order: equal inputs give equal bits.  Queued on the current stream; nothing
+    slots of a token are added in their order: equal inputs give equal bits.  ``out`` may be given, and may be ``x``
+    itself.  Queued on the current stream; nothing
     is read back."""
     if len(gate_up.shape) != 3 or len(down.shape) != 3 or gate_up.experts != down.experts or gate_up.k != down.rows or (
             gate_up.rows != 2 * down.k):
@@ -279,15 +280,20 @@ def stored_experts(x: torch.Tensor, index: torch.Tensor, weight: torch.Tensor, g
     if index.dtype not in (torch.int64, torch.int32) or weight.dtype not in DTYPES:
         raise ValueError("stored_experts: index must hold integers, weight fp32, fp16 or bf16")
     no_gradient("stored_experts", x, weight, out)
+    y = None
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=dev)
         ld_out = down.rows
     else:
-        ld_out = output_rows(out, x.shape, x, "stored_experts").stride(0)
+        y = output_rows(out, x.shape, x, "stored_experts")
+        ld_out = y.stride(0)
     tokens, top_k = rows.shape[0], index.shape[-1]
     if tokens == 0:
         return out
     index, weight = index.to(torch.int64).contiguous(), weight.to(torch.float32).contiguous()
+    if y is not None:
+        for name, t in (("index", index), ("weight", weight)):
+            apart("stored_experts", name, t.view(tokens, top_k), y)
     need = _lib.load().hi2_stored_experts_workspace_bytes(gate_up.arg, dtype, tokens, top_k)
     space, at = workspace(need, dev)
     _lib.launch("hi2_stored_experts", dev.index, gate_up.arg, down.arg, rows.data_ptr(), dtype, tokens, rows.stride(0), index.data_ptr(),

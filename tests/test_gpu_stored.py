@@ -1,15 +1,18 @@
 """Products with packed weights and the routed experts over stacks of them, against the 64-bit
 reconstruction (``format.dequantize_stored``) and elementwise bounds from the number formats."""
 
+import threading
+
 import pytest
 import torch
 
-from hi2_b200 import linear, moe, stack
+from hi2_b200 import _lib, linear, moe, stack
 from hi2_b200.format import dequantize_stored, reference_linear
 from tests.stored_helpers import DTYPES, FORMATS, experts64, linear64, packed, within
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+NUMBER = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
 def _gen(seed):
@@ -24,6 +27,8 @@ def _x(tokens, k, dtype, seed, spread=1.0):
 
 def _check(t, x, dtype, bias=None, activation=None, residual=None, out=None):
     w = linear.lay_out(t, DEV)
+    if x.numel() // x.shape[-1] > 1000:  # sizes that are meant for the wide tiles
+        assert _lib.load().hi2_stored_linear_workspace_bytes(w.arg, NUMBER[dtype], x.numel() // x.shape[-1]) > 0
     keep = None if residual is None else residual.clone()
     y = linear.stored_linear(x, w, bias=bias, activation=activation, residual=residual, out=out)
     flat = x.reshape(-1, x.shape[-1])
@@ -37,7 +42,10 @@ def _check(t, x, dtype, bias=None, activation=None, residual=None, out=None):
 
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 @pytest.mark.parametrize("rows,k,tokens", [(1, 64, 1), (33, 64, 2), (128, 128, 1), (129, 192, 7), (257, 1088, 16),
-                                           (500, 320, 17), (640, 2048, 33), (96, 4160, 70), (1000, 576, 129), (300, 64, 300)])
+                                           (500, 320, 17), (640, 2048, 33), (96, 4160, 70), (1000, 576, 129), (300, 64, 300),
+                                           (1, 64, 2501), (33, 64, 2600), (129, 192, 2501), (257, 1088, 701), (257, 1088, 1101),
+                                           (500, 320, 2400),
+                                           (640, 2048, 333), (96, 4160, 600), (1000, 576, 1300), (300, 64, 5003)])
 def test_linear_sizes_and_types(rows, k, tokens, dtype):
     t = packed(rows, k, rows + k)
     _check(t, _x(tokens, k, DTYPES[dtype], tokens), DTYPES[dtype])
@@ -48,11 +56,12 @@ def test_every_row_format_alone(form):
     t = packed(160, 256, 7, [form])
     _check(t, _x(5, 256, torch.float32, 3), torch.float32)
     _check(t, _x(40, 256, torch.bfloat16, 4), torch.bfloat16)
+    _check(t, _x(2501, 256, torch.float32, 5), torch.float32)
 
 
 @pytest.mark.parametrize("activation", [None, "relu", "silu", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
-@pytest.mark.parametrize("tokens", [1, 50])
+@pytest.mark.parametrize("tokens", [1, 50, 1500])
 def test_epilogue(activation, dtype, tokens):
     dt = DTYPES[dtype]
     t = packed(200, 320, 11)
@@ -71,7 +80,7 @@ def test_many_rows_and_many_columns(rows, k, tokens, dtype):
     _check(t, _x(tokens, k, DTYPES[dtype], 1), DTYPES[dtype])
 
 
-@pytest.mark.parametrize("tokens", [8, 17, 40])
+@pytest.mark.parametrize("tokens", [8, 17, 40, 400])
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 def test_epilogue_behind_a_sum_of_slices(tokens, dtype):
     dt = DTYPES[dtype]
@@ -88,7 +97,7 @@ def test_steps_on_both_sides_of_the_short_decoding(scale):
     """Groups whose steps (times a power of two) are fp16 numbers are decoded by one operation, others by two."""
     t = packed(400, 192, 17)
     t.row_consts = (t.row_consts.float() * torch.where(torch.arange(400) % 3 == 0, scale, 1.0)[:, None]).half()
-    for tokens in (2, 50):
+    for tokens in (2, 50, 1500):
         _check(t, _x(tokens, 192, torch.float32, 3), torch.float32)
     # every weight of a one-hot product is the stored one, to the bit
     eye = torch.eye(192, device=DEV)
@@ -99,11 +108,13 @@ def test_steps_on_both_sides_of_the_short_decoding(scale):
     for lo in range(0, 192, 8):
         assert torch.equal(linear.stored_linear(eye[lo : lo + 8], w), v[:, lo : lo + 8].T)
     assert torch.equal(linear.stored_linear(eye, w), v.T)
+    assert torch.equal(linear.stored_linear(eye.repeat(14, 1), w), v.T.repeat(14, 1))
 
 
-def test_agrees_with_the_reference_product():
+@pytest.mark.parametrize("tokens", [9, 1501])
+def test_agrees_with_the_reference_product(tokens):
     t = packed(300, 512, 21)
-    x = _x(9, 512, torch.float32, 8)
+    x = _x(tokens, 512, torch.float32, 8)
     y = linear.stored_linear(x, linear.lay_out(t, DEV))
     want = reference_linear(x, t)
     assert (y.double() - want).norm() / want.norm() < 2e-6
@@ -112,11 +123,11 @@ def test_agrees_with_the_reference_product():
 @pytest.mark.parametrize("scaled,flags", [(False, 0.0), (False, 1.0), (True, 0.0)])
 def test_without_smoothing_or_rotation(scaled, flags):
     t = packed(130, 192, 5, scaled=scaled, flags=flags)
-    for tokens in (3, 65):
+    for tokens in (3, 65, 2501):
         _check(t, _x(tokens, 192, torch.float16, tokens), torch.float16)
 
 
-@pytest.mark.parametrize("tokens", [4, 66])
+@pytest.mark.parametrize("tokens", [4, 66, 1501])
 def test_strides_offsets_and_out(tokens):
     dt = torch.bfloat16
     t = packed(190, 256, 31)
@@ -136,11 +147,12 @@ def test_strides_offsets_and_out(tokens):
     _check(t, wide[:tokens, :256], dt, bias=bias)
 
 
-def test_range_of_the_activations():
+@pytest.mark.parametrize("tokens", [20, 2501])
+def test_range_of_the_activations(tokens):
     t = packed(140, 128, 3)
     for dt, sizes in ((torch.bfloat16, (1e30, 1e-30, 1e-36)), (torch.float32, (1e30, 1e-28)), (torch.float16, (6e4, 1e-6))):
         for size in sizes:
-            x = _x(20, 128, torch.float32, 2, 0.0).clamp(-1, 1)
+            x = _x(tokens, 128, torch.float32, 2, 0.0).clamp(-1, 1)
             if dt == torch.float16 and size > 1:
                 t1 = packed(140, 128, 3, scaled=False, flags=0.0)
                 y = linear.stored_linear((x * size / 128).to(dt), linear.lay_out(t1, DEV))
@@ -153,7 +165,7 @@ def test_range_of_the_activations():
     assert not linear.stored_linear(torch.zeros(3, 128, dtype=torch.bfloat16, device=DEV), w).any()
 
 
-@pytest.mark.parametrize("tokens", [5, 130])
+@pytest.mark.parametrize("tokens", [5, 130, 1501])
 def test_non_finite_activations_stay_in_their_row(tokens):
     t = packed(150, 192, 41)
     x = _x(tokens, 192, torch.bfloat16, 6)
@@ -175,10 +187,11 @@ def test_no_tokens_and_one_row():
     assert y.shape == (70,)
 
 
-def test_equal_inputs_give_equal_bits():
+@pytest.mark.parametrize("tokens", [16, 200, 1500])
+def test_equal_inputs_give_equal_bits(tokens):
     t = packed(260, 640, 51)
     w = linear.lay_out(t, DEV)
-    x = _x(200, 640, torch.bfloat16, 7)
+    x = _x(tokens, 640, torch.bfloat16, 7)
     whole = linear.stored_linear(x, w)
     again = linear.stored_linear(x, w)
     assert torch.equal(whole, again)
@@ -204,7 +217,9 @@ def _stacks(experts, hidden, inner, seed, formats=None):
 @pytest.mark.parametrize("dtype", sorted(DTYPES))
 @pytest.mark.parametrize("experts,top_k,hidden,inner,tokens", [(1, 1, 64, 64, 1), (5, 3, 128, 192, 1), (5, 3, 320, 64, 37),
                                                                (8, 2, 256, 128, 300), (40, 8, 64, 64, 64), (3, 3, 192, 320, 130),
-                                                               (24, 2, 1088, 576, 96), (6, 2, 2112, 64, 3)])
+                                                               (24, 2, 1088, 576, 96), (6, 2, 2112, 64, 3),
+                                                               (1, 1, 64, 64, 2501), (5, 3, 320, 64, 900), (8, 2, 256, 128, 1501),
+                                                               (40, 8, 64, 64, 1024), (3, 3, 192, 320, 1300), (24, 2, 1088, 576, 400)])
 def test_experts_sizes_and_types(experts, top_k, hidden, inner, tokens, dtype):
     dt = DTYPES[dtype]
     gu, dn, gate_up, down = _stacks(experts, hidden, inner, 100 * experts + tokens)
@@ -222,15 +237,16 @@ def test_experts_sizes_and_types(experts, top_k, hidden, inner, tokens, dtype):
     gu.check(), dn.check()
 
 
-def test_experts_extremes():
+@pytest.mark.parametrize("n", [90, 1700])
+def test_experts_extremes(n):
     gu, dn, gate_up, down = _stacks(4, 128, 64, 900)
-    x = _x(90, 128, torch.float32, 4, 0.5)
-    index = torch.full((90, 2), 2, device=DEV)  # one expert for everybody, twice
-    weight = torch.rand(90, 2, generator=_gen(1), device=DEV)
+    x = _x(n, 128, torch.float32, 4, 0.5)
+    index = torch.full((n, 2), 2, device=DEV)  # one expert for everybody, twice
+    weight = torch.rand(n, 2, generator=_gen(1), device=DEV)
     want, bound = experts64(x, index, weight, gate_up, down, torch.float32)
     within(moe.stored_experts(x, index, weight, gu, dn), want, bound)
     # indices that no expert has, of either sign, and int32
-    far = torch.full((90, 2), 4, device=DEV, dtype=torch.int32)
+    far = torch.full((n, 2), 4, device=DEV, dtype=torch.int32)
     far[::2] = -7
     assert not moe.stored_experts(x, far, weight, gu, dn).any()
     far[3, 1] = 1
@@ -240,12 +256,16 @@ def test_experts_extremes():
     assert not y[4:].any() and y[3].any()
     assert moe.stored_experts(x[:0], index[:0], weight[:0], gu, dn).shape == (0, 128)
     # strided activations and a given output; other activations
-    wide = _x(90, 300, torch.bfloat16, 5, 0.5)
-    buf = torch.ones(90, 200, dtype=torch.bfloat16, device=DEV)
+    wide = _x(n, 300, torch.bfloat16, 5, 0.5)
+    buf = torch.ones(n, 200, dtype=torch.bfloat16, device=DEV)
     y = moe.stored_experts(wide[:, 3:131], index, weight.bfloat16(), gu, dn, activation="gelu", out=buf[:, 7:135])
     want, bound = experts64(wide[:, 3:131], index, weight.bfloat16().float(), gate_up, down, torch.bfloat16, "gelu")
     within(y, want, bound)
     assert bool((buf[:, :7] == 1).all()) and bool((buf[:, 135:] == 1).all())
+    # in place of the activations
+    y = moe.stored_experts(x, index, weight, gu, dn)
+    same = x.clone()
+    assert torch.equal(moe.stored_experts(same, index, weight, gu, dn, out=same), y) and torch.equal(same, y)
 
 
 def test_mixture_layer_one_token_and_a_batch():
@@ -258,7 +278,7 @@ def test_mixture_layer_one_token_and_a_batch():
     router = torch.randn(experts, hidden, generator=_gen(3), device=DEV) * 0.1
     module = moe.StoredExperts(gu, dn)
     assert len(module) == experts
-    for tokens in (1, 48):
+    for tokens in (1, 48, 1500):
         a, stream = _x(tokens, 320, torch.float32, 1, 0.5), _x(tokens, hidden, torch.float32, 2, 0.2)
         h = linear.stored_linear(a, proj, residual=stream)
         index, weight = moe.route(h @ router.T, top_k, scores="sigmoid", bias=torch.zeros(experts, device=DEV), groups=4,
@@ -275,7 +295,7 @@ def test_captured_graphs_and_side_streams():
     """Two graphs of the same weights, replayed beside each other and beside eager calls."""
     gu, dn, _, _ = _stacks(6, 128, 64, 700)
     w = linear.lay_out(packed(128, 128, 70), DEV)
-    xs = [_x(n, 128, torch.bfloat16, n) for n in (1, 40)]
+    xs = [_x(n, 128, torch.bfloat16, n) for n in (1, 40, 2501)]
 
     def step(x):
         index, weight = moe.route(x[:, :6].contiguous(), 2)
@@ -306,6 +326,53 @@ def test_captured_graphs_and_side_streams():
         x.copy_(x.flip(0) * 0.5)
         g.replay()
         assert torch.equal(o, step(x))
+
+
+def test_threads_with_streams_of_their_own():
+    gu, dn, _, _ = _stacks(6, 128, 64, 700)
+    w = linear.lay_out(packed(128, 128, 70), DEV)
+    xs = [_x(n, 128, torch.float32, n) for n in (3, 2501, 60, 2501)]
+
+    def step(x):
+        index, weight = moe.route(x[:, :6], 2, scores="sigmoid")
+        return linear.stored_linear(moe.stored_experts(x, index, weight, gu, dn), w, activation="gelu")
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    got = [[] for _ in xs]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = [step(xs[i]) for _ in range(10)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(xs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for ys, y in zip(got, want):
+        assert len(ys) == 10 and all(torch.equal(v, y) for v in ys)
+    w.check(), gu.check(), dn.check()
+
+
+@pytest.mark.parametrize("tokens", [5, 1500])
+def test_operands_and_results_in_one_buffer(tokens):
+    t = packed(190, 128, 61)
+    w = linear.lay_out(t, DEV)
+    buf = _x(tokens, 400, torch.bfloat16, 3)
+    want = linear.stored_linear(buf[:, :128].clone(), w, residual=buf[:, 200:390].clone())
+    y = linear.stored_linear(buf[:, :128], w, residual=buf[:, 200:390], out=buf[:, 200:390])  # other columns: allowed
+    assert torch.equal(y, want)
+    flat = buf.reshape(-1)
+    for call in (
+        lambda: linear.stored_linear(buf[:, :128], w, out=buf[:, 100:290]),
+        lambda: linear.stored_linear(buf[:, :128], w, residual=buf[:, 201:391], out=buf[:, 200:390]),
+        lambda: linear.stored_linear(buf[:, :128], w, bias=buf[0, 200:390], out=buf[:, 200:390]),
+        lambda: linear.stored_linear(flat[: 128 * tokens].view(tokens, 128), w, out=flat[: 190 * tokens].view(tokens, 190)),
+    ):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
 
 
 def test_refusals_on_the_device():

@@ -24,9 +24,14 @@ def test_stored_linear_arguments():
 
     ok = _struct()
     assert lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.BF16, 4) == 0  # a few rows need none
-    need = lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.BF16, 400)
-    assert need >= 400 * 128 * 2 + 400 * 4
-    assert lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.F32, 400) >= 2 * 400 * 128 * 2
+    assert linear.FEW_TOKENS == 16
+    long = _struct(rows_per_expert=1 << 20, groups_per_expert=1 << 15, k=1 << 16)
+    for dtype in (_lib.BF16, _lib.F16, _lib.F32):
+        assert lib.hi2_stored_linear_workspace_bytes(C.byref(long), dtype, 16) == 0
+        assert lib.hi2_stored_linear_workspace_bytes(C.byref(long), dtype, 17) >= 17 * (1 << 16) * 2
+    need = lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.BF16, 4000)
+    assert need >= 4000 * 128 * 2 + 4000 * 4
+    assert lib.hi2_stored_linear_workspace_bytes(C.byref(ok), _lib.F32, 4000) >= 2 * 4000 * 128 * 2
     assert call(ok, tokens=0) == _lib.OK
     for bad in (_struct(k=100), _struct(experts=2), _struct(data=None), _struct(groups_per_expert=3),
                 _struct(rows_per_expert=129), _struct(experts=0), _struct(k=0)):
@@ -34,7 +39,7 @@ def test_stored_linear_arguments():
     for kw in (dict(dtype=_lib.F64), dict(act=5), dict(act=-1), dict(tokens=-1), dict(tokens=1 << 31), dict(x=None), dict(out=None)):
         assert call(ok, **kw) == _lib.ERR_ARG
     for kw in (dict(ws=None), dict(size=need - 1), dict(ws=264)):
-        assert call(ok, tokens=400, **kw) == _lib.ERR_WORKSPACE
+        assert call(ok, tokens=4000, **kw) == _lib.ERR_WORKSPACE
 
 
 def test_stored_experts_arguments():
