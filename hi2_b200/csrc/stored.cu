@@ -269,7 +269,7 @@ inline int64_t rows_per_expert(int64_t experts, int64_t pairs) {  // with half a
 }
 inline bool few_experts(const hi2_stored_weight& gate_up, int64_t pairs, int parts) {  // both products, or neither
   if (rows_per_expert(gate_up.experts, pairs) <= 2 * FEW_WIDTH) return true;
-  const int64_t tiles = pairs / FEW_WIDTH + gate_up.experts, hidden = gate_up.k, inner = gate_up.rows_per_expert / 2;
+  const int64_t tiles = few_tiles(gate_up.experts, pairs), hidden = gate_up.k, inner = gate_up.rows_per_expert / 2;
   return few_plan(hidden, ceil_div(2 * inner, (int64_t)TILE_ROWS), tiles, FEW_WIDTH, parts).cost <= FEW_COST &&
          few_plan(inner, ceil_div(hidden, (int64_t)TILE_ROWS), tiles, FEW_WIDTH, parts).cost <= FEW_COST;
 }

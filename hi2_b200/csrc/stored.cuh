@@ -339,6 +339,7 @@ struct FewPlan {
   int64_t cost;    // of the fullest SM, in chunks
 };
 FewPlan few_plan(int64_t k, int64_t row_tiles, int64_t tiles, int64_t width, int parts);
+int64_t few_tiles(int64_t experts, int64_t rows);
 int product_few(const Product& p, cudaStream_t stream, const char* what);
 // Wide tiles, from prepared activations.
 int wide_width(int64_t rows);

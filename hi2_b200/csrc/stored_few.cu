@@ -375,9 +375,13 @@ FewPlan few_plan(int64_t k, int64_t row_tiles, int64_t tiles, int64_t width, int
   return plan;
 }
 
+// Of a stack: about as many as there will be, with half of every expert's last one empty.
+int64_t few_tiles(int64_t experts, int64_t rows) { return rows / FEW_WIDTH + experts / 2 + 1; }
+
 int product_few(const Product& p, cudaStream_t stream, const char* what) {
   const int64_t width = p.tiles.width < p.tiles.rows ? p.tiles.width : p.tiles.rows;
-  const FewPlan plan = few_plan(p.w.k, p.w.groups_per_expert / 4, p.max_tiles, width, p.parts);
+  const int64_t tiles = p.tiles.count != nullptr ? few_tiles(p.w.experts, p.tiles.rows) : p.max_tiles;
+  const FewPlan plan = few_plan(p.w.k, p.w.groups_per_expert / 4, tiles, width, p.parts);
   return p.parts == 1 ? launch<1>(p, plan.split, plan.run, stream, what) : launch<2>(p, plan.split, plan.run, stream, what);
 }
 
