@@ -16,7 +16,8 @@ namespace stored {
 namespace {
 
 // ---- layout -----------------------------------------------------------------------------------------
-// One thread moves one row's 64 columns: codes into their words, parameter pairs behind them.
+// One thread moves one row's 64 columns: codes into their words, parameter pairs behind them.  Its own format follows
+// from the length of its code words and pairs; the group's form may be wider, with shorter blocks.
 __global__ void __launch_bounds__(256)
 lay_out_kernel(const hi2_stored_weight w, const int32_t* __restrict__ src_row, const int32_t* __restrict__ codes,
                const int32_t* __restrict__ code_off, const uint8_t* __restrict__ blk_params,
@@ -31,20 +32,24 @@ lay_out_kernel(const hi2_stored_weight w, const int32_t* __restrict__ src_row, c
     const int g = (int)(i & 7), r = (int)(i >> 3 & 3);
     uint8_t* slab = data + (int64_t)form.base * 16 + chunk * form.slab_bytes();
     const int nbits = 1 << form.width(), per_word = 32 / nbits, per_piece = nbits / 2;
-    const uint32_t mask = (1u << nbits) - 1u;
-    const int32_t* words = codes + code_off[src] + chunk * 2 * nbits;
+    const int own_words = (int)((code_off[src + 1] - code_off[src]) / chunks);  // of a chunk: two per bit of a code
+    const int own_bits = own_words / 2, own_pairs = (int)((param_off[src + 1] - param_off[src]) / chunks);
+    const uint32_t mask = (1u << own_bits) - 1u;
+    const int32_t* words = codes + code_off[src] + chunk * own_words;
     for (int q = 0; q < 2 * nbits; ++q) {
-      const uint32_t v = (uint32_t)words[q];
       uint32_t fields = 0;
-      for (int f = 0; f < per_word; ++f) fields |= (v >> (f * nbits) & mask) << ((f >> 1) * nbits + (f & 1) * 16);
+      for (int f = 0; f < per_word; ++f) {
+        const int bit = (q * per_word + f) * own_bits;
+        fields |= ((uint32_t)words[bit >> 5] >> (bit & 31) & mask) << ((f >> 1) * nbits + (f & 1) * 16);
+      }
       reinterpret_cast<uint32_t*>(slab)[128 * (q % per_piece) + code_word(g, q / per_piece) + r] = fields;
     }
     const int pairs = 4 >> form.shift();
-    const uint8_t* from = blk_params + 2 * (param_off[src] + chunk * pairs);
+    const uint8_t* from = blk_params + 2 * ((int64_t)param_off[src] + chunk * own_pairs);
     uint8_t* to = slab + form.code_bytes();
     for (int t = 0; t < pairs; ++t) {
-      const int unit = 4 * (pairs * g + t) + r;
-      to[2 * unit] = from[2 * t], to[2 * unit + 1] = from[2 * t + 1];
+      const int unit = 4 * (pairs * g + t) + r, own = t * own_pairs / pairs;
+      to[2 * unit] = from[2 * own], to[2 * unit + 1] = from[2 * own + 1];
     }
   }
 }

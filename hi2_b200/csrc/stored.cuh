@@ -1,7 +1,9 @@
 // Packed weights laid out for products, and how they are decoded.
 //
-// The rows of a tensor (of each expert of a stack) are sorted by row format and dealt out to groups of 32 rows
-// of ONE format (the last group of a format is filled up with padding rows).  A group's data is cut into
+// The rows of a tensor (of each expert of a stack) are sorted by row format and cut into groups of 32 rows.  All rows of
+// a group are kept in ONE form: where formats meet, rows with narrower codes or longer blocks take the others' width
+// and block (the same codes in wider fields, their parameters repeated), so that only the last group of an expert has
+// padding rows.  (Padding every format's last group instead took 17 tiles for 2048 rows of four formats.)  A group's data is cut into
 // chunks of 64 columns; a chunk (a slab) holds the codes of its 32 rows and behind them their (lo, step) byte
 // pairs, so a warp reads a run of chunks as one contiguous range.  Row 8 r + g of a group (g < 8, r < 4) has in
 // a chunk nbits / 2 words of codes for each of its four 16-column pieces t; word h of piece t lies at word

@@ -103,41 +103,36 @@ def _lay_out_on(f: dict, experts: int, rows: int, k: int, stacked: bool, dev: to
     if not all(good[1:]):
         raise ValueError("lay_out: the row offsets do not fit the buffers")
 
-    # Rows by (width, block), a stable order.  Every format's rows fill groups of 32; the last one of each is
-    # filled up with padding, and so are the groups of an expert to whole tiles.
+    # Rows by width and falling block, a stable order, cut into groups of 32 and filled up to whole tiles.  A group has
+    # the widest codes and the shortest blocks of its rows.
     shift = torch.log2(block.double()).round().long() - 4       # 0, 1, 2
     width = torch.log2(nbits.double()).round().long()           # 1, 2, 3
-    key = (3 * (width - 1) + shift).view(experts, rows)
-    counts = torch.zeros(experts, 9, dtype=torch.int64, device=dev).scatter_add_(1, key, torch.ones_like(key))
-    groups = (counts + _GROUP_ROWS - 1) // _GROUP_ROWS
-    first = groups.cumsum(1) - groups                           # first group of every format
-    most = int(groups.sum(1).max())
-    per_expert = -(-most // _TILE_GROUPS) * _TILE_GROUPS
-    sorted_key, order = torch.sort(key, dim=1, stable=True)
-    before = counts.cumsum(1) - counts
-    place = _GROUP_ROWS * first.gather(1, sorted_key) + torch.arange(rows, device=dev) - before.gather(1, sorted_key)
-    expert = torch.arange(experts, device=dev)[:, None]
-    src = torch.full((experts, per_expert * _GROUP_ROWS), -1, dtype=torch.int64, device=dev)
-    src.scatter_(1, place, expert * rows + order)
-    lead = src[:, ::_GROUP_ROWS].reshape(-1)                    # a group's first row is never padding, unless all are
-    at = lead.clamp_min(0)
-    live = lead >= 0
-    # groups whose largest step, times the power of two that its codes are read with, is still an fp16 number
-    limit = 65504.0 / 2.0 ** (16 + 2 * torch.log2(nbits.double()).round())  # 2^18, 2^20, 2^22
-    step = 255 * consts[:, 2].float()
-    small = ((step >= 0) & (step <= limit))[src.clamp_min(0)] | (src < 0)
-    small = small.view(-1, _GROUP_ROWS).all(1).long()
-    form = torch.where(live, width[at] | shift[at] << 2 | small << 4, torch.zeros_like(lead))
-    units = torch.where(live, (16 << width[at]) + (16 >> shift[at]), torch.zeros_like(lead))  # of 16 bytes, per chunk
+    order = torch.sort((3 * width - shift).view(experts, rows), dim=1, stable=True).indices
+    tile_rows = _GROUP_ROWS * _TILE_GROUPS
+    src = torch.full((experts, -(-rows // tile_rows) * tile_rows), -1, dtype=torch.int64, device=dev)
+    src[:, :rows] = order + rows * torch.arange(experts, device=dev)[:, None]
+    src = src.reshape(-1)
+    real, at = src >= 0, src.clamp_min(0)
+
+    def of_groups(t):
+        return t.view(-1, _GROUP_ROWS)
+
+    live = of_groups(real)[:, 0]  # the others have padding rows only
+    widest = of_groups(torch.where(real, width[at], 0)).amax(1)
+    shortest = of_groups(torch.where(real, shift[at], 2)).amin(1)
+    # groups whose largest step, times the power of two that their codes are read with, is still an fp16 number
+    limit = 65504.0 / 2.0 ** (16 + 2 * widest)[:, None]  # 2^18, 2^20, 2^22
+    step = of_groups(255 * consts[:, 2].float()[at])
+    small = (((step >= 0) & (step <= limit)) | ~of_groups(real)).all(1).long()
+    form = torch.where(live, widest | shortest << 2 | small << 4, 0)
+    units = torch.where(live, (16 << widest) + (16 >> shortest), 0)  # of 16 bytes, per chunk
     base = (units * (k // CHUNK)).cumsum(0)
     total_units = int(base[-1].item())
     if total_units >= 2**32:
         raise ValueError("lay_out: more than 64 GiB of packed rows")
     base = base - units * (k // CHUNK)
-    src = src.reshape(-1)
-    at = src.clamp_min(0)
     half = consts.view(torch.int16).long() & 0xFFFF
-    rows_t = torch.stack([torch.where(src >= 0, at % rows, torch.full_like(at, 2**32 - 1)),
+    rows_t = torch.stack([torch.where(real, at % rows, 2**32 - 1),
                           (half[:, 0] | half[:, 1] << 16)[at], half[:, 2][at], torch.zeros_like(at)], 1)
 
     def words(t):  # the low 32 bits
