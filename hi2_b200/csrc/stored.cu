@@ -264,7 +264,7 @@ inline int parts_of(int dtype) { return dtype == HI2_BF16 ? 1 : 2; }
 // is one launch where the other takes three).  Measured, few / wide, us (and cost): 256 tokens x 512 x 512 8.7 / 15.4
 // (24), 77 x 1001 x 1088 in fp32 11.8 / 16.9 (26), 64 x 2048 x 2048 12.8 / 17.4 (36), 24 x 4096 x 4096 19.5 / 19.0 (42),
 // 64 x 4096 x 4096 34 / 22 (84); 111 pairs of 5 experts of 192 x 320 in fp32 25.1 / 32.8 (25).
-constexpr int64_t FEW_COST = 40;
+constexpr double FEW_COST = 40;
 inline bool few(const hi2_stored_weight& w, int64_t tokens, int parts) {
   return tokens <= 2 * FEW_WIDTH || few_plan(w.k, w.groups_per_expert / 4, ceil_div(tokens, (int64_t)FEW_WIDTH), FEW_WIDTH, parts).cost <= FEW_COST;
 }

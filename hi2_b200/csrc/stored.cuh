@@ -337,8 +337,8 @@ struct Product {
 // Products with up to 8 activation rows per tile, which prepare their activations themselves.
 constexpr int FEW_WIDTH = 8;
 struct FewPlan {
-  int split, run;  // slices of the columns; tiles of packed rows per block
-  int64_t cost;    // of the fullest SM, in chunks
+  int split, runs;  // slices of the columns (a cluster); runs of row tiles, a block each
+  double cost;      // of the fullest SM, in chunks
 };
 FewPlan few_plan(int64_t k, int64_t row_tiles, int64_t tiles, int64_t width, int parts);
 int64_t few_tiles(int64_t experts, int64_t rows);

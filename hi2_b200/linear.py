@@ -198,7 +198,7 @@ def stored_linear(x: torch.Tensor, w: StoredWeight, bias: torch.Tensor | None = 
         res = res if res.stride(1) == 1 else res.contiguous()
         res_ptr, ld_res = res.data_ptr(), res.stride(0)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        out = x.new_empty(shape)
         ld_out = n
     else:
         y = output_rows(out, shape, x, "stored_linear")

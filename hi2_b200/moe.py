@@ -250,8 +250,8 @@ def route(logits: torch.Tensor, top_k: int, scores: str = "softmax", bias: torch
         bias = bias.contiguous()
         bias_ptr = bias.data_ptr()
     shape = (*logits.shape[:-1], top_k)
-    index = torch.empty(shape, dtype=torch.int64, device=dev)
-    weight = torch.empty(shape, dtype=torch.float32, device=dev)
+    index = logits.new_empty(shape, dtype=torch.int64)
+    weight = logits.new_empty(shape, dtype=torch.float32)
     _lib.launch("hi2_route", dev.index, rows.data_ptr(), dtype, rows.shape[0], experts, rows.stride(0), top_k, sigmoid, bias_ptr, groups,
                 groups if top_groups is None else top_groups, 1 if renormalise else 0, scale, index.data_ptr(), weight.data_ptr())
     return index, weight
@@ -282,7 +282,7 @@ def stored_experts(x: torch.Tensor, index: torch.Tensor, weight: torch.Tensor, g
     no_gradient("stored_experts", x, weight, out)
     y = None
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        out = x.new_empty(x.shape)
         ld_out = down.rows
     else:
         y = output_rows(out, x.shape, x, "stored_experts")
