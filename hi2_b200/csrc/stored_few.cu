@@ -1,5 +1,5 @@
-// The product of packed rows with up to 8 activation rows: decode steps and small batches, where the packed
-// bytes are what has to be moved.
+// The product of packed rows with tiles of up to 8 activation rows: single tokens, small batches, experts with a few
+// tokens each.
 //
 // A block takes 128 sorted rows and a slice of the columns; the slices of a row tile are a cluster and join
 // their sums through distributed shared memory in rank order.  Warps 0..3 and 4..7 take the tile's four groups
@@ -9,11 +9,14 @@
 //
 // The slice is taken in blocks of 1024 columns.  First the warps form the activations' fp16 parts of the block
 // in shared memory (divided, rotated, relative to a power of two per row and half of the BLOCK, so nothing
-// waits for a whole row's largest value); then every warp decodes chunk after chunk straight into the A fragments of warp-level
-// products m16n8k16: lane 4 g + t holds 16 columns of rows g, g + 8, g + 16 and g + 24, and the column order
+// waits for a whole row's largest value); then every warp decodes chunk after chunk straight into the A fragments of
+// warp-level products m16n8k16: lane 4 g + t holds 16 columns of rows g, g + 8, g + 16 and g + 24, and the column order
 // inside a chunk is the same permutation for both operands, so a lane's 16 columns are contiguous in memory.
-// The tensor pipe is idle most of the time; what bounds the kernel is the decoding, about 150 instructions per
-// warp for 2048 INT2 weights, and behind it the packed bytes.
+//
+// What bounds it: decoding and products share the fp16 pipe (183 clocks for 2048 INT2 weights, stored.cuh).  28672 x 8192
+// INT2 weights with one row take 41 us where streaming them alone takes 16 and the products without decoding 22; the
+// packed bytes ask for 12.  In the smallest calls it is latency: 4096 x 4096 with one row takes 7.7 us.  Measured and
+// dropped: three stages per ring with one block per SM; the next chunk's words read ahead of the products.
 #include <type_traits>
 
 #include "stored_async.cuh"

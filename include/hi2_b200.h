@@ -333,9 +333,11 @@ int hi2_allocate_bits(const double* cost, const double* bits, int n_cand, int64_
  * A packed tensor, or a stack of `experts` of them with rows_per_expert rows each, laid out for products
  * (hi2_lay_out_rows).  This struct lives in HOST memory; its pointers are device pointers.  `rows` holds
  * four words per sorted row (output row, fp16 lo_min and lo_scale, fp16 step scale, 0), `groups` two per 32
- * sorted rows, which share one format (first 16-byte unit of the group's data; log2 of the code width, 0 for
- * padding, log2(block / 16) << 2, and 1 << 4 where 255 * step scale of every row is at most 65504 / 2^18,
- * 2^20 or 2^22 for 2-, 4- and 8-bit codes); groups_per_expert is a multiple of 4.  had [experts, k/16], inv_scale fp32 [experts, k] (reciprocal smoothing vector; null: none).
+ * sorted rows, which are kept in one form, at least as wide and with blocks at most as long as their formats'
+ * (first 16-byte unit of the group's data; log2 of the code width, 0 for padding only, log2(block / 16) << 2, and
+ * 1 << 4 where 255 * step scale of every row is at most 65504 / 2^18, 2^20 or 2^22 for 2-, 4- and 8-bit codes);
+ * groups_per_expert is a multiple of 4.  had [experts, k/16], inv_scale fp32 [experts, k] (reciprocal smoothing
+ * vector; null: none).
  * status: a device int that a bounded wait which ran out raises and nothing clears. */
 typedef struct {
   const void* data;
@@ -350,7 +352,8 @@ typedef struct {
 enum { HI2_ACT_NONE = 0, HI2_ACT_RELU = 1, HI2_ACT_SILU = 2, HI2_ACT_GELU = 3, HI2_ACT_GELU_TANH = 4 };
 
 /* Fill `data` (zeroed by the caller) from the flat buffers of the format: sorted row i is row
- * src_row[i] of the flat buffers (negative: padding), its place given by w->rows and w->groups.
+ * src_row[i] of the flat buffers (negative: padding), its place given by w->rows and w->groups.  Products may
+ * read `data` before the kernel ahead of them on their stream has ended: wait for this one before the first.
  * No counterpart in the reference: its decode kernels live in the inference engine. */
 int hi2_lay_out_rows(const hi2_stored_weight* w_host, const int32_t* src_row, const int32_t* codes,
                      const int32_t* code_off, const uint8_t* blk_params, const int32_t* param_off, void* data,
@@ -360,7 +363,7 @@ int hi2_lay_out_rows(const hi2_stored_weight* w_host, const int32_t* src_row, co
  * out[m, n] = act(x' @ W^T + bias) + residual, x' the smoothed and rotated activations, W the fp16
  * reconstruction in the stored basis (w->experts is 1).  x [tokens, k] with row stride ldx; bias [n] and residual
  * [tokens, n] (row stride ld_residual) may be null; out [tokens, n] with row stride ld_out.  dtype (F32, F16 or
- * BF16) is that of x, bias, residual and out.  out may be residual. */
+ * BF16) is that of x, bias, residual and out.  out may be residual, and shares no memory with the others. */
 size_t hi2_stored_linear_workspace_bytes(const hi2_stored_weight* w_host, int dtype, int64_t tokens);
 int hi2_stored_linear(const hi2_stored_weight* w_host, const void* x, int dtype, int64_t tokens, int64_t ldx,
                       const void* bias, int act, const void* residual, int64_t ld_residual, void* out, int64_t ld_out,
@@ -370,7 +373,7 @@ int hi2_stored_linear(const hi2_stored_weight* w_host, const void* x, int dtype,
  * hi2/moe.py:53-121): out[t] = sum_j weight[t, j] * down_e(act(gate_e(x[t])) * up_e(x[t])) with
  * e = index[t, j]; a slot whose index lies outside 0 .. experts - 1 adds nothing.  gate_up has 2 I rows per
  * expert (gate first) over k = hidden columns, down `hidden` rows over I.  x [tokens, hidden] with row stride ldx,
- * index int64 and weight fp32 [tokens, top_k] contiguous, out [tokens, hidden] with row stride ld_out. */
+ * index int64 and weight fp32 [tokens, top_k] contiguous, out [tokens, hidden] with row stride ld_out; out may be x. */
 size_t hi2_stored_experts_workspace_bytes(const hi2_stored_weight* gate_up_host, int dtype, int64_t tokens, int top_k);
 int hi2_stored_experts(const hi2_stored_weight* gate_up_host, const hi2_stored_weight* down_host, const void* x,
                        int dtype, int64_t tokens, int64_t ldx, const int64_t* index, const float* weight, int top_k,
