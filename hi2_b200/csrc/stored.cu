@@ -296,11 +296,11 @@ struct LinearSpace {
     if (!small) {
       xs = c.take<__half>((size_t)tokens * w.k * parts_of(dtype));
       scale = c.take<float>(tokens);
-      width = wide_width(tokens);
+      width = wide_width(tokens, dtype == HI2_F32);
     }
     max_tiles = ceil_div(tokens, (int64_t)width);
     if (!small) {
-      const int splits = wide_splits(w.k, w.rows_per_expert, tokens, max_tiles, false, dtype == HI2_F32);
+      const int splits = wide_splits(w.k, w.rows_per_expert, max_tiles, false);
       if (splits > 1) partial = c.take<float>((size_t)splits * tokens * w.rows_per_expert);
     }
     bytes = c.used;
@@ -309,7 +309,7 @@ struct LinearSpace {
 
 struct ExpertSpace {
   __half* xs = nullptr;  // of the gate/up product, then of the down product
-  float *scale = nullptr, *partial = nullptr, *z, *y;
+  float *scale = nullptr, *z, *y;
   int32_t *pair_of = nullptr, *row_of = nullptr, *next_row = nullptr, *used = nullptr, *tile_count = nullptr;
   TokenTile* tiles = nullptr;
   bool small;
@@ -331,10 +331,6 @@ struct ExpertSpace {
     if (!small) {
       xs = c.take<__half>(pairs * (hidden > inner ? hidden : inner) * parts_of(dtype));
       scale = c.take<float>(pairs);
-      const bool exact = dtype == HI2_F32;
-      const size_t up = wide_splits(hidden, 2 * inner, pairs, 1, true, exact), dn = wide_splits(inner, hidden, pairs, 1, true, exact);
-      const size_t most = 2 * inner * (up > 1 ? up : 0) > hidden * (dn > 1 ? dn : 0) ? 2 * inner * up : hidden * (dn > 1 ? dn : 0);
-      if (most > 0) partial = c.take<float>(pairs * most);
     }
     bytes = c.used;
   }
@@ -425,7 +421,7 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   int rc;
   if (!apart(pairs)) {
     const int64_t busy = rows_per_expert(experts, pairs);
-    tiles = Tiles{index, space.pair_of, space.tile_count, space.tiles, pairs, experts, space.small ? FEW_WIDTH : wide_width(busy)};
+    tiles = Tiles{index, space.pair_of, space.tile_count, space.tiles, pairs, experts, space.small ? FEW_WIDTH : wide_width(busy, dtype == HI2_F32)};
     max_tiles = pairs / tiles.width + experts + 1;
     count_kernel<<<1, SORT_THREADS, 0, s>>>(index, pairs, experts, tiles.width, space.next_row, space.used, space.tile_count, space.tiles);
     if ((rc = check_launch("stored_experts: dispatch")) != HI2_OK) return rc;
@@ -435,10 +431,10 @@ extern "C" int hi2_stored_experts(const hi2_stored_weight* gate_up, const hi2_st
   }
   const Product up{*gate_up, Source{x, ldx, kind_of(dtype), HI2_ACT_NONE, rows_aligned(x, ldx, dtype), top_k}, tiles, max_tiles, parts,
                    Epilogue{nullptr, nullptr, nullptr, space.z, 0, 2 * inner, HI2_ACT_NONE, HI2_F32}, dtype == HI2_F32, false, space.xs,
-                   space.scale, space.partial};
+                   space.scale, nullptr};
   const Product dn{*down, Source{space.z, 2 * inner, FROM_GATED, act, true, top_k}, tiles, max_tiles, parts,
                    Epilogue{weight, nullptr, nullptr, space.y, 0, hidden, HI2_ACT_NONE, HI2_F32}, dtype == HI2_F32, true, space.xs,
-                   space.scale, space.partial};
+                   space.scale, nullptr};
   for (const Product* p : {&up, &dn}) {
     if (space.small) {
       rc = product_few(*p, s, "stored_experts");

@@ -344,8 +344,8 @@ FewPlan few_plan(int64_t k, int64_t row_tiles, int64_t tiles, int64_t width, int
 int64_t few_tiles(int64_t experts, int64_t rows);
 int product_few(const Product& p, cudaStream_t stream, const char* what);
 // Wide tiles, from prepared activations.
-int wide_width(int64_t rows);
-int wide_splits(int64_t k, int64_t rows_of_tensor, int64_t rows, int64_t max_tiles, bool stack, bool exact);
+int wide_width(int64_t rows, bool exact);
+int wide_splits(int64_t k, int64_t rows_of_tensor, int64_t max_tiles, bool stack);
 int product_wide(const Product& p, cudaStream_t stream, const char* what);
 
 }  // namespace stored

@@ -38,7 +38,8 @@ namespace {
 
 constexpr int DECODE_WARPS = 8, X_WARP = 8, MMA_WARP = 9, FIRST_EPILOGUE = 10, EPILOGUE_WARPS = 4;
 constexpr int THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE_WARPS);
-constexpr int MAX_WIDTH = 192;
+constexpr int MAX_WIDTH = 192, MAX_EXACT_WIDTH = 128;
+constexpr int EXACT_STEPS = 2;  // of a sum that the tensor cores form for an fp32 result
 constexpr int MAX_SLOTS = 4, A_COLUMNS = CHUNK / 2, SLOT_COLUMNS = 2 * A_COLUMNS;
 constexpr int RING_STAGES = 2, RING_BYTES = 3072;  // a stage: four chunks of INT2, two of INT4, one of INT8
 constexpr int MAX_X_STAGES = 6;
@@ -112,6 +113,15 @@ __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)
       "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
       "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const float (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]),
+      "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
       : "memory");
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -334,6 +344,10 @@ __device__ __forceinline__ void put_rows(const Epilogue& out, float (&v)[16], in
   else write_rows<float>(out.out, out.ld_out, row, col, count, v);
 }
 
+// EXACT: fp32 results.  The tensor cores' accumulator drops what does not fit it at every step, always towards zero,
+// which over 2048 columns costs 2e-6 of a result and over 256 3e-7.  So a sum there covers 256 columns, small parts first, and
+// the epilogue's warps add the sums up in fp32, in tensor memory of their own.  (@EXACT@)
+template <bool EXACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shape shape) {
   extern __shared__ uint8_t raw[];
@@ -365,7 +379,8 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
   fence_after();
   const uint32_t tmem = ctl->tmem_base;
   const uint32_t d_columns = (uint32_t)(shape.width + 31) & ~31u;
-  const uint32_t a_tmem = tmem + 2 * d_columns;  // behind the two accumulators
+  const uint32_t s_tmem = tmem + 2 * d_columns;  // behind the two accumulators: sums of several, for fp32 results
+  const uint32_t a_tmem = s_tmem + (EXACT ? d_columns : 0);
   const int64_t first_item = blockIdx.x >> 1, stride = gridDim.x >> 1;
   chain_wait();  // the tile list, the activations, and whatever the outputs overwrite
   bool ok = true;
@@ -456,11 +471,15 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
       const int cols = (item.tile.end - item.tile.begin + 15) & ~15;
       // fp16 operands (format 0 at bits 7 and 10), fp32 accumulator (1 << 4), N >> 3 at bit 17, M >> 4 at bit 24
       const uint32_t idesc = (1u << 4) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(2 * TILE_ROWS >> 4) << 24);
-      const uint32_t d = d_first + buf * d_columns;
       const int second = second_chunks(shape, item);
-      ok = __all_sync(0xffffffffu, bar_wait(&ctl->d_empty[buf], d_phase, &ctl->abort, status));
-      if (!ok) break;
+      int in_sum = 0;
       for (int i = 0; i < item.count; ++i) {
+        if (in_sum == 0) {
+          ok = __all_sync(0xffffffffu, bar_wait(&ctl->d_empty[buf], d_phase, &ctl->abort, status));
+          if (!ok) break;
+        }
+        const bool last = (EXACT && in_sum + 1 == EXACT_STEPS) || i == item.count - 1;
+        const uint32_t d = d_first + buf * d_columns;
         const uint32_t a = a_first + slot * SLOT_COLUMNS;
         const uint64_t b = b_first + (uint32_t)(stage * stage_bytes >> 4);
         ok = bar_wait(&ctl->x_full[stage], phase, &ctl->abort, status);
@@ -469,7 +488,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
         if (!ok) break;
         fence_after();
         if (elected()) {
-          uint32_t accumulate = i > 0 ? 1u : 0u;
+          uint32_t accumulate = in_sum > 0 ? 1u : 0u;
           for (int part = p.parts - 1; part >= 0; --part) {  // small parts first
 #pragma unroll
             for (int kk = 0; kk < CHUNK / 16; ++kk) mma_pair(d, a + kk * 8, b + part * box + kk * 2, idesc, kk > 0 ? 1u : accumulate);
@@ -481,13 +500,17 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
           }
           commit_both(&ctl->a_empty[slot]);
           commit_both(&ctl->x_empty[stage]);
-          if (i == item.count - 1) commit_both(&ctl->d_full[buf]);
+          if (last) commit_both(&ctl->d_full[buf]);
         }
         __syncwarp();
         if (++stage == shape.x_stages) stage = 0, phase ^= 1;
         if (++slot == shape.slots) slot = 0, slot_phase ^= 1;
+        ++in_sum;
+        if (last) {
+          in_sum = 0;
+          if (++buf == 2) buf = 0, d_phase ^= 1;
+        }
       }
-      if (++buf == 2) buf = 0, d_phase ^= 1;
     }
   } else if (warp >= FIRST_EPILOGUE) {
     // ------------------------------------------------------------ epilogue
@@ -508,16 +531,45 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
         if (p.out.pair_weight != nullptr) scale[t] *= p.out.pair_weight[p.tiles.pair(item.tile.begin + t)];
       }
       __syncwarp();
+      Epilogue out = p.out;
+      if (shape.splits > 1) out.out = static_cast<float*>(out.out) + (int64_t)item.slice * p.tiles.rows * out.ld_out;
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const int sums = !EXACT ? 1 : (item.count + EXACT_STEPS - 1) / EXACT_STEPS;
+      for (int i = 0; i < sums - 1; ++i) {  // sums that do not end the item are added up behind the accumulators
+        ok = __all_sync(0xffffffffu, bar_wait(&ctl->d_full[buf], phase, &ctl->abort, status));
+        if (!ok) break;
+        fence_after();
+#pragma unroll 1
+        for (int t0 = 0; t0 < tokens; t0 += 16) {
+          float v[16], sum[16];
+          tmem_load16(tmem + buf * d_columns + lanes + t0, v);
+          if (i > 0) {
+            tmem_load16(s_tmem + lanes + t0, sum);
+#pragma unroll
+            for (int t = 0; t < 16; ++t) v[t] += sum[t];
+          }
+          tmem_store16(s_tmem + lanes + t0, v);
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive_cluster(in_rank(s32(&ctl->d_empty[buf]), 0));
+        if (++buf == 2) buf = 0, phase ^= 1;
+      }
+      if (!ok) break;
       ok = __all_sync(0xffffffffu, bar_wait(&ctl->d_full[buf], phase, &ctl->abort, status));
       if (!ok) break;
       fence_after();
-      const uint32_t taddr = tmem + buf * d_columns + ((uint32_t)(quarter * 32) << 16);
-      Epilogue out = p.out;
-      if (shape.splits > 1) out.out = static_cast<float*>(out.out) + (int64_t)item.slice * p.tiles.rows * out.ld_out;
+      const uint32_t taddr = tmem + buf * d_columns + lanes;
 #pragma unroll 1
       for (int t0 = 0; t0 < tokens; t0 += 16) {
         float v[16];
         tmem_load16(taddr + t0, v);
+        if (EXACT && sums > 1) {
+          float sum[16];
+          tmem_load16(s_tmem + lanes + t0, sum);
+#pragma unroll
+          for (int t = 0; t < 16; ++t) v[t] += sum[t];
+        }
 #pragma unroll
         for (int t = 0; t < 16; t += 4) {
           const float4 f = *reinterpret_cast<const float4*>(scale + t0 + t);
@@ -573,12 +625,9 @@ EncodeFn encoder() {
 
 }  // namespace
 
-// Slices of the columns.  Of one tensor, for tiles that are fewer than the SM pairs: the number that leaves the busiest pair
-// the fewest steps, with start and end of an item counted as six of them; each at least four steps.  For fp32 results
-// (`exact`), as far as 1 GiB of partial sums goes, slices of 128 columns, of 256 with many rows: the tensor cores'
-// accumulator drops what does not fit it at every step, always towards zero, which over 2048 columns costs 2e-6 of a result
-// and over 256 3e-7 (small parts are added first).
-int wide_splits(int64_t k, int64_t rows_of_tensor, int64_t rows, int64_t max_tiles, bool stack, bool exact) {
+// Slices of the columns, for tiles that are fewer than the SM pairs: the number that leaves the busiest pair the fewest
+// steps, with start and end of an item counted as six of them; each at least four steps.  Of a stack always one.
+int wide_splits(int64_t k, int64_t rows_of_tensor, int64_t max_tiles, bool stack) {
   const int64_t items = (ceil_div(rows_of_tensor, (int64_t)TILE_ROWS) + 1) / 2 * max_tiles, count = (k / CHUNK + 1) / 2;
   int best = 1;
   int64_t least = INT64_MAX;
@@ -586,16 +635,11 @@ int wide_splits(int64_t k, int64_t rows_of_tensor, int64_t rows, int64_t max_til
     const int64_t cost = ceil_div(items * s, (int64_t)74) * (ceil_div(count, (int64_t)s) + 6);
     if (cost < least) least = cost, best = s;
   }
-  if (exact) {
-    const int64_t fit = ((int64_t)1 << 30) / (rows * rows_of_tensor * (int64_t)sizeof(float)), want = rows <= 2048 ? count : (count + 1) / 2;
-    const int64_t s = want < fit ? want : fit;
-    if (s > best) best = (int)(s < 256 ? s : 256);
-  }
   return best;
 }
 
-int wide_width(int64_t rows) {
-  const int64_t tiles = ceil_div(rows, (int64_t)MAX_WIDTH);
+int wide_width(int64_t rows, bool exact) {
+  const int64_t tiles = ceil_div(rows, (int64_t)(exact ? MAX_EXACT_WIDTH : MAX_WIDTH));
   return (int)(ceil_div(ceil_div(rows, tiles), (int64_t)16) * 16);
 }
 
@@ -607,18 +651,17 @@ int product_wide(const Product& p, cudaStream_t stream, const char* what) {
   const int stage_bytes = 2 * p.parts * (s.width / 2) * CHUNK * 2;
   s.x_stages = 144 * 1024 / stage_bytes;  // at least three
   if (s.x_stages > MAX_X_STAGES) s.x_stages = MAX_X_STAGES;
-  s.slots = (512 - 2 * ((s.width + 31) & ~31)) / SLOT_COLUMNS;  // at least two
+  s.slots = (512 - (p.exact ? 3 : 2) * ((s.width + 31) & ~31)) / SLOT_COLUMNS;  // at least two
   if (s.slots > MAX_SLOTS) s.slots = MAX_SLOTS;
   s.chunks = (int)(p.w.k / CHUNK), s.half0 = (s.chunks + 1) / 2;
   s.row_pairs = (int)((p.w.groups_per_expert / 4 + 1) / 2);
-  s.splits = wide_splits(p.w.k, p.w.rows_per_expert, p.tiles.rows, p.max_tiles, p.tiles.index != nullptr, p.exact);
+  s.splits = wide_splits(p.w.k, p.w.rows_per_expert, p.max_tiles, p.tiles.index != nullptr);
   size_t smem = (size_t)s.x_stages * stage_bytes + DECODE_WARPS * RING_STAGES * RING_BYTES + sizeof(Control) + 1024;
   // A block takes all of an SM's tensor memory: two must never be resident on one SM.
   if (smem < 120 * 1024) smem = 120 * 1024;
   Product q = p;
   if (s.splits > 1) {  // plain sums of the slices; joined below
     q.out = Epilogue{};
-    q.out.pair_weight = p.out.pair_weight;
     q.out.out = p.partial, q.out.ld_out = p.w.rows_per_expert, q.out.dtype = HI2_F32;
   }
 
@@ -634,7 +677,7 @@ int product_wide(const Product& p, cudaStream_t stream, const char* what) {
     set_error("%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
     return HI2_ERR_DRIVER;
   }
-  if (!reserve_smem<wide_kernel>())
+  if (!(p.exact ? reserve_smem<wide_kernel<true>>() : reserve_smem<wide_kernel<false>>()))
     return fail(HI2_ERR_LAUNCH, "stored product: cannot reserve shared memory");
   constexpr int sms = 148;
   const int64_t items = (int64_t)s.row_pairs * s.splits * p.max_tiles;
@@ -645,7 +688,7 @@ int product_wide(const Product& p, cudaStream_t stream, const char* what) {
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute, config.numAttrs = 1;
-  cudaLaunchKernelEx(&config, wide_kernel, map, q, s);
+  cudaLaunchKernelEx(&config, p.exact ? wide_kernel<true> : wide_kernel<false>, map, q, s);
   const int rc = check_launch(what);
   if (rc != HI2_OK || s.splits == 1) return rc;
   const int64_t values = p.tiles.rows * p.w.rows_per_expert;
