@@ -39,7 +39,7 @@ namespace {
 constexpr int DECODE_WARPS = 8, X_WARP = 8, MMA_WARP = 9, FIRST_EPILOGUE = 10, EPILOGUE_WARPS = 4;
 constexpr int THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE_WARPS);
 constexpr int MAX_WIDTH = 192, MAX_EXACT_WIDTH = 128;
-constexpr int EXACT_STEPS = 2;  // of a sum that the tensor cores form for an fp32 result
+constexpr int EXACT_STEPS = 1;  // of a sum that the tensor cores form for an fp32 result
 constexpr int MAX_SLOTS = 4, A_COLUMNS = CHUNK / 2, SLOT_COLUMNS = 2 * A_COLUMNS;
 constexpr int RING_STAGES = 2, RING_BYTES = 3072;  // a stage: four chunks of INT2, two of INT4, one of INT8
 constexpr int MAX_X_STAGES = 6;
@@ -345,8 +345,10 @@ __device__ __forceinline__ void put_rows(const Epilogue& out, float (&v)[16], in
 }
 
 // EXACT: fp32 results.  The tensor cores' accumulator drops what does not fit it at every step, always towards zero,
-// which over 2048 columns costs 2e-6 of a result and over 256 3e-7.  So a sum there covers 256 columns, small parts first, and
-// the epilogue's warps add the sums up in fp32, in tensor memory of their own.  (@EXACT@)
+// which over 2048 columns costs 2e-6 of a result.  So a sum there covers one step of 128 columns, small parts first, and the
+// epilogue's warps add the sums up in fp32, in tensor memory of their own.  Measured (2048 rows x 11008 x 4096; error of
+// 512 tokens through experts of 1024 x 512, where a plain fp32 product has 9.6e-7): one step 399 us, 5.3e-7; two 335 us,
+// 1.4e-6; four 322 us, 3.1e-6; slices of the columns joined through memory 1361 us.
 template <bool EXACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shape shape) {
