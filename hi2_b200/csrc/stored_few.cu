@@ -28,7 +28,7 @@ namespace {
 constexpr int WARPS = 8, THREADS = 256;
 constexpr int BLOCK_CHUNKS = 16, BLOCK_COLUMNS = BLOCK_CHUNKS * CHUNK;
 constexpr int HALF_CHUNKS = BLOCK_CHUNKS / 2;
-constexpr int RING_STAGES = 2, RING_BYTES = 3072;  // a stage: four chunks of INT2, two of INT4, one of INT8
+constexpr int RING_STAGES = 2, RING_BYTES = 3 * 1024;  // a stage: four chunks of INT2, two of INT4, one of INT8
 constexpr int X_PITCH = BLOCK_COLUMNS + 8;         // halves; the extra 16 bytes keep 128-bit reads of eight rows apart
 constexpr int SUM_PITCH = TILE_ROWS + 4;
 constexpr int MAX_SPLIT = 8;

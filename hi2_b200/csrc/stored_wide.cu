@@ -41,7 +41,7 @@ constexpr int THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE_WARPS);
 constexpr int MAX_WIDTH = 192, MAX_EXACT_WIDTH = 128;
 constexpr int EXACT_STEPS = 1;  // of a sum that the tensor cores form for an fp32 result
 constexpr int MAX_SLOTS = 4, A_COLUMNS = CHUNK / 2, SLOT_COLUMNS = 2 * A_COLUMNS;
-constexpr int RING_STAGES = 2, RING_BYTES = 3072;  // a stage: four chunks of INT2, two of INT4, one of INT8
+constexpr int RING_STAGES = 2, RING_BYTES = 3 * 1024;  // a stage: four chunks of INT2, two of INT4, one of INT8
 constexpr int MAX_X_STAGES = 6;
 
 struct Control {
