@@ -24,6 +24,8 @@ struct RouteParams {
   float* weight;
   float scale;
   int dtype, experts, top_k, sigmoid, groups, top_groups, renormalise;
+  int team_log;              // lanes that read through a group: as many as the groups leave, a power of two
+  uint32_t per, per_inverse; // experts of a group; e / per = e * per_inverse >> 20 for e < 1024 (per * per_inverse < 2^20 + per)
 };
 
 // Order-preserving integers; 0 is below every number and marks a closed expert.  -0 counts as 0.
@@ -138,17 +140,14 @@ route_kernel(const RouteParams p) {
     }
     if (p.groups > 1) {
       // Several lanes read through a group each, and find its two best keys together.
-      const int per = p.experts / p.groups;
       uint64_t* const all = shared[threadIdx.x >> 5].keys;
 #pragma unroll
       for (int i = 0; i < PER; ++i) all[i * 32 + lane] = key[i];
       __syncwarp();
-      int team = 32;  // lanes per group
-      while (team * p.groups > 32) team >>= 1;
-      const int mine = lane / team;
+      const int team = 1 << p.team_log, per = (int)p.per, mine = lane >> p.team_log;
       uint64_t first = 0, second = 0;
       if (mine < p.groups)
-        for (int e = mine * per + lane % team; e < (mine + 1) * per; e += team) {
+        for (int e = mine * per + (lane & (team - 1)); e < (mine + 1) * per; e += team) {
           const uint64_t k = all[e];
           if (k > first) second = first, first = k;
           else if (k > second) second = k;
@@ -160,7 +159,7 @@ route_kernel(const RouteParams p) {
         second = low > high ? low : high;
       }
       uint64_t total = first != 0 ? key_of(value_of(first) + (second != 0 ? value_of(second) : 0.0)) : 0;
-      total = __shfl_sync(ALL, total, (lane * team) & 31);  // lane q: the key of group q
+      total = __shfl_sync(ALL, total, (lane << p.team_log) & 31);  // lane q: the key of group q
       if (lane >= p.groups) total = 0;
       uint32_t kept = 0;
       uint64_t of_group[1] = {total};
@@ -171,7 +170,7 @@ route_kernel(const RouteParams p) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int e = i * 32 + lane;
-        if (e < p.experts && !(kept >> (e / per) & 1)) key[i] = 0;
+        if (!(kept >> ((uint32_t)e * p.per_inverse >> 20 & 31) & 1)) key[i] = 0;  // (those behind the last are closed already)
       }
     }
     if (p.bias == nullptr) {
@@ -220,7 +219,11 @@ extern "C" int hi2_route(const void* logits, int dtype, int64_t tokens, int expe
   HI2_REQUIRE(tokens >= 0 && tokens < (int64_t)1 << 31, "route: too many tokens");
   if (tokens == 0) return HI2_OK;
   HI2_REQUIRE(logits && index && weight, "route: null pointer");
-  const RouteParams p{logits, bias, tokens, ld, index, weight, scale, dtype, experts, top_k, sigmoid, groups, top_groups, renormalise};
+  int team_log = 5;
+  while (groups << team_log > 32) --team_log;
+  const uint32_t per = (uint32_t)(experts / groups);
+  const RouteParams p{logits, bias, tokens, ld, index, weight, scale, dtype, experts, top_k, sigmoid, groups, top_groups, renormalise,
+                      team_log, per, ((1u << 20) + per - 1) / per};
   const bool exact = bias != nullptr || groups > 1;
   const unsigned grid = (unsigned)ceil_div(tokens, (int64_t)ROUTE_WARPS);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
