@@ -18,8 +18,10 @@ def activation_number(name) -> int:
 
 
 def no_gradient(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what}: there is no gradient; call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what}: there is no gradient; call it under torch.no_grad()")
 
 
 def on_device(what: str, dev: torch.device, *tensors) -> None:
