@@ -60,6 +60,7 @@ lay_out_kernel(const hi2_stored_weight w, const int32_t* __restrict__ src_row, c
 template <int THREADS, int WARPS, int HOLD, int PARTS>
 __global__ void __launch_bounds__(THREADS)
 prepare_kernel(const Product p, const int32_t* __restrict__ used) {
+  chain_next();  // the product sets up and decodes its first chunks meanwhile
   constexpr int TEAM = WARPS * 32;
   const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
   const int64_t row = (int64_t)blockIdx.x * (THREADS / TEAM) + team;

@@ -384,7 +384,8 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
   const uint32_t s_tmem = tmem + 2 * d_columns;  // behind the two accumulators: sums of several, for fp32 results
   const uint32_t a_tmem = s_tmem + (EXACT ? d_columns : 0);
   const int64_t first_item = blockIdx.x >> 1, stride = gridDim.x >> 1;
-  chain_wait();  // the tile list, the activations, and whatever the outputs overwrite
+  // Only the warps that touch what the preparation of the activations writes, or the outputs, wait for it.  The tile list
+  // was complete before that one began.
   bool ok = true;
   Item item;
 
@@ -438,6 +439,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
     }
   } else if (warp == X_WARP) {
     // ------------------------------------------------------------ activations
+    chain_wait();
     int stage = 0;
     uint32_t phase = 1;
     for (int64_t at = first_item; ok && get_item(p, shape, at, rank, item); at += stride) {
@@ -516,6 +518,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
     }
   } else if (warp >= FIRST_EPILOGUE) {
     // ------------------------------------------------------------ epilogue
+    chain_wait();
     // a warp may only touch the 32 tensor-memory lanes of its index modulo 4
     const int quarter = warp & 3;
     int buf = 0;
