@@ -60,6 +60,7 @@ lay_out_kernel(const hi2_stored_weight w, const int32_t* __restrict__ src_row, c
 template <int THREADS, int WARPS, int HOLD, int PARTS>
 __global__ void __launch_bounds__(THREADS)
 prepare_kernel(const Product p, const int32_t* __restrict__ used) {
+  chain_wait();
   chain_next();  // the product sets up and decodes its first chunks meanwhile
   constexpr int TEAM = WARPS * 32;
   const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
@@ -125,8 +126,8 @@ prepare_kernel(const Product p, const int32_t* __restrict__ used) {
 template <int THREADS, int WARPS, int HOLD>
 void launch_prepare(const Product& p, const int32_t* used, cudaStream_t stream) {
   const unsigned grid = (unsigned)ceil_div(p.tiles.rows, (int64_t)(THREADS / 32 / WARPS));
-  if (p.parts == 1) prepare_kernel<THREADS, WARPS, HOLD, 1><<<grid, THREADS, 0, stream>>>(p, used);
-  else prepare_kernel<THREADS, WARPS, HOLD, 2><<<grid, THREADS, 0, stream>>>(p, used);
+  launch_link(p.parts == 1 ? prepare_kernel<THREADS, WARPS, HOLD, 1> : prepare_kernel<THREADS, WARPS, HOLD, 2>, dim3(grid),
+              dim3(THREADS), 0, stream, p, used);
 }
 // Two warps per row where the rows fill the machine (32768 rows of 2048 columns: 65 us, one warp with four pieces per lane
 // 80); else a block per row, one piece per thread as far as that goes (32 rows of 11008 columns: 14 us with 128
