@@ -17,8 +17,8 @@
 // next tile is computed in the other; behind them are two to four slots of 2 x 32 columns for decoded chunks.  A step is one
 // chunk of each half of the columns, in a fixed order: equal inputs give equal bits.
 //
-// What bounds it: 2048 rows of bf16 x 11008 x 4096 take 213 us, of which the product kernel has 197 with the tensor pipe 42 %
-// and issue 44 % busy, and no memory above a quarter.  With two slots the decoding of a step and its products do not
+// What bounds it: 2048 rows of bf16 x 11008 x 4096 take 213 us, of which the product kernel has 197 with the tensor pipe
+// 42 % and issue 44 % busy, and no memory above a quarter.  With two slots the decoding of a step and its products do not
 // fully overlap: without the decoding 176 us, without the epilogue 185, without both 145.  With short sums the epilogue
 // shows: 32768 pairs of experts of 2048 x 1024 take 850 us, without it 667; its stores of 32 rows of a format touch 11.5
 // sectors each, and an SM passes about one per clock.  Measured and dropped: sixteen decoding warps (the same); the
