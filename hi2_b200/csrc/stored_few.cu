@@ -87,10 +87,11 @@ struct Ring {
   uint32_t phase;
 };
 
-// `count` chunks against the activations at x.  False when a wait ran out.
+// `count` chunks against the activations at x, whose powers of two are s0 and s1 for the lane's two rows of the result.  One
+// part: added to acc as they are.  Two: added with their powers of two.  False when a wait ran out.
 template <int PARTS, int NBITS, bool SMALL, typename REFILL>
 __device__ __forceinline__ bool multiply(Ring& ring, const __half* x, int count, int first_word, int pair_unit, const LaneRows& rows,
-                                         float (&acc)[2][4], volatile uint32_t* abort, int32_t* status, const REFILL& refill) {
+                                         float s0, float s1, float (&acc)[2][4], volatile uint32_t* abort, int32_t* status, const REFILL& refill) {
   constexpr int PER_COPY = 8 / NBITS;
   while (count > 0) {
     if (!__all_sync(0xffffffffu, bar_wait(ring.full + ring.stage, ring.phase, abort, status))) return false;
@@ -121,7 +122,7 @@ __device__ __forceinline__ bool multiply(Ring& ring, const __half* x, int count,
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[m][q] = PARTS == 1 ? sum[m][q] : acc[m][q] + sum[m][q];
+        for (int q = 0; q < 4; ++q) acc[m][q] = PARTS == 1 ? sum[m][q] : acc[m][q] + sum[m][q] * (q & 1 ? s1 : s0);
     }
     count -= here;
     __syncwarp();  // every lane has read the stage
@@ -272,17 +273,19 @@ few_kernel(const Product p, const int split, const int runs) {
       for (int sub = 0; sub < here; ++sub) {
         const int chunks = b0 + sub == blocks - 1 ? last_chunks : BLOCK_CHUNKS, half0 = b0 + sub == blocks - 1 ? last_half0 : HALF_CHUNKS;
         // ---- this warp's chunks of a block; lanes without a row of their own read the last one's
-        float acc[2][4];
+        const float s0 = sm.scale[half][sub * tokens + min(2 * t, tokens - 1)], s1 = sm.scale[half][sub * tokens + min(2 * t + 1, tokens - 1)];
+        float block_sum[2][4];
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][i] = 0.0f;
+          for (int i = 0; i < 4; ++i) block_sum[m][i] = 0.0f;
+        float (&acc)[2][4] = PARTS == 1 ? block_sum : total;
         const int first = half == 0 ? 0 : half0, count = half == 0 ? half0 : chunks - half0;
         if (ok) {  // one loop per code width
           const __half* x = xs + (sub * tokens + min(g, tokens - 1)) * X_PITCH + first * CHUNK + 16 * t;
           const auto run = [&](auto nbits, auto small) {
-            return multiply<PARTS, decltype(nbits)::value, decltype(small)::value>(ring, x, count, first_word, pair_unit, rows, acc, &sm.abort,
-                                                                                       status, refill);
+            return multiply<PARTS, decltype(nbits)::value, decltype(small)::value>(ring, x, count, first_word, pair_unit, rows, s0, s1, acc,
+                                                                                   &sm.abort, status, refill);
           };
           typedef std::integral_constant<int, 2> Int2;
           typedef std::integral_constant<int, 4> Int4;
@@ -291,9 +294,8 @@ few_kernel(const Product p, const int split, const int runs) {
           else if (form.width() == 2) ok = form.small_steps() ? run(Int4(), std::true_type()) : run(Int4(), std::false_type());
           else if (form.width() == 3) ok = form.small_steps() ? run(Int8(), std::true_type()) : run(Int8(), std::false_type());
         }
-        const float s0 = sm.scale[half][sub * tokens + min(2 * t, tokens - 1)], s1 = sm.scale[half][sub * tokens + min(2 * t + 1, tokens - 1)];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int m = 0; m < 2 && PARTS == 1; ++m) {
           total[m][0] += acc[m][0] * s0, total[m][1] += acc[m][1] * s1;
           total[m][2] += acc[m][2] * s0, total[m][3] += acc[m][3] * s1;
         }
