@@ -33,16 +33,17 @@ def on_device(what: str, dev: torch.device, *tensors) -> None:
 
 
 def rows_of(x: torch.Tensor, k: int, what: str):
-    """``(x as [tokens, k] with unit column stride, its dtype's number)``; a copy only where the strides ask for one."""
+    """``(x as [tokens, k] with unit column stride, its row stride, its dtype's number)``; a copy only where the strides
+    ask for one."""
     dtype = DTYPES.get(x.dtype)
     if dtype is None:
         raise ValueError(f"{what}: unsupported dtype {x.dtype}")
-    if x.dim() == 2 and x.shape[1] == k:
-        return (x if x.stride(1) == 1 else x.contiguous()), dtype
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"{what}: the last dimension must be {k}, got shape {tuple(x.shape)}")
-    x = x.reshape(-1, k)
-    return (x if x.stride(1) == 1 else x.contiguous()), dtype
+    if x.dim() != 2 or x.shape[1] != k:
+        if x.dim() < 1 or x.shape[-1] != k:
+            raise ValueError(f"{what}: the last dimension must be {k}, got shape {tuple(x.shape)}")
+        x = x.reshape(-1, k)
+    ld, unit = x.stride()
+    return (x, ld, dtype) if unit == 1 else (x.contiguous(), k, dtype)
 
 
 def output_rows(out, shape, like: torch.Tensor, what: str):

@@ -180,7 +180,7 @@ def stored_linear(x: torch.Tensor, w: StoredWeight, bias: torch.Tensor | None = 
     if len(w.shape) != 2:
         raise ValueError("stored_linear: a stack of experts goes through moe.stored_experts")
     act = activation_number(activation)
-    rows, dtype = rows_of(x, w.k, "stored_linear")
+    rows, ldx, dtype = rows_of(x, w.k, "stored_linear")
     dev = w.device
     on_device("stored_linear", dev, x, bias, residual, out)
     no_gradient("stored_linear", x, bias, residual, out)
@@ -195,8 +195,10 @@ def stored_linear(x: torch.Tensor, w: StoredWeight, bias: torch.Tensor | None = 
         if residual.shape != shape or residual.dtype != x.dtype:
             raise ValueError(f"stored_linear: residual must have shape {shape} and dtype {x.dtype}")
         res = residual if len(shape) == 2 else residual.reshape(-1, n)
-        res = res if res.stride(1) == 1 else res.contiguous()
-        res_ptr, ld_res = res.data_ptr(), res.stride(0)
+        ld_res, unit = res.stride()
+        if unit != 1:
+            res, ld_res = res.contiguous(), n
+        res_ptr = res.data_ptr()
     if out is None:
         out = x.new_empty(shape)
         ld_out = n
@@ -215,7 +217,7 @@ def stored_linear(x: torch.Tensor, w: StoredWeight, bias: torch.Tensor | None = 
     if tokens > FEW_TOKENS:
         need = _lib.load().hi2_stored_linear_workspace_bytes(w.arg, dtype, tokens)
         space, at = workspace(need, dev)
-    _lib.launch("hi2_stored_linear", dev.index, w.arg, rows.data_ptr(), dtype, tokens, rows.stride(0),
+    _lib.launch("hi2_stored_linear", dev.index, w.arg, rows.data_ptr(), dtype, tokens, ldx,
                 None if bias is None else bias.data_ptr(), act, res_ptr, ld_res, out.data_ptr(), ld_out, at, need)
     return out
 

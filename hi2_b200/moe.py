@@ -235,7 +235,7 @@ def route(logits: torch.Tensor, top_k: int, scores: str = "softmax", bias: torch
     if logits.dim() < 1:
         raise ValueError("route: logits must have a dimension of experts")
     experts = logits.shape[-1]
-    rows, dtype = rows_of(logits, experts, "route")
+    rows, ld, dtype = rows_of(logits, experts, "route")
     dev = logits.device
     if not logits.is_cuda or bias is not None:
         _lib.need_cuda(logits, bias)
@@ -252,7 +252,7 @@ def route(logits: torch.Tensor, top_k: int, scores: str = "softmax", bias: torch
     shape = (*logits.shape[:-1], top_k)
     index = logits.new_empty(shape, dtype=torch.int64)
     weight = logits.new_empty(shape, dtype=torch.float32)
-    _lib.launch("hi2_route", dev.index, rows.data_ptr(), dtype, rows.shape[0], experts, rows.stride(0), top_k, sigmoid, bias_ptr, groups,
+    _lib.launch("hi2_route", dev.index, rows.data_ptr(), dtype, rows.shape[0], experts, ld, top_k, sigmoid, bias_ptr, groups,
                 groups if top_groups is None else top_groups, 1 if renormalise else 0, scale, index.data_ptr(), weight.data_ptr())
     return index, weight
 
@@ -270,7 +270,7 @@ def stored_experts(x: torch.Tensor, index: torch.Tensor, weight: torch.Tensor, g
             gate_up.rows != 2 * down.k):
         raise ValueError(f"stored_experts: stacks {gate_up.shape} and {down.shape} are not the gate/up and down of one layer")
     act = activation_number(activation)
-    rows, dtype = rows_of(x, gate_up.k, "stored_experts")
+    rows, ldx, dtype = rows_of(x, gate_up.k, "stored_experts")
     dev = gate_up.device
     on_device("stored_experts", dev, x, index, weight, out)
     if down.device != dev:
@@ -296,7 +296,7 @@ def stored_experts(x: torch.Tensor, index: torch.Tensor, weight: torch.Tensor, g
             apart("stored_experts", name, t.view(tokens, top_k), y)
     need = _lib.load().hi2_stored_experts_workspace_bytes(gate_up.arg, dtype, tokens, top_k)
     space, at = workspace(need, dev)
-    _lib.launch("hi2_stored_experts", dev.index, gate_up.arg, down.arg, rows.data_ptr(), dtype, tokens, rows.stride(0), index.data_ptr(),
+    _lib.launch("hi2_stored_experts", dev.index, gate_up.arg, down.arg, rows.data_ptr(), dtype, tokens, ldx, index.data_ptr(),
                 weight.data_ptr(), top_k, act, out.data_ptr(), ld_out, at, need)
     return out
 
