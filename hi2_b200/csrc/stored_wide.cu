@@ -22,7 +22,7 @@
 // fully overlap: without the decoding 176 us, without the epilogue 185, without both 145.  With short sums the epilogue
 // shows: 32768 pairs of experts of 2048 x 1024 take 850 us, without it 667; its stores of 32 rows of a format touch 11.5
 // sectors each, and an SM passes about one per clock.  Measured and dropped: sixteen decoding warps (the same); the
-// outputs turned to column order in shared memory first (213 -> 209 and 850 -> 910: the extra exchange costs four
+// outputs turned to column order in shared memory first (213 -> 209 us and 850 -> 910: the extra exchange costs four
 // warps more than the sectors); eight epilogue warps (96 registers, which spill).
 //
 // Every mbarrier wait is bounded by a clock limit and raises *status.
