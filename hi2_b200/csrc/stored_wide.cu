@@ -39,6 +39,9 @@ namespace {
 constexpr int DECODE_WARPS = 8, X_WARP = 8, MMA_WARP = 9, FIRST_EPILOGUE = 10, EPILOGUE_WARPS = 4;
 constexpr int THREADS = 32 * (FIRST_EPILOGUE + EPILOGUE_WARPS);
 constexpr int MAX_WIDTH = 192, MAX_EXACT_WIDTH = 128;
+// Columns of a product for that many activation rows: with A in tensor memory a pair of blocks takes 32, 64, .. of them.
+__host__ __device__ constexpr int product_columns(int rows) { return (rows + 31) & ~31; }
+static_assert(MAX_WIDTH % 32 == 0 && MAX_EXACT_WIDTH % 32 == 0, "tiles are whole steps of a product's columns");
 constexpr int EXACT_STEPS = 1;  // of a sum that the tensor cores form for an fp32 result
 constexpr int MAX_SLOTS = 4, A_COLUMNS = CHUNK / 2, SLOT_COLUMNS = 2 * A_COLUMNS;
 constexpr int RING_STAGES = 2, RING_BYTES = 3 * 1024;  // a stage: four chunks of INT2, two of INT4, one of INT8
@@ -243,7 +246,7 @@ __device__ __forceinline__ bool empty_steps(Decoder& d, int chunks, int count) {
 }
 
 struct Shape {
-  int width;       // activation rows of a tile, a multiple of 16
+  int width;       // activation rows of a tile, a multiple of 32
   int x_stages;
   int slots;       // of decoded chunks
   int splits;      // slices of the columns
@@ -380,7 +383,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
   cluster_sync();  // the peer's barriers exist before anything signals them
   fence_after();
   const uint32_t tmem = ctl->tmem_base;
-  const uint32_t d_columns = (uint32_t)(shape.width + 31) & ~31u;
+  const uint32_t d_columns = (uint32_t)shape.width;
   const uint32_t s_tmem = tmem + 2 * d_columns;  // behind the two accumulators: sums of several, for fp32 results
   const uint32_t a_tmem = s_tmem + (EXACT ? d_columns : 0);
   const int64_t first_item = blockIdx.x >> 1, stride = gridDim.x >> 1;
@@ -443,7 +446,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
     int stage = 0;
     uint32_t phase = 1;
     for (int64_t at = first_item; ok && get_item(p, shape, at, rank, item); at += stride) {
-      const int cols = (item.tile.end - item.tile.begin + 15) & ~15;  // of the product
+      const int cols = product_columns(item.tile.end - item.tile.begin);
       const int y = item.tile.begin + (int)rank * (cols / 2);
       const int second = second_chunks(shape, item);
       for (int i = 0; i < item.count; ++i) {
@@ -472,7 +475,7 @@ wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shap
     int stage = 0, slot = 0, buf = 0;
     uint32_t phase = 0, slot_phase = 0, d_phase = 1;
     for (int64_t at = first_item; ok && get_item(p, shape, at, rank, item); at += stride) {
-      const int cols = (item.tile.end - item.tile.begin + 15) & ~15;
+      const int cols = product_columns(item.tile.end - item.tile.begin);
       // fp16 operands (format 0 at bits 7 and 10), fp32 accumulator (1 << 4), N >> 3 at bit 17, M >> 4 at bit 24
       const uint32_t idesc = (1u << 4) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(2 * TILE_ROWS >> 4) << 24);
       const int second = second_chunks(shape, item);
@@ -645,7 +648,7 @@ int wide_splits(int64_t k, int64_t rows_of_tensor, int64_t max_tiles, bool stack
 
 int wide_width(int64_t rows, bool exact) {
   const int64_t tiles = ceil_div(rows, (int64_t)(exact ? MAX_EXACT_WIDTH : MAX_WIDTH));
-  return (int)(ceil_div(ceil_div(rows, tiles), (int64_t)16) * 16);
+  return product_columns((int)ceil_div(rows, tiles));
 }
 
 int product_wide(const Product& p, cudaStream_t stream, const char* what) {
@@ -656,7 +659,7 @@ int product_wide(const Product& p, cudaStream_t stream, const char* what) {
   const int stage_bytes = 2 * p.parts * (s.width / 2) * CHUNK * 2;
   s.x_stages = 144 * 1024 / stage_bytes;  // at least three
   if (s.x_stages > MAX_X_STAGES) s.x_stages = MAX_X_STAGES;
-  s.slots = (512 - (p.exact ? 3 : 2) * ((s.width + 31) & ~31)) / SLOT_COLUMNS;  // at least two
+  s.slots = (512 - (p.exact ? 3 : 2) * s.width) / SLOT_COLUMNS;  // at least two
   if (s.slots > MAX_SLOTS) s.slots = MAX_SLOTS;
   s.chunks = (int)(p.w.k / CHUNK), s.half0 = (s.chunks + 1) / 2;
   s.row_pairs = (int)((p.w.groups_per_expert / 4 + 1) / 2);
