@@ -80,7 +80,7 @@ def _lay_out_on(f: dict, experts: int, rows: int, k: int, stacked: bool, dev: to
     code_off, param_off = up("code_off", torch.int32), up("param_off", torch.int32)
     nbits, block = up("row_nbits", torch.int64), up("row_block", torch.int64)
     consts = _lib.upload(f["row_consts"], dev, torch.float16).reshape(-1, 3)
-    had = up("had", torch.uint8)
+    had = up("had", torch.uint8).clone()  # (every other field is made anew below)
     total = experts * rows
     for name, t, n in (("row_nbits", nbits, total), ("row_block", block, total), ("row_consts", consts, 3 * total),
                        ("code_off", code_off, total + 1), ("param_off", param_off, total + 1),
@@ -139,7 +139,7 @@ def _lay_out_on(f: dict, experts: int, rows: int, k: int, stacked: bool, dev: to
         return torch.where(t >= 2**31, t - 2**32, t).to(torch.int32).contiguous()
 
     tensors = dict(data=torch.zeros(max(total_units, 1) * 16, dtype=torch.uint8, device=dev),
-                   groups=words(torch.stack([base, form], 1)), rows=words(rows_t), had=had.contiguous(),
+                   groups=words(torch.stack([base, form], 1)), rows=words(rows_t), had=had,
                    inv_scale=None if scale is None else scale.reciprocal(),
                    status=torch.zeros(1, dtype=torch.int32, device=dev))
     w = StoredWeight((experts, rows, k), stacked, tensors)

@@ -1,0 +1,50 @@
+"""What a laid-out weight keeps, and what it shares with nobody."""
+
+import dataclasses
+
+import pytest
+import torch
+
+from hi2_b200 import linear, moe, stack
+from tests.stored_helpers import packed
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+FIELDS = ("codes", "code_off", "blk_params", "param_off", "row_consts", "row_nbits", "row_block", "had", "col_scale")
+
+
+def _overwrite(t):
+    t.copy_(torch.where(t == 0, torch.ones_like(t), torch.zeros_like(t)))
+
+
+def test_a_laid_out_tensor_keeps_nothing_of_its_source():
+    t = packed(150, 192, 3)
+    t = dataclasses.replace(t, **{f: getattr(t, f).to(DEV) for f in FIELDS})
+    w = linear.lay_out(t)
+    x = torch.randn(5, 192, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+    want = linear.stored_linear(x, w)
+    for f in FIELDS:
+        _overwrite(getattr(t, f))
+        assert torch.equal(linear.stored_linear(x, w), want), f
+
+
+def test_a_laid_out_stack_keeps_nothing_of_its_source():
+    def part(like, rows, k, seed):
+        t = packed(rows, k, seed)
+        if like is not None:
+            t.had, t.col_scale = like.had, like.col_scale
+        return t
+
+    gates = [part(None, 64, 128, e) for e in range(3)]
+    arrays = (stack.build_stack([[g, part(g, 64, 128, 10 + e)] for e, g in enumerate(gates)]),
+              stack.build_stack([[part(None, 128, 64, 20 + e)] for e in range(3)]))
+    arrays = [{name: t.to(DEV) for name, t in a.items()} for a in arrays]
+    gu, dn = linear.lay_out_stack(arrays[0], 2), linear.lay_out_stack(arrays[1], 1)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x, index = torch.randn(7, 128, generator=g, device=DEV), torch.randint(0, 3, (7, 2), generator=g, device=DEV)
+    weight = torch.rand(7, 2, generator=g, device=DEV)
+    want = moe.stored_experts(x, index, weight, gu, dn)
+    for a in arrays:
+        for name, t in a.items():
+            _overwrite(t)
+            assert torch.equal(moe.stored_experts(x, index, weight, gu, dn), want), name
