@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -22,6 +23,10 @@ def no_gradient(what: str, *tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{what}: there is no gradient; call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:  # inside a dual level, which no_grad() does not end
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{what}: there is no derivative; give it the primal of a dual tensor")
 
 
 def on_device(what: str, dev: torch.device, *tensors) -> None:
