@@ -33,7 +33,9 @@ class _Struct(C.Structure):  # hi2_stored_weight
 
 class StoredWeight:
     """Packed rows laid out for products: ``shape`` is ``(rows, K)``, or ``(experts, rows, K)`` for a stack.
-    Made by :func:`lay_out` or :func:`lay_out_stack`; read-only, and usable on any stream of its device."""
+    Made by :func:`lay_out` or :func:`lay_out_stack`; read-only, and usable on any stream of its device.  Its memory
+    belongs to the stream that was current then: before the last reference goes while calls on OTHER streams may still
+    be queued, :meth:`record_stream` them (as for a tensor) or wait for them.  A captured graph does not keep it alive."""
 
     def __init__(self, shape, stacked: bool, tensors: dict):
         experts, rows, k = shape
@@ -50,6 +52,12 @@ class StoredWeight:
     @property
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in self._tensors.values() if t is not None)
+
+    def record_stream(self, stream: torch.cuda.Stream) -> None:
+        """Keep the memory from being handed out again before what is queued on ``stream`` by the time the weight goes has run."""
+        for t in self._tensors.values():
+            if t is not None:
+                t.record_stream(stream)
 
     def check(self) -> None:
         """Raise ``RuntimeError`` if a device-side wait of a product with this weight ever ran out (waits

@@ -48,3 +48,26 @@ def test_a_laid_out_stack_keeps_nothing_of_its_source():
         for name, t in a.items():
             _overwrite(t)
             assert torch.equal(moe.stored_experts(x, index, weight, gu, dn), want), name
+
+
+def test_memory_of_a_weight_in_use_on_another_stream():
+    w = linear.lay_out(packed(4096, 1024, 5, [(8, 16)]), DEV)
+    x = torch.randn(4, 1024, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    want = linear.stored_linear(x, w)
+    torch.cuda.synchronize()
+    tensors = [t for t in w._tensors.values() if t is not None]
+    ranges = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors]
+    del tensors
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)  # some 0.2 s
+        y = linear.stored_linear(x, w)
+    w.record_stream(side)
+    del w
+    new = [torch.empty(hi - lo, dtype=torch.uint8, device=DEV) for lo, hi in ranges for _ in range(3)]
+    assert not side.query()
+    for t in new:  # nothing of it is handed out while the call waits
+        for lo, hi in ranges:
+            assert t.data_ptr() >= hi or t.data_ptr() + t.numel() <= lo
+    side.synchronize()
+    assert torch.equal(y, want)
