@@ -62,6 +62,7 @@ class StoredWeight:
     def check(self) -> None:
         """Raise ``RuntimeError`` if a device-side wait of a product with this weight ever ran out (waits
         for the device; products themselves never wait)."""
+        torch.cuda.synchronize(self.device)  # calls on every stream
         if int(self._status.item()):
             raise RuntimeError("stored product: a bounded device-side wait ran out; results since then are not valid")
 

@@ -5,7 +5,7 @@ import dataclasses
 import pytest
 import torch
 
-from hi2_b200 import linear, moe, stack
+from hi2_b200 import _lib, linear, moe, stack
 from tests.stored_helpers import packed
 
 pytestmark = pytest.mark.gpu
@@ -64,10 +64,38 @@ def test_memory_of_a_weight_in_use_on_another_stream():
         y = linear.stored_linear(x, w)
     w.record_stream(side)
     del w
-    new = [torch.empty(hi - lo, dtype=torch.uint8, device=DEV) for lo, hi in ranges for _ in range(3)]
-    assert not side.query()
-    for t in new:  # nothing of it is handed out while the call waits
+    try:
+        new = [torch.empty(hi - lo, dtype=torch.uint8, device=DEV) for lo, hi in ranges for _ in range(3)]
+        waiting = not side.query()
+    finally:
+        side.synchronize()  # before anything else is allocated: a product must not meet tables that somebody wrote over
+    assert waiting
+    for t in new:  # nothing of it was handed out while the call waited
         for lo, hi in ranges:
             assert t.data_ptr() >= hi or t.data_ptr() + t.numel() <= lo
-    side.synchronize()
     assert torch.equal(y, want)
+
+
+def test_check_reports_a_wait_that_ran_out():
+    """The status word as a kernel raises it, set from the host: nothing on the device has to wait for it."""
+    gu = linear.lay_out_stack(stack.build_stack([[packed(64, 64, e), packed(64, 64, e)] for e in range(2)]), 2, DEV)
+    for w in (linear.lay_out(packed(70, 64, 1), DEV), gu):
+        w.check()
+        w._status.fill_(_lib.ERR_TIMEOUT)
+        for _ in range(2):  # nothing clears it
+            with pytest.raises(RuntimeError, match="ran out"):
+                w.check()
+
+
+def test_check_waits_for_every_stream():
+    w = linear.lay_out(packed(70, 64, 1), DEV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)  # some 0.2 s
+        w._status.fill_(_lib.ERR_TIMEOUT)
+    try:
+        with pytest.raises(RuntimeError, match="ran out"):
+            w.check()
+    finally:
+        side.synchronize()
