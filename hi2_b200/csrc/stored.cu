@@ -99,7 +99,8 @@ prepare_kernel(const Product p, const int32_t* __restrict__ used) {
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) top = fmaxf(top, warp_top[i]);
   }
-  const PowerOfTwo power = power_for(top);
+  // (the power of a row that a (token, slot) pair's weight follows is multiplied by it: room for 16 bits below)
+  const PowerOfTwo power = power_for(top, p.out.pair_weight != nullptr ? -110 : -126);
   if (lane == 0) p.row_scale[row] = power.back;
   auto store = [&](int g, const float (&x)[16]) {
     uint4 hi[2], lo[2];

@@ -243,15 +243,16 @@ __device__ __forceinline__ float largest(const float (&v)[16]) {
   for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(v[i]));
   return top;
 }
-// The power of two that takes `top` to [2^14, 2^15); values without a size, or with an infinity, stay as they are.
+// The power of two that takes `top` to [2^14, 2^15); values without a size, or with an infinity, stay as they are.  It stops
+// at 2^`lowest`, so that both directions are normal fp32 numbers.
 struct PowerOfTwo {
   float to, back;
 };
-__device__ __forceinline__ PowerOfTwo power_for(float top) {
+__device__ __forceinline__ PowerOfTwo power_for(float top, int lowest = -126) {
   const int biased = (int)(__float_as_uint(top) >> 23);
   int e = biased - 127 - 14;
   if (top == 0.0f || biased == 255) e = 0;
-  if (e < -110) e = -110;  // 2^-e has to be an fp32 number
+  if (e < lowest) e = lowest;
   return PowerOfTwo{__uint_as_float((uint32_t)(127 - e) << 23), __uint_as_float((uint32_t)(127 + e) << 23)};
 }
 // The fp16 parts of 16 values times `to`, as two 16-byte words each.
