@@ -8,6 +8,8 @@ from torch.autograd import forward_ad
 
 from hi2_b200 import _lib
 from hi2_b200._args import no_gradient
+from tests.stored_accuracy import SIZES, check_product, form_of
+from tests.stored_helpers import DTYPES, packed, turned
 
 
 @pytest.mark.parametrize("exact,widest", [(False, 192), (True, 128)])
@@ -35,3 +37,34 @@ def test_dual_tensors_are_refused():
             no_gradient("op", x, dual)
     with pytest.raises(ValueError, match="no derivative"):
         torch.func.jvp(lambda v: no_gradient("op", v), (x,), (torch.ones(3),))
+
+
+@pytest.mark.parametrize("rows,k,tokens", [(64, 65536, 8), (96, 34816, 2), (200, 1024, 33), (96, 4160, 70)])
+def test_error_limits_reject_what_is_lost(rows, k, tokens):
+    """The limits that the products are held to on the device, met by a rounded result and not by one with a defect."""
+    t = packed(rows, k, rows + tokens)
+    g = torch.Generator().manual_seed(tokens)
+    v = 0.05 * torch.randn(rows, k, generator=g, dtype=torch.float64)
+    x = turned(torch.randn(tokens, k, generator=g).double() * torch.exp(0.5 * torch.randn(k, generator=g)), t)
+    want, size = x @ v.T, ((x * x) @ (v * v).T).sqrt()
+    for dtype in DTYPES.values():
+        check_product(want.to(dtype), want, size, dtype)
+        without = x.clone()
+        without[:, -64:] = 0  # a chunk of columns
+        with pytest.raises(AssertionError):
+            check_product((without @ v.T).to(dtype), want, size, dtype)
+        with pytest.raises(AssertionError):
+            check_product(torch.zeros_like(want).to(dtype), want, size, dtype)
+    one_part = x.half().double()
+    check_product((one_part @ v.T).bfloat16(), want, size, torch.bfloat16)
+    with pytest.raises(AssertionError):
+        check_product((one_part @ v.T).float(), want, size, torch.float32)
+    with pytest.raises(AssertionError):  # truncated towards zero all along 2048 columns
+        check_product((want * (1 - 2e-6)).float(), want, size, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+def test_sizes_cover_every_form(dtype):
+    forms = [(form_of(*size, DTYPES[dtype]), size[1]) for size in SIZES]
+    for form in ("few", "sliced", "whole"):
+        assert sum(f == form and k >= 4096 for f, k in forms) >= 2, (form, forms)
