@@ -1,0 +1,61 @@
+"""Dispatch of many (token, slot) pairs and many experts: passes of the counting loop, sums over many warps of experts,
+experts without pairs and experts with nearly all of them."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from hi2_b200 import linear, moe
+from hi2_b200.format import dequantize_stored
+from tests.stored_helpers import DTYPES, experts64, packed, within
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HIDDEN = INNER = 64
+
+
+def _stack(experts, rows, k, parts, seed):
+    """A stack cut out of one packed tensor, with a transform for every expert."""
+    t = packed(experts * rows, k, seed)
+    g = torch.Generator().manual_seed(seed)
+    arrays = {f: getattr(t, f) for f in ("codes", "code_off", "blk_params", "param_off", "row_consts", "row_nbits", "row_block")}
+    arrays["had"] = (torch.rand(experts, k // 16, generator=g) < 0.7).to(torch.uint8)
+    arrays["col_scale"] = torch.exp(0.5 * torch.randn(experts, k, generator=g)).half()
+    arrays["part_off"] = rows // parts * torch.arange(parts * experts + 1, dtype=torch.int32)
+    values = dequantize_stored(t, DEV).view(experts, rows, k)
+    had, scale = arrays["had"].to(DEV), arrays["col_scale"].to(DEV)
+    return linear.lay_out_stack(arrays, parts, DEV), [(SimpleNamespace(had=had[e], col_scale=scale[e]), values[e]) for e in range(experts)]
+
+
+def _choice(kind, tokens, experts, top_k, g):
+    if kind == "spread":
+        return torch.stack([torch.randperm(experts, generator=g, device=DEV)[:top_k] for _ in range(tokens)])
+    index = torch.randint(0, experts, (tokens, top_k), generator=g, device=DEV)
+    if kind == "one":  # nearly everybody takes the last expert
+        index[torch.rand(index.shape, generator=g, device=DEV) < 0.95] = experts - 1
+    else:  # few experts with pairs, and most slots without one
+        index = index // 97 * 97
+        index[torch.rand(index.shape, generator=g, device=DEV) < 0.8] = -1
+    return index
+
+
+@pytest.mark.parametrize("dtype", sorted(DTYPES))
+@pytest.mark.parametrize("experts,top_k,tokens,kind", [(64, 8, 1024, "spread"), (64, 8, 1025, "spread"), (64, 8, 2500, "spread"), (200, 8, 300, "spread"),
+                                                       (1024, 8, 64, "spread"), (1024, 8, 3000, "spread"), (1024, 1, 1, "spread"),
+                                                       (64, 2, 10000, "one"), (1000, 4, 3000, "one"), (1024, 8, 5000, "holes"), (33, 8, 700, "holes")])
+def test_many_pairs_and_many_experts(experts, top_k, tokens, kind, dtype):
+    dt = DTYPES[dtype]
+    gu, gate_up = _stack(experts, 2 * INNER, HIDDEN, 2, 7)
+    dn, down = _stack(experts, HIDDEN, INNER, 1, 8)
+    g = torch.Generator(device=DEV).manual_seed(tokens)
+    index = _choice(kind, tokens, experts, top_k, g)
+    weight = torch.rand(index.shape, generator=g, device=DEV)
+    x = torch.randn(tokens, HIDDEN, generator=g, device=DEV).to(dt)
+    y = moe.stored_experts(x, index, weight, gu, dn)
+    want, bound = experts64(x, index, weight, gate_up, down, dt)
+    within(y, want, bound)
+    if dt == torch.float32:
+        assert (y - want).norm() < 2.0**-19 * want.norm()
+    assert torch.equal(y, moe.stored_experts(x, index, weight, gu, dn))
+    gu.check(), dn.check()
