@@ -67,12 +67,20 @@ class ChainGraph {
 
 // Launch of a link of a chain of short kernels: the kernel may be set up while its predecessor in the
 // stream still runs (programmatic dependent launch; in a captured chain the edge is a programmatic
-// one).  Every such kernel calls chain_wait() before it touches global memory, which returns once the
-// predecessor has finished and its writes are visible; since every link waits for the one before it,
-// order along the stream is kept for whatever follows.  A predecessor calls chain_next() when all that
+// one).  chain_wait() returns once the predecessor has finished and its writes are visible.  What a link keeps to:
+//  - before its chain_wait() it reads only what was complete when its predecessor released its dependents, and writes no global
+//    memory.  That is what the predecessor itself had waited for before its chain_next() (so every link waits first and
+//    releases afterwards), what lies before a plain launch in the stream, and memory that no queued kernel writes, such as a laid-out weight
+//    (its layout has been waited for on the host).
+//  - it does not end before its predecessor has: some thread of it waits.  Only then does order along the stream hold
+//    for whatever follows the chain.  A block may leave early where it has nothing to do; if ALL blocks do, then the
+//    predecessor's blocks must have had nothing to do either (blocks without a tile in the routed experts' products: both
+//    products go by the same list).
+// A predecessor whose successor's blocks are large calls chain_next() when all that
 // is left to it is its stores: the successor's thread blocks hold their registers and shared memory
 // while they wait, and set up any earlier they kept other streams' kernels off the SMs (a decoder layer
-// with its tables and factor chains side by side 53.6 -> 58.6 ms).
+// with its tables and factor chains side by side 53.6 -> 58.6 ms).  The products with packed weights call it as soon as
+// they have waited: their successors set up and ask for packed rows meanwhile.
 template <typename... Params, typename... Args>
 inline void launch_link(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t config = {};

@@ -61,7 +61,7 @@ template <int THREADS, int WARPS, int HOLD, int PARTS>
 __global__ void __launch_bounds__(THREADS)
 prepare_kernel(const Product p, const int32_t* __restrict__ used) {
   chain_wait();
-  chain_next();  // the product sets up and decodes its first chunks meanwhile
+  chain_next();  // the product sets up and decodes its first chunks meanwhile; never before the wait: it goes by the tile list at once
   constexpr int TEAM = WARPS * 32;
   const int team = threadIdx.x / TEAM, lane = threadIdx.x % TEAM;
   const int64_t row = (int64_t)blockIdx.x * (THREADS / TEAM) + team;
@@ -146,7 +146,9 @@ int prepare(const Product& p, const int32_t* used, cudaStream_t stream) {
 // ---- dispatch -----------------------------------------------------------------------------------------
 // Counting sort of the (token, slot) pairs by expert: one block counts and makes the list of token tiles, then many place
 // the pairs.  Pairs of one expert come in no particular order: a row's result does not depend on its place, so the outputs
-// are the same every time.  (One block for both, keeping the order by matching the lanes of a warp, took 36 us for 32768
+// are the same every time.  The products read the index and the tile list before they
+// wait for the kernel ahead of them: both kernels here must have ended before that one releases its dependents, as it does after a
+// wait of its own.  (One block for both, keeping the order by matching the lanes of a warp, took 36 us for 32768
 // pairs, without the order 26 us: its scattered stores all go through one SM.)
 constexpr int SORT_THREADS = 1024, SORT_BATCH = 8;
 constexpr int MAX_EXPERTS = 1024;

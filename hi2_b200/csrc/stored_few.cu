@@ -210,7 +210,7 @@ few_kernel(const Product p, const int split, const int runs) {
   const int first_word = code_word(g, t);
 
   chain_wait();  // the activations
-  chain_next();
+  chain_next();  // (after the wait: the next product may go by the index or the tile list at once)
   bool ok = true, prepared = false;
   for (;; ++row_tile) {
     LaneRows rows;

@@ -59,3 +59,44 @@ def test_many_pairs_and_many_experts(experts, top_k, tokens, kind, dtype):
         assert (y - want).norm() < 2.0**-19 * want.norm()
     assert torch.equal(y, moe.stored_experts(x, index, weight, gu, dn))
     gu.check(), dn.check()
+
+
+@pytest.mark.parametrize("tokens", [3, 40, 700])
+@pytest.mark.parametrize("before", ["copy", "fill", "join", "nothing"])
+def test_first_calls_of_a_graph(before, tokens):
+    """A captured call behind a copy from the host, a fill, a kernel on each of two streams, or as the graph's root; with a
+    call on another stream beside it."""
+    gu, _ = _stack(4, 2 * INNER, HIDDEN, 2, 9)
+    dn, _ = _stack(4, HIDDEN, INNER, 1, 10)
+    w = linear.lay_out(packed(HIDDEN, HIDDEN, 11), DEV)
+    g = torch.Generator(device=DEV).manual_seed(tokens)
+    index = torch.randint(0, 4, (tokens, 2), generator=g, device=DEV)
+    weight = torch.rand(tokens, 2, generator=g, device=DEV)
+    host = torch.randn(tokens, HIDDEN, generator=torch.Generator().manual_seed(tokens)).bfloat16().pin_memory()
+    x, residual = host.to(DEV), torch.zeros(tokens, HIDDEN, dtype=torch.bfloat16, device=DEV)
+    linear.stored_linear(x, w, residual=residual), moe.stored_experts(x, index, weight, gu, dn)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        if before == "copy":
+            x.copy_(host, non_blocking=True)
+        elif before == "fill":
+            residual.zero_()
+        elif before == "join":
+            side.wait_stream(here)
+            with torch.cuda.stream(side):
+                residual.add_(1)
+            x.mul_(1)
+            here.wait_stream(side)
+        y = linear.stored_linear(x, w, residual=residual)
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            beside = linear.stored_linear(x, w)
+        z = moe.stored_experts(x, index, weight, gu, dn)
+        here.wait_stream(side)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, linear.stored_linear(x, w, residual=residual)) and torch.equal(beside, linear.stored_linear(x, w))
+    assert torch.equal(z, moe.stored_experts(x, index, weight, gu, dn))
