@@ -100,3 +100,25 @@ def test_first_calls_of_a_graph(before, tokens):
     torch.cuda.synchronize()
     assert torch.equal(y, linear.stored_linear(x, w, residual=residual)) and torch.equal(beside, linear.stored_linear(x, w))
     assert torch.equal(z, moe.stored_experts(x, index, weight, gu, dn))
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 results, and more than 2^31 intermediate values of the routed experts."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    w = linear.lay_out(packed(28672, 64, 12), DEV)
+    x = torch.randn(80000, 64, generator=g, device=DEV).bfloat16()
+    y = linear.stored_linear(x, w)
+    assert y.numel() > 2**31
+    for rows in (slice(0, 3001), slice(74000, 77001), slice(76999, 80000)):
+        assert torch.equal(y[rows], linear.stored_linear(x[rows], w))
+    del y
+    inner, tokens = 512, 270_000
+    gu, _ = _stack(4, 2 * inner, HIDDEN, 2, 13)
+    dn, _ = _stack(4, HIDDEN, inner, 1, 14)
+    index = torch.randint(0, 4, (tokens, 8), generator=g, device=DEV)
+    weight = torch.rand(tokens, 8, generator=g, device=DEV)
+    assert tokens * 8 * 2 * inner > 2**31
+    x = torch.randn(tokens, HIDDEN, generator=g, device=DEV).bfloat16()
+    y = moe.stored_experts(x, index, weight, gu, dn)
+    for rows in (slice(0, 5000), slice(131_072, 136_000), slice(265_000, 270_000)):
+        assert torch.equal(y[rows], moe.stored_experts(x[rows], index[rows], weight[rows], gu, dn))
