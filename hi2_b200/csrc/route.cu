@@ -8,8 +8,8 @@
 // agree to the last fp32 bits must still be told apart the way their exact values are.
 //
 // What bounds it: with groups the integer pipe (64 % busy in a capture before the keys were compared as fp64, 1343 instructions
-// per token): 16384 tokens of 128 experts in 8 groups take 23.6 us (28.9 with 64-bit integer keys and a division per expert).
-// A single token takes 2.6 us, one launch.
+// per token): 16384 tokens of 128 experts in 8 groups take 24.6 us a call, 23.1 replayed (a call 28.9 with 64-bit integer keys and a division per expert).
+// A single token takes 2.5 us, one launch.
 #include <type_traits>
 
 #include "common.cuh"

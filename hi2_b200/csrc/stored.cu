@@ -5,8 +5,9 @@
 // A product is y = act(x' V^T + bias) + residual with V the format's fp16 weights, exactly as stored, and x' the
 // activations in the stored basis: divided by the smoothing vector and rotated by the order-16 Hadamard matrix
 // in the flagged groups.  x' is formed in fp32 and rounded to fp16 once, relative to a power of two that
-// takes the row's largest value to [2^14, 2^15): 11 bits for every value within 2^-29 of that.  bf16 calls
-// (8 bits) take that one part; fp16 and fp32 calls take a second part, fp16(x' - first), and twice the products.
+// takes the largest value of the row (in the kernel for few rows: of each half of a block of 1024 columns) to
+// [2^14, 2^15): 11 bits for every value within 2^-29 of that.  bf16 calls take that one part; fp16 and fp32 calls
+// take a second part, fp16(x' - first), and twice the products.
 #include <initializer_list>
 
 #include "stored.cuh"
@@ -264,10 +265,14 @@ struct Carver {
   }
 };
 
+// One part for bf16 calls: what 11 bits leave out lies below the rounding of a bf16 result.  Measured, one part / two: errors of
+// 512 tokens through experts of 1024 x 512 against 64 bits 1.69e-3 / 1.65e-3 (1.65e-3 is the rounding of the exact result);
+// 2048 tokens x 11008 x 4096 212 / 271 us, 4096 tokens through 64 experts of 2048 x 1024 870 / 1105, 64 tokens 130 / 179, one token
+// x 28672 x 8192 40 / 52.  fp16 results (11 bits themselves) would show it, fp32 results all the more.
 inline int parts_of(int dtype) { return dtype == HI2_BF16 ? 1 : 2; }
 // Which kernel takes a product: the one for few rows up to 16 of them, and as long as its tiles of eight are little work (it
 // is one launch where the other takes three).  Measured, few / wide, us (and cost): 256 tokens x 512 x 512 8.7 / 15.4
-// (24), 77 x 1001 x 1088 in fp32 11.8 / 16.9 (26), 64 x 2048 x 2048 12.8 / 17.4 (36), 24 x 4096 x 4096 19.5 / 19.0 (42),
+// (27), 77 x 1001 x 1088 in fp32 11.8 / 16.9 (29), 64 x 2048 x 2048 12.8 / 17.4 (39), 24 x 4096 x 4096 19.5 / 19.0 (45),
 // 64 x 4096 x 4096 34 / 22 (84); 111 pairs of 5 experts of 192 x 320 in fp32 25.1 / 32.8 (25).
 constexpr double FEW_COST = 40;
 inline bool few(const hi2_stored_weight& w, int64_t tokens, int parts) {

@@ -14,8 +14,8 @@
 // inside a chunk is the same permutation for both operands, so a lane's 16 columns are contiguous in memory.
 //
 // What bounds it: decoding and products share the fp16 pipe (183 clocks for 2048 INT2 weights, stored.cuh).  28672 x 8192
-// INT2 weights with one row take 41 us where streaming them alone takes 16 and the products without decoding 22; the
-// packed bytes ask for 12.  In the smallest calls it is latency: 4096 x 4096 with one row takes 7.7 us.  Measured and
+// INT2 weights with one row take 40 us where streaming them alone takes 16 and the products without decoding 22; the
+// packed bytes ask for 12.  In the smallest calls it is latency: 4096 x 4096 with one row takes 7.2 us.  Measured and
 // dropped: three stages per ring with one block per SM; the next chunk's words read ahead of the products.
 #include <type_traits>
 
@@ -368,9 +368,8 @@ int launch(const Product& p, const FewPlan& plan, cudaStream_t stream, const cha
 // Slices of the columns and runs of row tiles: what leaves the fullest SM the least work, with what a tile costs besides its
 // chunks (start of its stream, the join) counted as eight of them, three more through a cluster, and what a block costs
 // (start, activations) as twelve.  The two blocks of an SM share its pipes: a run that is longer than the mean may have a
-// shorter one beside it.  Measured, us: 28672 x 8192, one row, whole columns in 224 blocks 41.0, two slices in 148 runs 42.1, in
-// 112 runs 42.3; 64 tokens of 64 experts of 2048 x 1024 with the gate/up product in runs of six tiles 160.9, of three 167.3, of
-// one 177.1.
+// shorter one beside it.  Measured, us: 28672 x 8192, one row, whole columns in 224 blocks 39.9, two slices in 148 runs 40.8, in
+// 112 runs 41.0; 64 tokens of 64 experts of 2048 x 1024 with both products in runs of six tiles 131, of three 143, of one 172.
 FewPlan few_plan(int64_t k, int64_t row_tiles, int64_t tiles, int64_t width, int parts) {
   const int64_t chunks = k / CHUNK, room = 2 * 148;
   const int places = parts == 1 ? PLACES<1> : PLACES<2>;

@@ -17,7 +17,7 @@
 // next tile is computed in the other; behind them are two to four slots of 2 x 32 columns for decoded chunks.  A step is one
 // chunk of each half of the columns, in a fixed order: equal inputs give equal bits.
 //
-// What bounds it: 2048 rows of bf16 x 11008 x 4096 take 213 us, of which the product kernel has 197 with the tensor pipe
+// What bounds it: 2048 rows of bf16 x 11008 x 4096 take 212 us, of which the product kernel has 197 with the tensor pipe
 // 42 % and issue 44 % busy, and no memory above a quarter.  With two slots the decoding of a step and its products do not
 // fully overlap: without the decoding 176 us, without the epilogue 185, without both 145.  With short sums the epilogue
 // shows: 32768 pairs of experts of 2048 x 1024 take 850 us, without it 667; its stores of 32 rows of a format touch 11.5
@@ -350,8 +350,8 @@ __device__ __forceinline__ void put_rows(const Epilogue& out, float (&v)[16], in
 // EXACT: fp32 results.  The tensor cores' accumulator drops what does not fit it at every step, always towards zero,
 // which over 2048 columns costs 2e-6 of a result.  So a sum there covers one step of 128 columns, small parts first, and the
 // epilogue's warps add the sums up in fp32, in tensor memory of their own.  Measured (2048 rows x 11008 x 4096; error of
-// 512 tokens through experts of 1024 x 512, where a plain fp32 product has 9.6e-7): one step 399 us, 5.3e-7; two 335 us,
-// 1.4e-6; four 322 us, 3.1e-6; slices of the columns joined through memory 1361 us.
+// 512 tokens through experts of 1024 x 512, where a plain fp32 product has 9.3e-7): one step 428 us, 5.4e-7; two 345 us,
+// 1.3e-6; four 325 us, 3.0e-6; slices of the columns joined through memory 1361 us.
 template <bool EXACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 wide_kernel(const __grid_constant__ CUtensorMap map, const Product p, const Shape shape) {

@@ -4,7 +4,8 @@
 A packed tensor (or a stack of routed experts) is laid out once with :func:`lay_out` /
 :func:`lay_out_stack`; the layout keeps the packed size but for a few groups (codes and ladder parameters are re-ordered).
 :func:`stored_linear` then multiplies activations with the fp16 reconstruction, decoded on the fly, and
-applies bias, activation and residual in the same kernel; :func:`hi2_b200.moe.stored_experts` is the
+applies bias, activation and residual as it stores the sums (behind the sum of the slices, where the columns of a product
+are split); :func:`hi2_b200.moe.stored_experts` is the
 same for a mixture layer.  bf16 activations are taken to 11 bits in the stored basis, fp16 and fp32 ones to
 22; sums are held in fp32.  Inference only: activations that require a gradient are refused.
 """
