@@ -166,7 +166,8 @@ class ExpertViews(nn.Module):
     ``(hidden_states, top_k_index, top_k_weights)``.  The (token, slot) pairs are sorted by expert
     once (a stable sort keeps the token order inside an expert) and their counts read back once;
     every expert that received tokens then runs its three Linears on its own rows, gate and up on
-    the SAME gathered tensor, so hooks on them see one shared input per expert."""
+    the SAME gathered tensor, so hooks on them see one shared input per expert.  A slot whose index is not an
+    expert's (the -1 of :func:`route`) adds nothing."""
 
     def __init__(self, fused: nn.Module):
         super().__init__()
@@ -191,10 +192,10 @@ class ExpertViews(nn.Module):
         slots = top_k_index.shape[-1]
         chosen = top_k_index.reshape(-1)
         order = torch.argsort(chosen, stable=True)
-        counts = (chosen[None, :] == torch.arange(self.n_experts, device=chosen.device)[:, None]).sum(1).tolist()
+        counts = (chosen[None, :] == torch.arange(self.n_experts, device=chosen.device)[:, None]).sum(1)
+        start, *counts = torch.cat([(chosen < 0).sum()[None], counts]).tolist()  # slots without an expert come first
         share = top_k_weights.reshape(-1)
         out = torch.zeros_like(x)
-        start = 0
         for e, n in enumerate(counts):
             pairs = order[start : start + n]
             start += n

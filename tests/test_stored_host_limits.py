@@ -6,7 +6,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from hi2_b200 import _lib
+from hi2_b200 import _lib, moe
 from hi2_b200._args import no_gradient
 from tests.stored_accuracy import SIZES, check_product, form_of
 from tests.stored_helpers import DTYPES, packed, turned
@@ -68,3 +68,31 @@ def test_sizes_cover_every_form(dtype):
     forms = [(form_of(*size, DTYPES[dtype]), size[1]) for size in SIZES]
     for form in ("few", "sliced", "whole"):
         assert sum(f == form and k >= 4096 for f, k in forms) >= 2, (form, forms)
+
+
+class _Fused(torch.nn.Module):
+    def __init__(self, experts, hidden, inner):
+        super().__init__()
+        g = torch.Generator().manual_seed(0)
+        self.gate_up_proj = torch.nn.Parameter(torch.randn(experts, 2 * inner, hidden, generator=g))
+        self.down_proj = torch.nn.Parameter(torch.randn(experts, hidden, inner, generator=g))
+        self.act_fn = torch.nn.SiLU()
+
+
+@pytest.mark.parametrize("unused", [[], [3], [0, 1, 2, 3], list(range(10))])
+def test_expert_views_pass_over_unused_slots(unused):
+    """Routing leaves -1 in slots that no expert is open for; the experts over unpacked weights take its outputs too."""
+    fused, g = _Fused(3, 6, 4), torch.Generator().manual_seed(1)
+    x, weight = torch.randn(5, 6, generator=g), torch.rand(5, 2, generator=g)
+    index = torch.randint(0, 3, (5, 2), generator=g)
+    index.view(-1)[unused] = -1
+    index[4, 1] = 3 if unused else index[4, 1]  # behind the last expert
+    want = torch.zeros(5, 6, dtype=torch.float64)
+    for t, j in ((t, j) for t in range(5) for j in range(2)):
+        e = int(index[t, j])
+        if 0 <= e < 3:
+            z = fused.gate_up_proj[e].double() @ x[t].double()
+            want[t] += weight[t, j].double() * (fused.down_proj[e].double() @ (fused.act_fn(z[:4]) * z[4:]))
+    with torch.no_grad():
+        y = moe.ExpertViews(fused)(x, index, weight)
+    assert (y - want).abs().max() <= 2.0**-20 * max(want.abs().max().item(), 1.0) * 8  # fp32 sums of 6, 4 and 2 terms
